@@ -792,6 +792,75 @@ int lq_argmax_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_idx, 
 int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_idx, int32_t* d_pos, int32_t delta,
                        void* stream);
 
+/* ---- serving from a paged key-value cache ------------------------------------ */
+/* A cache in pages (no counterpart in the reference, whose decode attends a dense cache): pages
+ * k / v [pages][Hkv][page][hd] of cache_type LQ_F16, LQ_BF16 or LQ_I8 (then one float32 scale per
+ * row in [pages][Hkv][page]: value = code * scale); d_table [seqs][table_stride] of page numbers;
+ * position p of sequence s is slot p % page of page d_table[s][p / page].  d_lengths [seqs]: the
+ * positions each sequence holds, the new tokens among them.
+ *
+ * Appends packed new tokens: token t's keys at d_k + t * ld (elements of src_type LQ_F32, LQ_F16
+ * or LQ_BF16; [Hkv][hd] contiguous), its values at d_v + t * ld.  Sequence s owns tokens
+ * d_starts[s] .. d_starts[s + 1] - 1 and they become its last positions; d_starts NULL: token s is
+ * the one new token of sequence s (tokens == seqs).  A float cache gets each value rounded once
+ * to nearest even.  An int8 cache gets scale = max|x| / 127 and code = rne(x * (127 / max|x|)) per
+ * row of hd; a row with an infinity or NaN gets a scale that is not finite and reads back as
+ * NaN, one whose magnitudes are below 127 / FLT_MAX as zeros.  A token is left out when its
+ * position is negative (a sequence of length 0), lies past the table, or its page number is
+ * outside [0, pages).  Two tokens of one call must not share a place. */
+int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t ld, int64_t tokens,
+                       const int32_t* d_starts, int64_t seqs, int64_t Hkv, int64_t hd, const int32_t* d_table,
+                       int64_t table_stride, const int32_t* d_lengths, void* d_k_pages, void* d_v_pages,
+                       int cache_type, float* d_k_scale, float* d_v_scale, int64_t pages, int64_t page, void* stream);
+/* Attention of one new token per sequence: q [B][H][hd] (rows ldq apart, q_type LQ_F16 or LQ_BF16)
+ * against positions 0 .. d_lengths[b] - 1 of the cache (of q_type or LQ_I8); query head h reads
+ * key head h / (H / Hkv); softmax(scale q.k) v with float32 scores, statistics and sums; out
+ * [B][H][hd] contiguous, of q_type or LQ_F32.  A sequence of length <= 0 has the output 0, one
+ * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
+ * lengths: the split over the positions is planned from it, and lengths past it are still
+ * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and finite.
+ * Workspace: lq_paged_attention_workspace_size bytes, no contents kept from call to call. */
+size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);
+int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
+                       const void* d_k_pages, const void* d_v_pages, int cache_type, const float* d_k_scale,
+                       const float* d_v_scale, int64_t pages, int64_t page, const int32_t* d_table,
+                       int64_t table_stride, const int32_t* d_lengths, int64_t max_length, float scale, void* d_out,
+                       int out_type, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Attention over packed sequences of different lengths: sequence s has queries d_q_starts[s] ..
+ * d_q_starts[s + 1] - 1 (rows of q, ldq elements apart, heads contiguous) and keys d_k_starts[s]
+ * .. d_k_starts[s + 1] - 1 (rows of k and v).  causal != 0: query i of nq sees keys 0 .. nk - nq +
+ * i (the queries are the last of the sequence's positions); else all nk.  Query head h reads key
+ * head h / (H / Hkv).  out [total_q][H][hd] contiguous, of `type` (LQ_F16 or LQ_BF16) or LQ_F32.
+ * A query that sees no key has the output 0; rows of no sequence are not written.  Keys a query
+ * does not see never reach it, whatever they hold.  Starts never decrease and stay within the
+ * totals (rows past the totals are neither read nor written).  hd a multiple of 8, at most 256;
+ * scale positive and finite. */
+int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v, int64_t ldv,
+                        int type, const int32_t* d_q_starts, const int32_t* d_k_starts, int64_t seqs, int64_t total_q,
+                        int64_t total_k, int64_t H, int64_t Hkv, int64_t hd, int causal, float scale, void* d_out,
+                        int out_type, void* stream);
+/* Log probabilities of given tokens under rows of logits x [rows][vocab] (ldx elements apart,
+ * LQ_F32, LQ_F16 or LQ_BF16), float32 out: lse[r] = log sum_j e^x_j; logprobs[r] = x[target] - lse
+ * (0 for a target outside [0, vocab)); entropy[r] = -sum_j p_j log p_j; the `top` most likely
+ * tokens in order (ties: the lower index; NaN above everything) with their log probabilities, in
+ * [rows][top].  d_logprobs, d_entropy, d_lse may be NULL; top 0 .. 64, at most vocab.  A logit of
+ * -inf is a token that is not allowed (probability 0); a row without any allowed token has lse =
+ * -inf, entropy 0 and log probabilities of -inf.  Workspace: lq_token_logprobs_workspace_size
+ * bytes, no contents kept from call to call. */
+size_t lq_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int64_t top);
+int lq_token_logprobs(const void* d_x, int type, int64_t ldx, int64_t rows, int64_t vocab, const int32_t* d_targets,
+                      int64_t top, float* d_logprobs, float* d_entropy, float* d_lse, float* d_top_logprobs,
+                      int32_t* d_top_ids, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Gradient in the logits of sum_r g_logprobs[r] logprobs[r] + g_entropy[r] entropy[r], from the
+ * lse and entropy of the forward call: grad_j = g (1[j = target] - p_j) - ge p_j (log p_j +
+ * entropy), p_j = e^(x_j - lse), of x's type (rows ldg apart; d_grad == d_x with equal strides
+ * works in place).  d_g_entropy (then d_entropy too) may be NULL: no entropy term.  A target outside
+ * [0, vocab) has no log probability term; a row without any allowed token has the gradient 0. */
+int lq_token_logprobs_backward(const void* d_x, int type, int64_t ldx, int64_t rows, int64_t vocab,
+                               const int32_t* d_targets, const float* d_lse, const float* d_entropy,
+                               const float* d_g_logprobs, const float* d_g_entropy, void* d_grad, int64_t ldg,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,14 @@ import numpy as np
 
 from lucid_amd import _C
 from lucid_amd._tensor import Tensor, empty, float32
+from lucid_amd.nn.generation import (  # noqa: F401  (part of this module's surface)
+    paged_attention,
+    paged_kv_append,
+    prompt_attention,
+    prompt_attention_qkv,
+    token_logprobs,
+    token_logprobs_backward,
+)
 from lucid_amd.quantization._device import on_device, require_gpu
 
 def _sig():

@@ -6,8 +6,15 @@
 
 namespace lq {
 
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 // Storage types: `load` is exact, `store` rounds once to nearest even.
 struct ElemF32 {
@@ -49,6 +56,91 @@ template <class F>
 inline void with_half(int t, F f) {
     if (t == LQ_F16) f(ElemF16{});
     else f(ElemBF16{});
+}
+
+// Eight 16-bit values of either type in four registers, as the matrix instructions take them.
+__device__ __forceinline__ f16v mfma_32x32x16(ElemF16, u4v a, u4v b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma_32x32x16(ElemBF16, u4v a, u4v b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+// Two values rounded to nearest even into one register, and back.
+__device__ __forceinline__ uint32_t pack2(ElemF16, float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), h2v));
+}
+__device__ __forceinline__ uint32_t pack2(ElemBF16, float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), b2v));
+}
+__device__ __forceinline__ f2v unpack2(ElemF16, uint32_t w) {
+    return __builtin_convertvector(__builtin_bit_cast(h2v, w), f2v);
+}
+__device__ __forceinline__ f2v unpack2(ElemBF16, uint32_t w) {
+    return f2v{__builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)};
+}
+// A weight that enters a product in 16 bits is 2^WEIGHT_SHIFT times its value relative to the
+// running maximum (which may lag by 2^RESCALE_AT): fp16 then resolves weights down to 2^-30 of
+// the largest and stays below 2^14; bfloat16 has float32's exponents and needs no shift.
+template <class E>
+constexpr float WEIGHT_SHIFT = E::code == LQ_F16 ? 6.0f : 0.0f;
+constexpr float RESCALE_AT = 8.0f;
+
+// Bits 15 and 31 are set where a 16-bit value of the word is an infinity or NaN.
+template <class E>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return E::code == LQ_F16 ? (w & 0x7c007c00u) + 0x04000400u : (w & 0x7f807f80u) + 0x00800080u;
+}
+
+// Where a weight is 0 because its key is not seen, an infinity or NaN in the value must not reach
+// the product: split_value takes such entries out of eight values and codes them (1 for +inf, 64
+// for -inf, 4096 for NaN), so that a product of the codes with 0 / 1 visibilities counts, per
+// query, those it does see (at most 63 of a kind, exact in the accumulator), and seen_value is
+// what they add to the sum.
+template <class E>
+__device__ __forceinline__ void split_value(u4v& v, u4v& codes) {
+    constexpr uint32_t EXP = E::code == LQ_F16 ? 0x7c00u : 0x7f80u;
+    constexpr uint32_t ONE = E::code == LQ_F16 ? 0x3c00u : 0x3f80u;
+    constexpr uint32_t MANY = E::code == LQ_F16 ? 0x5400u : 0x4280u, NAN_ = E::code == LQ_F16 ? 0x6c00u : 0x4580u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t keep = 0, code = 0;
+#pragma unroll
+        for (int s = 0; s < 32; s += 16) {
+            const uint32_t x = (v[j] >> s) & 0xffffu;
+            const bool odd = (x & EXP) == EXP;
+            const uint32_t c = (x & 0x7fffu) > EXP ? NAN_ : (x & 0x8000u) ? MANY : ONE;
+            keep |= (odd ? 0u : x) << s;
+            code |= (odd ? c : 0u) << s;
+        }
+        v[j] = keep;
+        codes[j] = code;
+    }
+}
+__device__ __forceinline__ float seen_value(float count) {
+    const int c = (int)count;
+    return c == 0 ? 0.0f : c >= 4096 || (c >= 64 && (c & 63)) ? __builtin_nanf("") : c >= 64 ? -INFINITY : INFINITY;
+}
+
+// The larger / the sum of the values that lanes l and l ^ 32 hold.
+__device__ __forceinline__ float half_max(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// LDS reads at a byte offset of the workgroup's LDS (written by copies the compiler does not see).
+typedef __attribute__((address_space(3))) u4v lds_u4v;
+typedef __attribute__((address_space(3))) s4v lds_s4v;
+__device__ __forceinline__ u4v lds_read16(uint32_t at) { return *reinterpret_cast<lds_u4v*>(at); }
+// Transposing read: of each 16 lanes, lane i points at four values of row i / 4 (columns 4 (i %
+// 4) ..) and receives column i of the four rows.
+__device__ __forceinline__ u2v lds_read_tr(uint32_t at) {
+    return __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4v*>(at)));
 }
 
 constexpr float LOG2E = 1.44269504088896341f;

@@ -7,6 +7,7 @@
 #include <hip/hip_fp16.h>
 
 #include "lq_attn.h"
+#include "lq_dma.h"
 #include "lq_place.h"
 
 namespace lq {
@@ -74,6 +75,248 @@ __global__ __launch_bounds__(256) void prompt_rows_kernel(PromptArgs a) {
     if (tid < hd) static_cast<typename Out::T*>(a.out)[(t * a.H + h) * hd + tid] = Out::store(len ? acc / l : 0.0f);
 }
 
+// ------------------------------------------------------------------------- the tile kernel
+
+constexpr int PT_WAVES = 4, PT_Q = 32 * PT_WAVES, PT_K = 64;  // queries of a workgroup, keys of a tile
+
+// Sequence and query block of workgroup index n (blocks of a sequence last to first: under the
+// causal mask the later ones have more keys, and the longest work starts first); false past the
+// last block.  Every wave finds it by a scan over 64 sequences at a time.
+__device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64_t& seq, int64_t& blk) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t base = 0; base < a.seqs; base += 64) {
+        const int64_t s = base + lane;
+        int cnt = 0;
+        if (s < a.seqs) cnt = (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + PT_Q - 1) / PT_Q);
+        int upto = cnt;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (n < all) {
+            const int l = __builtin_ctzll(__ballot(upto > n));
+            seq = base + l;
+            blk = __builtin_amdgcn_readlane(upto, l) - 1 - n;
+            return true;
+        }
+        n -= all;
+    }
+    return false;
+}
+
+template <int HDP, class E, class Out>
+__global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile_kernel(PromptArgs a) {
+    constexpr int CPR = HDP / 8;                                // 16-byte chunks of a row
+    constexpr int TILE = PT_K * HDP * 2;                        // bytes of a K (or V) tile
+    constexpr int COPIES = PT_K * CPR / (64 * PT_WAVES);        // 16-byte copies of a lane per tile
+    constexpr int KS = HDP / 16, DT = HDP / 32, KT = PT_K / 32;
+    constexpr bool TWO = Out::code == LQ_F32;                   // weights as two terms
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, hh = lane >> 5;
+    const uint32_t group = (uint32_t)(a.H / a.Hkv);
+    const uint32_t n = blockIdx.x / (uint32_t)a.H, hx = blockIdx.x - n * (uint32_t)a.H;
+    // consecutive workgroups (on consecutive XCDs) take different key heads: an XCD's L2 then
+    // serves few of them
+    const int hk = hx % (uint32_t)a.Hkv, h = hk * group + hx / (uint32_t)a.Hkv;
+    int64_t seq, blk;
+    if (!find_block(a, n, seq, blk)) return;
+    const Packed pk = packed_sequence(a.qs, a.ks, seq, a.total_q, a.total_k);
+    const bool causal = a.causal != 0;
+    const int64_t qb = blk * PT_Q, qw = qb + 32 * wave;  // first query of the workgroup, of the wave
+    const int hd = (int)a.hd;
+
+    // B operand of S^T = K Q^T: query qw + col, dims 16 s + 8 hh ..
+    u4v qf[KS];
+    {
+        const int64_t qi = min(qw + col, pk.nq - 1);
+        const uint16_t* qr = static_cast<const uint16_t*>(a.q) + (pk.q0 + qi) * a.ldq + (int64_t)h * hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * hh;
+            qf[s] = d < hd ? *reinterpret_cast<const u4v*>(qr + d) : u4v{0, 0, 0, 0};
+        }
+    }
+    // keys seen by this lane's query, by the wave's first and last one, and by the workgroup
+    const int lim = (int)keys_seen(pk, qw + col, causal);
+    const int seen_first = (int)keys_seen(pk, qw, causal);
+    const int seen_wave = qw < pk.nq ? (int)keys_seen(pk, qw + 31, causal) : 0;
+    const int seen_all = (int)keys_seen(pk, min(qb + PT_Q, pk.nq) - 1, causal);
+    const int tiles = (seen_all + PT_K - 1) / PT_K;
+
+    // copies: lane of copy j of its wave fills LDS slot (j * waves + wave) * 64 + lane; slot x of row
+    // r holds chunk x ^ swizzle(r), so that the reads below spread over the banks
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+    uint32_t koff[COPIES], voff[COPIES];
+    const uint32_t ldk = (uint32_t)a.ldk * 2, ldv = (uint32_t)a.ldv * 2;
+    auto vswz = [](int r) { return CPR == 8 ? 2 * ((r >> 1) & 3) : CPR % 16 == 0 ? 2 * (r & 7) : 2 * (r & 3); };
+#pragma unroll
+    for (int j = 0; j < COPIES; ++j) {
+        const int slot = (j * PT_WAVES + wave) * 64 + lane, r = slot / CPR, x = slot % CPR;
+        const int ck = x ^ (r & 7), cv = x ^ vswz(r);
+        koff[j] = 8 * ck < hd ? r * ldk + ck * 16 : 0x80000000u;  // past the head dim: out of range, read as 0
+        voff[j] = 8 * cv < hd ? r * ldv + cv * 16 : 0x80000000u;
+    }
+    const char* kbase = static_cast<const char*>(a.k) + (pk.k0 * a.ldk + (int64_t)hk * hd) * 2;
+    const char* vbase = static_cast<const char*>(a.v) + (pk.k0 * a.ldv + (int64_t)hk * hd) * 2;
+    auto issue = [&](int t) __attribute__((always_inline)) {
+        const int rows = (int)min((int64_t)PT_K, pk.nk - (int64_t)t * PT_K);  // at least 1
+        const v4i rk = buffer_rsrc(kbase + (int64_t)t * PT_K * ldk, (uint32_t)((rows - 1) * ldk + 2 * hd));
+        const v4i rv = buffer_rsrc(vbase + (int64_t)t * PT_K * ldv, (uint32_t)((rows - 1) * ldv + 2 * hd));
+        const uint32_t to = lds0 + (t & 1) * 2 * TILE + wave * 1024;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) lds_dma16(rk, koff[j], 0u, to + j * PT_WAVES * 1024);
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) lds_dma16(rv, voff[j], 0u, to + TILE + j * PT_WAVES * 1024);
+    };
+
+    f16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const float sl2 = a.scale * LOG2E;
+    // reads of K: row col of a 32-key block, chunk 2 s + hh; of V: rows 4 hh + (i >> 2) (+ 8), see lds_read_tr
+    const uint32_t krow = lds0 + col * HDP * 2;
+    const int vi = lane & 15, vr = 4 * hh + (vi >> 2), vc = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
+    const uint32_t vrow = lds0 + TILE + vr * HDP * 2 + 8 * (vi & 1);
+
+    if (tiles > 0) issue(0);
+    for (int t = 0; t < tiles; ++t) {
+        wait_vmcnt<0>();
+        block_barrier();  // tile t has landed, and every wave is done with the buffer of tile t + 1
+        if (t + 1 < tiles) issue(t + 1);
+        const int kb = t * PT_K;
+        if (kb >= seen_wave) continue;
+        const uint32_t buf = (t & 1) * 2 * TILE;
+        f16v sc[KT];
+#pragma unroll
+        for (int b = 0; b < KT; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ (col & 7)) << 4)),
+                                      qf[s], sc[b]);
+        }
+        const bool whole = kb + PT_K <= seen_first;  // every query of the wave sees every key of the tile
+        if (!whole) {
+            const int left = lim - kb - 4 * hh;
+#pragma unroll
+            for (int b = 0; b < KT; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * b + 8 * (i >> 2) + (i & 3) >= left) sc[b][i] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < KT; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
+        mx = half_max(mx) * sl2;
+        // the accumulators follow the maximum only when it has risen by more than 2^RESCALE_AT
+        if (__any(mx > m + RESCALE_AT)) {
+            const float mn = fmaxf(m, mx);
+            const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+        }
+        const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<E>;
+        u4v p[2 * KT], pl[TWO ? 2 * KT : 1];
+#pragma unroll
+        for (int b = 0; b < KT; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], sl2, -base));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i + 1], sl2, -base));
+                l += x + y;
+                const uint32_t w = pack2(E{}, x, y);
+                p[2 * b + (i >> 3)][(i & 7) >> 1] = w;
+                if constexpr (TWO) {
+                    const f2v r = unpack2(E{}, w);
+                    pl[2 * b + (i >> 3)][(i & 7) >> 1] = pack2(E{}, x - r[0], y - r[1]);
+                }
+            }
+        auto value = [&](int d, int ks) __attribute__((always_inline)) {
+            const uint32_t at = vrow + buf + ks * 16 * HDP * 2 + (((4 * d + vc) ^ vswz(vr)) << 4);
+            const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * HDP * 2);
+            return u4v{lo[0], lo[1], hi[0], hi[1]};
+        };
+        if (!whole) {  // keys not seen have the weight 0: no infinity or NaN may meet it
+            uint32_t odd = 0;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int ks = 0; ks < 2 * KT; ++ks) {
+                    const u4v v = value(d, ks);
+                    odd |= not_finite<E>(v[0]) | not_finite<E>(v[1]) | not_finite<E>(v[2]) | not_finite<E>(v[3]);
+                }
+            if (__any((odd & 0x80008000u) != 0)) {
+                const int left = lim - kb - 4 * hh;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                    for (int b = 0; b < KT; ++b) {  // 32 keys at a time
+                        f16v count;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) count[i] = 0.0f;
+#pragma unroll
+                        for (int ks = 2 * b; ks < 2 * b + 2; ++ks) {
+                            u4v v = value(d, ks), codes, sees;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int key = 16 * ks + 8 * (j >> 1) + 2 * (j & 1);
+                                sees[j] = pack2(E{}, key < left ? 1.0f : 0.0f, key + 1 < left ? 1.0f : 0.0f);
+                            }
+                            split_value<E>(v, codes);
+                            o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
+                            if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
+                            count = mfma_32x32x16(E{}, codes, sees, count);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] += seen_value(count[i]);
+                    }
+                }
+                continue;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int ks = 0; ks < 2 * KT; ++ks) {
+                const u4v v = value(d, ks);
+                o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
+                if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
+            }
+    }
+    l = half_sum(l);
+    const float r = seen_all > 0 && lim > 0 ? 1.0f / l : 0.0f;
+    const int64_t qi = qw + col;
+    if (qi < pk.nq) {
+        typename Out::T* orow = static_cast<typename Out::T*>(a.out) + ((pk.q0 + qi) * a.H + h) * hd;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int dim = 32 * d + 2 * i + 4 * hh;
+                if (dim < hd) {
+                    if constexpr (TWO) {
+                        *reinterpret_cast<vf4*>(orow + dim) = vf4{o[d][i] * r, o[d][i + 1] * r, o[d][i + 2] * r, o[d][i + 3] * r};
+                    } else {
+                        *reinterpret_cast<u2v*>(orow + dim) = u2v{pack2(E{}, o[d][i] * r, o[d][i + 1] * r),
+                                                                  pack2(E{}, o[d][i + 2] * r, o[d][i + 3] * r)};
+                    }
+                }
+            }
+    }
+}
+
 }  // namespace
 }  // namespace lq
 
@@ -100,6 +343,30 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
     const PromptArgs a{d_q, d_k, d_v, ldq, ldk, ldv, d_q_starts, d_k_starts, seqs, total_q, total_k, H, Hkv, hd,
                        causal, scale, d_out};
     const hipStream_t st = as_stream(stream);
+    // 16-byte copies and loads: bases and rows aligned to them, offsets of a tile's rows within 31 bits
+    const bool vec = aligned16(d_q) && aligned16(d_k) && aligned16(d_v) && aligned16(d_out) && ldq % 8 == 0 &&
+                     ldk % 8 == 0 && ldv % 8 == 0 && ldk < (1 << 23) && ldv < (1 << 23);
+    const int64_t blocks = (total_q + (PT_Q - 1) * (seqs < total_q ? seqs : total_q)) / PT_Q;
+    if (vec && blocks * H <= 0x7fffffff) {
+        const dim3 tiles((unsigned)(blocks * H)), wg(64 * PT_WAVES);
+        with_half(type, [&](auto e) {
+            using E = decltype(e);
+            auto go = [&](auto w, auto o) {
+                hipLaunchKernelGGL((prompt_tile_kernel<decltype(w)::value, E, decltype(o)>), tiles, wg, 0, st, a);
+            };
+            auto width = [&](auto o) {
+                if (hd <= 64) go(std::integral_constant<int, 64>{}, o);
+                else if (hd <= 128) go(std::integral_constant<int, 128>{}, o);
+                else if (hd <= 192) go(std::integral_constant<int, 192>{}, o);
+                else go(std::integral_constant<int, 256>{}, o);
+            };
+            if (out_type == LQ_F32) width(ElemF32{});
+            else width(E{});
+        });
+        note_path("prompt tile");
+        return launch_status("lq_prompt_attention");
+    }
+    note_path("prompt rows");
     const dim3 grid((unsigned)H, (unsigned)(total_q < 65535 ? total_q : 65535), (unsigned)((total_q + 65534) / 65535));
     with_half(type, [&](auto e) {
         using E = decltype(e);

@@ -91,36 +91,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return E::code == LQ_F16 ? (w & 0x7c007c00u) + 0x04000400u : (w & 0x7f807f80u) + 0x00800080u;
 }
 
-// Where a weight is 0 because its key is not seen, an infinity or NaN in the value must not reach
-// the product: split_value takes such entries out of eight values and codes them (1 for +inf, 64
-// for -inf, 4096 for NaN), so that a product of the codes with 0 / 1 visibilities counts, per
-// query, those it does see (at most 63 of a kind, exact in the accumulator), and seen_value is
-// what they add to the sum.
-template <class E>
-__device__ __forceinline__ void split_value(u4v& v, u4v& codes) {
-    constexpr uint32_t EXP = E::code == LQ_F16 ? 0x7c00u : 0x7f80u;
-    constexpr uint32_t ONE = E::code == LQ_F16 ? 0x3c00u : 0x3f80u;
-    constexpr uint32_t MANY = E::code == LQ_F16 ? 0x5400u : 0x4280u, NAN_ = E::code == LQ_F16 ? 0x6c00u : 0x4580u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t keep = 0, code = 0;
-#pragma unroll
-        for (int s = 0; s < 32; s += 16) {
-            const uint32_t x = (v[j] >> s) & 0xffffu;
-            const bool odd = (x & EXP) == EXP;
-            const uint32_t c = (x & 0x7fffu) > EXP ? NAN_ : (x & 0x8000u) ? MANY : ONE;
-            keep |= (odd ? 0u : x) << s;
-            code |= (odd ? c : 0u) << s;
-        }
-        v[j] = keep;
-        codes[j] = code;
-    }
-}
-__device__ __forceinline__ float seen_value(float count) {
-    const int c = (int)count;
-    return c == 0 ? 0.0f : c >= 4096 || (c >= 64 && (c & 63)) ? __builtin_nanf("") : c >= 64 ? -INFINITY : INFINITY;
-}
-
 // The larger / the sum of the values that lanes l and l ^ 32 hold.
 __device__ __forceinline__ float half_max(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);

@@ -23,56 +23,59 @@ struct PromptArgs {
     void* out;
 };
 
-// One workgroup per (head, query), 256 keys at a time: the simplest form.
+// Query t of head h (key head hk) over keys k0 .. k0 + len - 1, by one wave: 64 keys at a time, a lane
+// scores one key, then adds its dims (lane, lane + 64, ...) of the weighted values.  Reads nothing
+// but the keys seen, element by element: for operands that no vector fits, and for queries whose
+// tiles hold infinities or NaN beyond what they see.
 template <class E, class Out>
-__global__ __launch_bounds__(256) void prompt_rows_kernel(PromptArgs a) {
-    __shared__ float qv[ATTN_MAX_HD];
-    __shared__ float p[256];
-    __shared__ float red[8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t h = blockIdx.x, t = blockIdx.y + (int64_t)blockIdx.z * 65535, hk = h / (a.H / a.Hkv);
+__device__ __forceinline__ void attend_row(const PromptArgs& a, int64_t t, int h, int hk, int64_t k0, int64_t len) {
+    constexpr int PARTS = ATTN_MAX_HD / 64;
+    const int lane = threadIdx.x & 63, hd = (int)a.hd;
+    const typename E::T* q = static_cast<const typename E::T*>(a.q) + t * a.ldq + (int64_t)h * hd;
+    const typename E::T* k = static_cast<const typename E::T*>(a.k) + k0 * a.ldk + (int64_t)hk * hd;
+    const typename E::T* v = static_cast<const typename E::T*>(a.v) + k0 * a.ldv + (int64_t)hk * hd;
+    float m = -INFINITY, l = 0.0f, acc[PARTS] = {};
+    for (int64_t kb = 0; kb < len; kb += 64) {
+        const int n = (int)min((int64_t)64, len - kb);
+        float s = -INFINITY;
+        if (lane < n) {
+            const typename E::T* kr = k + (kb + lane) * a.ldk;
+            s = 0.0f;
+            for (int d = 0; d < hd; ++d) s = __builtin_fmaf(E::load(q[d]), E::load(kr[d]), s);
+            s *= a.scale * LOG2E;
+        }
+        float mx = s;
+        for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+        mx = fmaxf(mx, m);
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float e = lane < n ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
+        const float corr = __builtin_amdgcn_exp2f(m - base);
+        m = mx;
+        l = l * corr + ln_wave_sum(e);
+#pragma unroll
+        for (int c = 0; c < PARTS; ++c) acc[c] *= corr;
+        for (int j = 0; j < n; ++j) {
+            const float p = __shfl(e, j, 64);
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c)
+                if (lane + 64 * c < hd) acc[c] = __builtin_fmaf(p, E::load(v[(kb + j) * a.ldv + lane + 64 * c]), acc[c]);
+        }
+    }
+    typename Out::T* o = static_cast<typename Out::T*>(a.out) + (t * a.H + h) * hd;
+#pragma unroll
+    for (int c = 0; c < PARTS; ++c)
+        if (lane + 64 * c < hd) o[lane + 64 * c] = Out::store(len > 0 ? acc[c] / l : 0.0f);
+}
+
+// One wave per (head, query).
+template <class E, class Out>
+__global__ __launch_bounds__(64) void prompt_rows_kernel(PromptArgs a) {
+    const int64_t t = blockIdx.y + (int64_t)blockIdx.z * 65535;
     if (t >= a.total_q) return;
-    const int hd = (int)a.hd;
     const int64_t sq = sequence_of(a.qs, a.seqs, t);
     const Packed pk = packed_sequence(a.qs, a.ks, sq, a.total_q, a.total_k);
     if (t < pk.q0 || t >= pk.q0 + pk.nq) return;
-    const int64_t k0 = pk.k0, len = keys_seen(pk, t - pk.q0, a.causal);
-    if (tid < hd) qv[tid] = E::load(static_cast<const typename E::T*>(a.q)[t * a.ldq + h * hd + tid]);
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int64_t kb = 0; kb < len; kb += 256) {
-        __syncthreads();
-        const int64_t key = kb + tid;
-        float s = -INFINITY;
-        if (key < len) {
-            const typename E::T* kr = static_cast<const typename E::T*>(a.k) + (k0 + key) * a.ldk + hk * hd;
-            s = 0.0f;
-            for (int d = 0; d < hd; ++d) s = __builtin_fmaf(qv[d], E::load(kr[d]), s);
-            s *= a.scale * LOG2E;
-        }
-        float mb = s;
-        for (int off = 32; off > 0; off >>= 1) mb = fmaxf(mb, __shfl_xor(mb, off, 64));
-        if (lane == 0) red[wave] = mb;
-        __syncthreads();
-        mb = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = fmaxf(m, mb);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float e = key < len ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
-        const float corr = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        p[tid] = e;
-        float sum = e;
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        if (lane == 0) red[4 + wave] = sum;
-        __syncthreads();
-        l = l * corr + (red[4] + red[5] + red[6] + red[7]);
-        acc *= corr;
-        if (tid < hd) {
-            const int n = (int)min((int64_t)256, len - kb);
-            const typename E::T* vr = static_cast<const typename E::T*>(a.v) + (k0 + kb) * a.ldv + hk * hd + tid;
-            for (int j = 0; j < n; ++j) acc = __builtin_fmaf(p[j], E::load(vr[j * a.ldv]), acc);
-        }
-    }
-    if (tid < hd) static_cast<typename Out::T*>(a.out)[(t * a.H + h) * hd + tid] = Out::store(len ? acc / l : 0.0f);
+    attend_row<E, Out>(a, t, blockIdx.x, blockIdx.x / (int)(a.H / a.Hkv), pk.k0, keys_seen(pk, t - pk.q0, a.causal));
 }
 
 // ------------------------------------------------------------------------- the tile kernel
@@ -177,19 +180,21 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    uint32_t careful = 0;
     const float sl2 = a.scale * LOG2E;
     // reads of K: row col of a 32-key block, chunk 2 s + hh; of V: rows 4 hh + (i >> 2) (+ 8), see lds_read_tr
     const uint32_t krow = lds0 + col * HDP * 2;
     const int vi = lane & 15, vr = 4 * hh + (vi >> 2), vc = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
     const uint32_t vrow = lds0 + TILE + vr * HDP * 2 + 8 * (vi & 1);
 
-    if (tiles > 0) issue(0);
-    for (int t = 0; t < tiles; ++t) {
+    // one tile: MASKED where some query of the wave does not see some of its keys
+    auto step = [&](int t, auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         wait_vmcnt<0>();
         block_barrier();  // tile t has landed, and every wave is done with the buffer of tile t + 1
         if (t + 1 < tiles) issue(t + 1);
         const int kb = t * PT_K;
-        if (kb >= seen_wave) continue;
+        if (MASKED && kb >= seen_wave) return;
         const uint32_t buf = (t & 1) * 2 * TILE;
         f16v sc[KT];
 #pragma unroll
@@ -201,8 +206,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ (col & 7)) << 4)),
                                       qf[s], sc[b]);
         }
-        const bool whole = kb + PT_K <= seen_first;  // every query of the wave sees every key of the tile
-        if (!whole) {
+        if constexpr (MASKED) {
             const int left = lim - kb - 4 * hh;
 #pragma unroll
             for (int b = 0; b < KT; ++b)
@@ -248,7 +252,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
             const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * HDP * 2);
             return u4v{lo[0], lo[1], hi[0], hi[1]};
         };
-        if (!whole) {  // keys not seen have the weight 0: no infinity or NaN may meet it
+        if constexpr (MASKED) {  // a key not seen has the weight 0, which no infinity or NaN may meet
             uint32_t odd = 0;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -256,35 +260,9 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 for (int ks = 0; ks < 2 * KT; ++ks) {
                     const u4v v = value(d, ks);
                     odd |= not_finite<E>(v[0]) | not_finite<E>(v[1]) | not_finite<E>(v[2]) | not_finite<E>(v[3]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            if (__any((odd & 0x80008000u) != 0)) {
-                const int left = lim - kb - 4 * hh;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-#pragma unroll
-                    for (int b = 0; b < KT; ++b) {  // 32 keys at a time
-                        f16v count;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) count[i] = 0.0f;
-#pragma unroll
-                        for (int ks = 2 * b; ks < 2 * b + 2; ++ks) {
-                            u4v v = value(d, ks), codes, sees;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int key = 16 * ks + 8 * (j >> 1) + 2 * (j & 1);
-                                sees[j] = pack2(E{}, key < left ? 1.0f : 0.0f, key + 1 < left ? 1.0f : 0.0f);
-                            }
-                            split_value<E>(v, codes);
-                            o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
-                            if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
-                            count = mfma_32x32x16(E{}, codes, sees, count);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] += seen_value(count[i]);
-                    }
-                }
-                continue;
-            }
+            careful |= odd & 0x80008000u;
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -294,6 +272,15 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
                 if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
             }
+    };
+    const int open = qw < pk.nq ? min(seen_first / PT_K, tiles) : 0;  // tiles whose keys every query of the wave sees
+    if (tiles > 0) issue(0);
+    for (int t = 0; t < open; ++t) step(t, std::false_type{});
+    for (int t = open; t < tiles; ++t) step(t, std::true_type{});
+    if (__any(careful != 0)) {  // the wave's queries again, one by one
+        for (int64_t i = qw; i < min(qw + 32, pk.nq); ++i)
+            attend_row<E, Out>(a, pk.q0 + i, h, hk, pk.k0, keys_seen(pk, i, causal));
+        return;
     }
     l = half_sum(l);
     const float r = seen_all > 0 && lim > 0 ? 1.0f / l : 0.0f;
@@ -371,9 +358,9 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
     with_half(type, [&](auto e) {
         using E = decltype(e);
         if (out_type == LQ_F32)
-            hipLaunchKernelGGL((prompt_rows_kernel<E, ElemF32>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((prompt_rows_kernel<E, ElemF32>), grid, dim3(64), 0, st, a);
         else
-            hipLaunchKernelGGL((prompt_rows_kernel<E, E>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((prompt_rows_kernel<E, E>), grid, dim3(64), 0, st, a);
     });
     return launch_status("lq_prompt_attention");
 }

@@ -818,8 +818,9 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
  * [B][H][hd] contiguous, of q_type or LQ_F32.  A sequence of length <= 0 has the output 0, one
  * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
  * lengths: the split over the positions is planned from it, and lengths past it are still
- * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and finite.
- * Workspace: lq_paged_attention_workspace_size bytes, no contents kept from call to call. */
+ * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and
+ * finite; pages 16-byte aligned.  Workspace: lq_paged_attention_workspace_size bytes (0 where one
+ * workgroup takes a whole sequence), no contents kept from call to call. */
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
                        const void* d_k_pages, const void* d_v_pages, int cache_type, const float* d_k_scale,

@@ -65,6 +65,12 @@ __device__ __forceinline__ f16v mfma_32x32x16(ElemF16, u4v a, u4v b, f16v c) {
 __device__ __forceinline__ f16v mfma_32x32x16(ElemBF16, u4v a, u4v b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ vf4 mfma_16x16x32(ElemF16, u4v a, u4v b, vf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ vf4 mfma_16x16x32(ElemBF16, u4v a, u4v b, vf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
 // Two values rounded to nearest even into one register, and back.
 __device__ __forceinline__ uint32_t pack2(ElemF16, float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), h2v));
@@ -101,6 +107,25 @@ __device__ __forceinline__ float half_sum(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
     const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// The largest / the sum of the values that the lanes 16 and 32 apart hold (four lanes).
+__device__ __forceinline__ float quarter_max(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return half_max(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return half_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+}
+
+// Four int8 codes of a word as two words of 16-bit values, exact in both types.
+template <class E>
+__device__ __forceinline__ u2v widen4(uint32_t w) {
+    const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8), c = (float)(int8_t)(w >> 16), d = (float)(int8_t)(w >> 24);
+    return u2v{pack2(E{}, a, b), pack2(E{}, c, d)};
 }
 
 // LDS reads at a byte offset of the workgroup's LDS (written by copies the compiler does not see).

@@ -844,7 +844,7 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
  * LQ_F32, LQ_F16 or LQ_BF16), float32 out: lse[r] = log sum_j e^x_j; logprobs[r] = x[target] - lse
  * (0 for a target outside [0, vocab)); entropy[r] = -sum_j p_j log p_j; the `top` most likely
  * tokens in order (ties: the lower index; NaN above everything) with their log probabilities, in
- * [rows][top].  d_logprobs, d_entropy, d_lse may be NULL; top 0 .. 64, at most vocab.  A logit of
+ * [rows][top].  d_logprobs, d_entropy, d_lse may be NULL; top 0 .. 64, at most vocab (2^30).  A logit of
  * -inf is a token that is not allowed (probability 0); a row without any allowed token has lse =
  * -inf, entropy 0 and log probabilities of -inf.  Workspace: lq_token_logprobs_workspace_size
  * bytes, no contents kept from call to call. */

@@ -18,6 +18,7 @@ namespace lq {
 namespace {
 
 constexpr int LP_MAX_TOP = 64;
+constexpr int64_t LP_MAX_VOCAB = (int64_t)1 << 30;
 
 struct LogprobArgs {
     const void* x;
@@ -40,69 +41,260 @@ __device__ __forceinline__ uint32_t rank_index(uint64_t key) { return ~(uint32_t
 // Log probability of a logit: -inf stays -inf in a row that allows nothing.
 __device__ __forceinline__ float logprob_of(float x, float lse) { return x == -INFINITY && lse == lse ? x : x - lse; }
 
-// One workgroup per row: the maximum, the sums, then one scan per alternative.
+// 16 bytes of a row's elements as float32.
 template <class E>
-__global__ __launch_bounds__(256) void logprobs_rows_kernel(LogprobArgs a) {
-    __shared__ float red[2][4];
-    __shared__ uint64_t best[4];
+struct Chunk {
+    static constexpr int N = 16 / (int)sizeof(typename E::T);
+    float v[N];
+};
+template <class E>
+__device__ __forceinline__ Chunk<E> widen(u4v w) {
+    Chunk<E> c;
+    if constexpr (E::code == LQ_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c.v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f2v p = unpack2(E{}, w[i]);
+            c.v[2 * i] = p[0];
+            c.v[2 * i + 1] = p[1];
+        }
+    }
+    return c;
+}
+
+// A row in 16-byte chunks of aligned addresses: chunk q holds elements q N - shift ... q N - shift +
+// N - 1, of which the first and the last chunk may own only some.
+template <class E>
+struct Row {
+    static constexpr int N = Chunk<E>::N;
+    const typename E::T* x;
+    int vocab, shift, chunks;
+    __device__ __forceinline__ Row(const typename E::T* row, int64_t n) : x(row), vocab((int)n) {
+        shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
+        chunks = (int)(((int64_t)vocab + shift + N - 1) / N);
+    }
+    __device__ __forceinline__ bool full(int q) const { return q * (int64_t)N >= shift && (q + 1) * (int64_t)N - shift <= vocab; }
+    __device__ __forceinline__ int first(int q) const { return q * N - shift; }
+    __device__ __forceinline__ u4v load(int q) const {
+        return __builtin_nontemporal_load(reinterpret_cast<const u4v*>(x + first(q)));
+    }
+    // an edge chunk, -inf where it owns nothing
+    __device__ __forceinline__ Chunk<E> edge(int q) const {
+        Chunk<E> c;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int j = first(q) + e;
+            c.v[e] = j >= 0 && j < vocab ? E::load(x[j]) : -INFINITY;
+        }
+        return c;
+    }
+    __device__ __forceinline__ Chunk<E> get(int q) const { return full(q) ? widen<E>(load(q)) : edge(q); }
+};
+
+constexpr int LP_CAND = 512;  // alternatives collected before the last choice
+
+// One workgroup per row, one pass over it.  A thread keeps a reference for its exponentials (it
+// follows the largest value only when that has risen by more than 16, so that the sums are rarely
+// rescaled), the sums of e^d and of e^d d, and its largest value.
+//
+// The alternatives come from those largest values: of 64 groups of threads, the top-th largest group
+// maximum `cut` has at least `top` elements at or above it, and only threads whose own maximum
+// reaches it can hold any.  Their chunks are read again (from the caches), elements at or above the
+// cut collected and ranked against each other.  Where too many tie with the cut (masked tokens) the
+// elements above it are collected alone and the ties taken in index order; rows with NaN or +inf,
+// and rows where even those are too many, are searched once per alternative.
+template <int NT, class E>
+__global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
+    constexpr int W = NT / 64, N = Chunk<E>::N, UNROLL = 4;
+    __shared__ float red[3][W];
+    __shared__ float tmax[NT];
+    __shared__ float s_cut;
+    __shared__ int s_who, s_count, s_wave[W + 1];
+    __shared__ int who[NT];
+    __shared__ uint64_t cand[LP_CAND];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
-    const typename E::T* x = static_cast<const typename E::T*>(a.x) + r * a.ldx;
-    float m = -INFINITY;
-    for (int64_t j = tid; j < a.vocab; j += 256) m = fmaxf(m, E::load(x[j]));
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    if (lane == 0) red[0][wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    __syncthreads();
-    const float base = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, ed = 0.0f;
-    for (int64_t j = tid; j < a.vocab; j += 256) {
-        const float d = E::load(x[j]) - base, e = __builtin_amdgcn_exp2f(d * LOG2E);
-        s += e;
-        ed = __builtin_fmaf(e, fmaxf(d, -1e4f), ed);
+    const Row<E> row(static_cast<const typename E::T*>(a.x) + r * a.ldx, a.vocab);
+
+    float ref = -INFINITY, base = 0.0f, top = -INFINITY, s = 0.0f, ed = 0.0f;  // base: ref, 0 while it is -inf
+    auto add = [&](const Chunk<E>& c) __attribute__((always_inline)) {
+        float m = c.v[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) m = fmaxf(m, c.v[e]);
+        top = fmaxf(top, m);
+        if (m > ref + 16.0f) {
+            const float f = s > 0.0f ? __builtin_amdgcn_exp2f((base - m) * LOG2E) : 0.0f;
+            ed = f > 0.0f ? f * __builtin_fmaf(s, base - m, ed) : 0.0f;
+            s *= f;
+            ref = base = m;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float d = c.v[e] - base, p = __builtin_amdgcn_exp2f(d * LOG2E);
+            s += p;
+            ed = __builtin_fmaf(p, fmaxf(d, -1000.0f), ed);  // p is 0 there: no 0 * inf
+        }
+    };
+    int q = tid;
+    for (; q + (UNROLL - 1) * NT < row.chunks; q += UNROLL * NT) {
+        u4v w[UNROLL];
+        if (row.full(q) && row.full(q + (UNROLL - 1) * NT)) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) w[u] = row.load(q + u * NT);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) add(widen<E>(w[u]));
+        } else {
+            for (int u = 0; u < UNROLL; ++u) add(row.get(q + u * NT));
+        }
     }
-    for (int off = 32; off > 0; off >>= 1) {
-        s += __shfl_xor(s, off, 64);
-        ed += __shfl_xor(ed, off, 64);
+    for (; q < row.chunks; q += NT) add(row.get(q));
+
+    // the row's sums: every thread's brought to the largest reference
+    float R = ref;
+    for (int off = 32; off > 0; off >>= 1) R = fmaxf(R, __shfl_xor(R, off, 64));
+    if (W > 1) {
+        if (lane == 0) red[0][wave] = R;
+        __syncthreads();
+        R = red[0][0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) R = fmaxf(R, red[0][w]);
+        __syncthreads();
     }
-    if (lane == 0) {
-        red[0][wave] = s;
-        red[1][wave] = ed;
+    if (s > 0.0f) {
+        const float f = __builtin_amdgcn_exp2f((base - R) * LOG2E);
+        ed = f > 0.0f ? f * __builtin_fmaf(s, base - R, ed) : 0.0f;
+        s *= f;
     }
-    __syncthreads();
-    s = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
-    ed = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const float log_s = logf(s), lse = base + log_s;  // -inf for a row that allows nothing
+    s = ln_wave_sum(s);
+    ed = ln_wave_sum(ed);
+    if (W > 1) {
+        if (lane == 0) {
+            red[1][wave] = s;
+            red[2][wave] = ed;
+        }
+        __syncthreads();
+        s = red[1][0];
+        ed = red[2][0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            s += red[1][w];
+            ed += red[2][w];
+        }
+    }
+    const float log_s = logf(s), lse = (R == -INFINITY ? 0.0f : R) + log_s;  // -inf for a row that allows nothing
     if (tid == 0) {
         if (a.lse) a.lse[r] = lse;
         if (a.entropy) a.entropy[r] = s == 0.0f ? 0.0f : log_s - ed / s;
         if (a.logprobs) {
             const int64_t t = a.targets[r];
-            a.logprobs[r] = t >= 0 && t < a.vocab ? logprob_of(E::load(x[t]), lse) : 0.0f;
+            a.logprobs[r] = t >= 0 && t < a.vocab ? logprob_of(E::load(row.x[t]), lse) : 0.0f;
+        }
+    }
+    if (a.top == 0) return;
+
+    auto put = [&](int at, uint64_t key) {
+        const int j = (int)rank_index(key);
+        a.top_ids[r * a.top + at] = j;
+        a.top_logprobs[r * a.top + at] = logprob_of(E::load(row.x[j]), lse);
+    };
+    if (s == s) {  // uniform: no NaN, no +inf in the row
+        tmax[tid] = top;
+        if (tid == 0) s_who = s_count = 0;
+        __syncthreads();
+        if (wave == 0) {
+            float gm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < W; ++w) gm = fmaxf(gm, tmax[64 * w + lane]);
+            int rank = 0;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+                const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, gm), j));
+                rank += o > gm || (o == gm && j < lane);
+            }
+            if (rank == a.top - 1) s_cut = gm;
+        }
+        __syncthreads();
+        const float cut = s_cut;
+        if (top >= cut) who[atomicAdd(&s_who, 1)] = tid;
+        __syncthreads();
+        // the elements at or above the cut (past it, when `strict`) of the threads listed: a wave reads one
+        // thread's chunks, a lane each
+        const int holders = s_who;
+        auto collect = [&](bool strict) {
+            for (int i = wave; i < holders; i += W)
+                for (int64_t c = who[i] + (int64_t)NT * lane; c < row.chunks; c += (int64_t)NT * 64) {
+                    const Chunk<E> v = row.get((int)c);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const int j = row.first((int)c) + e;
+                        if (j >= 0 && j < row.vocab && (strict ? v.v[e] > cut : v.v[e] >= cut)) {
+                            const int at = atomicAdd(&s_count, 1);
+                            if (at < LP_CAND) cand[at] = rank_key(v.v[e], (uint32_t)j);
+                        }
+                    }
+                }
+            __syncthreads();
+            return s_count;
+        };
+        // each candidate's place is the number of larger ones (keys are distinct)
+        auto rank_all = [&](int n) {
+            for (int i = tid; i < n; i += NT) {
+                const uint64_t key = cand[i];
+                int at = 0;
+                for (int j = 0; j < n; ++j) at += cand[j] > key;
+                if (at < a.top) put(at, key);
+            }
+        };
+        int n = collect(false);
+        if (n <= LP_CAND) {
+            rank_all(n);
+            return;
+        }
+        __syncthreads();
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        n = collect(true);
+        if (n <= LP_CAND) {
+            rank_all(n);
+            int at = n;  // then the ties, the lowest indices first
+            for (int64_t j0 = 0; j0 < row.vocab && at < a.top; j0 += NT) {
+                const int64_t j = j0 + tid;
+                const bool hit = j < row.vocab && E::load(row.x[j]) == cut;
+                const uint64_t bits = __ballot(hit);
+                __syncthreads();
+                if (lane == 0) s_wave[wave] = __popcll(bits);
+                __syncthreads();
+                int before = at + __popcll(bits & (((uint64_t)1 << lane) - 1));
+                int all = at;
+                for (int w = 0; w < W; ++w) {
+                    before += w < wave ? s_wave[w] : 0;
+                    all += s_wave[w];
+                }
+                if (hit && before < a.top) put(before, rank_key(cut, (uint32_t)j));
+                at = all;
+            }
+            return;
         }
     }
     uint64_t last = ~(uint64_t)0;
     for (int k = 0; k < a.top; ++k) {
         uint64_t b = 0;
-        for (int64_t j = tid; j < a.vocab; j += 256) {
-            const uint64_t key = rank_key(E::load(x[j]), (uint32_t)j);
+        for (int64_t j = tid; j < row.vocab; j += NT) {
+            const uint64_t key = rank_key(E::load(row.x[j]), (uint32_t)j);
             if (key < last && key > b) b = key;
         }
         for (int off = 32; off > 0; off >>= 1) {
             const uint64_t o = __shfl_xor(b, off, 64);
             b = o > b ? o : b;
         }
-        if (lane == 0) best[wave] = b;
         __syncthreads();
-        for (int w = 0; w < 4; ++w) b = best[w] > b ? best[w] : b;
+        if (lane == 0) cand[wave] = b;
         __syncthreads();
+        for (int w = 0; w < W; ++w) b = cand[w] > b ? cand[w] : b;
         last = b;
-        if (tid == 0) {
-            const int64_t j = rank_index(b);
-            a.top_ids[r * a.top + k] = (int32_t)j;
-            a.top_logprobs[r * a.top + k] = logprob_of(E::load(x[j]), lse);
-        }
+        if (tid == 0) put(k, b);
     }
 }
 
@@ -115,22 +307,77 @@ struct LogprobGradArgs {
     int64_t ldg;
 };
 
+// What a row's elements have in common, and one element's gradient.
+struct GradRow {
+    float g, ge, H, lse;
+    int64_t target;  // -1: none
+    bool none;       // a row that allows nothing
+    __device__ __forceinline__ GradRow(const LogprobGradArgs& a, int64_t r) {
+        const int64_t t = a.targets[r];
+        lse = a.lse[r];
+        none = lse == -INFINITY;
+        target = t >= 0 && t < a.vocab && !none ? t : -1;
+        g = target >= 0 ? a.g_logprobs[r] : 0.0f;
+        ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
+        H = a.g_entropy ? a.entropy[r] : 0.0f;
+    }
+    __device__ __forceinline__ float at(float x, int64_t j) const {
+        const float lp = x - lse, p = none ? 0.0f : __builtin_amdgcn_exp2f(lp * LOG2E);
+        const float w = __builtin_fmaf(ge, fmaxf(lp, -1e4f) + H, g);  // p is 0 below: no 0 * inf
+        return (j == target ? g : 0.0f) - p * w;
+    }
+};
+
+constexpr int LG_CHUNKS = 4;  // 16-byte chunks of a thread
+
+// Rows of x and grad that share their alignment: a workgroup takes 1024 chunks of a row.
 template <class E>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogprobGradArgs a) {
+    constexpr int N = Chunk<E>::N;
+    const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 65535;
+    if (r >= a.rows) return;
+    const Row<E> row(static_cast<const typename E::T*>(a.x) + r * a.ldx, a.vocab);
+    typename E::T* y = static_cast<typename E::T*>(a.grad) + r * a.ldg;
+    const int q0 = blockIdx.x * (256 * LG_CHUNKS) + threadIdx.x;
+    u4v w[LG_CHUNKS];
+#pragma unroll
+    for (int u = 0; u < LG_CHUNKS; ++u) {
+        const int q = q0 + 256 * u;
+        if (q < row.chunks && row.full(q)) w[u] = row.load(q);
+    }
+    const GradRow gr(a, r);
+#pragma unroll
+    for (int u = 0; u < LG_CHUNKS; ++u) {
+        const int q = q0 + 256 * u;
+        if (q >= row.chunks) break;
+        const int j0 = row.first(q);
+        if (row.full(q)) {
+            const Chunk<E> c = widen<E>(w[u]);
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = gr.at(c.v[e], j0 + e);
+            u4v p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (E::code == LQ_F32) p[i] = __builtin_bit_cast(uint32_t, o[i]);
+                else p[i] = pack2(E{}, o[2 * i], o[2 * i + 1]);
+            }
+            __builtin_nontemporal_store(p, reinterpret_cast<u4v*>(y + j0));
+        } else {
+            for (int e = 0; e < N; ++e)
+                if (j0 + e >= 0 && j0 + e < row.vocab) y[j0 + e] = E::store(gr.at(E::load(row.x[j0 + e]), j0 + e));
+        }
+    }
+}
+
+// Any alignment, element by element.
+template <class E>
+__global__ __launch_bounds__(256) void logprobs_grad_any_kernel(LogprobGradArgs a) {
     const int64_t r = blockIdx.x;
     const typename E::T* x = static_cast<const typename E::T*>(a.x) + r * a.ldx;
     typename E::T* y = static_cast<typename E::T*>(a.grad) + r * a.ldg;
-    const int64_t t = a.targets[r];
-    const bool given = t >= 0 && t < a.vocab;
-    const float g = given ? a.g_logprobs[r] : 0.0f, lse = a.lse[r];
-    const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f, H = a.g_entropy ? a.entropy[r] : 0.0f;
-    const bool none = lse == -INFINITY;
-    for (int64_t j = threadIdx.x; j < a.vocab; j += 256) {
-        const float lp = E::load(x[j]) - lse, p = none ? 0.0f : __builtin_amdgcn_exp2f(lp * LOG2E);
-        const float w = g + ge * (fmaxf(lp, -1e4f) + H);
-        const float hot = !none && given && j == t ? g : 0.0f;
-        y[j] = E::store(hot - p * w);
-    }
+    const GradRow gr(a, r);
+    for (int64_t j = threadIdx.x; j < a.vocab; j += 256) y[j] = E::store(gr.at(E::load(x[j]), j));
 }
 
 }  // namespace
@@ -149,7 +396,7 @@ int lq_token_logprobs(const void* d_x, int type, int64_t ldx, int64_t rows, int6
                       int64_t top, float* d_logprobs, float* d_entropy, float* d_lse, float* d_top_logprobs,
                       int32_t* d_top_ids, void* d_workspace, size_t workspace_bytes, void* stream) {
     LQ_REQUIRE(is_float_type(type), "lq_token_logprobs: logits must be float32, fp16 or bfloat16");
-    LQ_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= 0x7fffffff && ldx >= vocab,
+    LQ_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= LP_MAX_VOCAB && ldx >= vocab,
                "lq_token_logprobs: bad shape");
     LQ_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= vocab,
                "lq_token_logprobs: at most 64 alternatives, and no more than the vocabulary holds");
@@ -159,8 +406,13 @@ int lq_token_logprobs(const void* d_x, int type, int64_t ldx, int64_t rows, int6
     const LogprobArgs a{d_x, ldx, rows, vocab, d_targets, (int)top, d_logprobs, d_entropy, d_lse, d_top_logprobs,
                         d_top_ids};
     with_float(type, [&](auto e) {
-        hipLaunchKernelGGL((logprobs_rows_kernel<decltype(e)>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream),
-                           a);
+        using E = decltype(e);
+        const dim3 grid((unsigned)rows);
+        const hipStream_t st = as_stream(stream);
+        const int64_t chunks = vocab * (int64_t)sizeof(typename E::T) / 16;
+        if (chunks <= 256) hipLaunchKernelGGL((logprobs_kernel<64, E>), grid, dim3(64), 0, st, a);
+        else if (chunks <= 1024) hipLaunchKernelGGL((logprobs_kernel<256, E>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((logprobs_kernel<1024, E>), grid, dim3(1024), 0, st, a);
     });
     return launch_status("lq_token_logprobs");
 }
@@ -170,7 +422,7 @@ int lq_token_logprobs_backward(const void* d_x, int type, int64_t ldx, int64_t r
                                const float* d_g_logprobs, const float* d_g_entropy, void* d_grad, int64_t ldg,
                                void* stream) {
     LQ_REQUIRE(is_float_type(type), "lq_token_logprobs_backward: logits must be float32, fp16 or bfloat16");
-    LQ_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= 0x7fffffff && ldx >= vocab && ldg >= vocab,
+    LQ_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab > 0 && vocab <= LP_MAX_VOCAB && ldx >= vocab && ldg >= vocab,
                "lq_token_logprobs_backward: bad shape");
     if (rows == 0) return LQ_OK;
     LQ_REQUIRE(d_x && d_targets && d_lse && d_g_logprobs && d_grad && (d_entropy || !d_g_entropy),
@@ -178,8 +430,18 @@ int lq_token_logprobs_backward(const void* d_x, int type, int64_t ldx, int64_t r
     LQ_REQUIRE(d_grad != d_x || ldg == ldx, "lq_token_logprobs_backward: in place needs equal strides");
     const LogprobGradArgs a{d_x, ldx, rows, vocab, d_targets, d_lse, d_entropy, d_g_logprobs, d_g_entropy, d_grad, ldg};
     with_float(type, [&](auto e) {
-        hipLaunchKernelGGL((logprobs_grad_kernel<decltype(e)>), dim3((unsigned)rows), dim3(256), 0, as_stream(stream),
-                           a);
+        using E = decltype(e);
+        constexpr int64_t S = sizeof(typename E::T), N = 16 / S;
+        const hipStream_t st = as_stream(stream);
+        if (((reinterpret_cast<uintptr_t>(d_x) - reinterpret_cast<uintptr_t>(d_grad)) & 15) == 0 &&
+            (ldx - ldg) * S % 16 == 0) {
+            const int64_t span = (vocab + 2 * (N - 1)) / N;  // chunks of a row at most
+            const dim3 grid((unsigned)((span + 256 * LG_CHUNKS - 1) / (256 * LG_CHUNKS)),
+                            (unsigned)(rows < 65535 ? rows : 65535), (unsigned)((rows + 65534) / 65535));
+            hipLaunchKernelGGL((logprobs_grad_kernel<E>), grid, dim3(256), 0, st, a);
+        } else {
+            hipLaunchKernelGGL((logprobs_grad_any_kernel<E>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        }
     });
     return launch_status("lq_token_logprobs_backward");
 }

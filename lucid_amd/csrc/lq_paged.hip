@@ -38,9 +38,9 @@ __device__ __forceinline__ int64_t token_row(const AppendArgs& a, int64_t t) {
     return position_row(pos, a.table + s * a.table_stride, a.table_stride, a.pages, a.Hkv, a.page);
 }
 
-// One thread per value: the simplest form.
+// One thread per value, for rows that 16-byte accesses do not fit.
 template <class Src, class Dst>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
     const int64_t per = a.Hkv * a.hd;
     const int64_t t = blockIdx.x;
     const int64_t row = token_row(a, t);
@@ -54,11 +54,79 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
 }
 
-// int8 rows: one wave per (token, head, k or v).  scale = max|x| / 127, code = rne(x * (127 /
-// max|x|)); a row whose largest magnitude is below 127 / FLT_MAX (or 0) is stored as zeros; one
-// that holds an infinity or NaN gets a scale that is not finite, so that it reads back as NaN.
+// Eight source values as float32, and eight values stored.
 template <class Src>
-__global__ __launch_bounds__(64) void append_i8_kernel(AppendArgs a) {
+__device__ __forceinline__ void load8(const typename Src::T* p, float (&x)[8]) {
+    if constexpr (Src::code == LQ_F32) {
+        const vf4 lo = __builtin_nontemporal_load(reinterpret_cast<const vf4*>(p));
+        const vf4 hi = __builtin_nontemporal_load(reinterpret_cast<const vf4*>(p) + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = lo[j];
+            x[j + 4] = hi[j];
+        }
+    } else {
+        const u4v w = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(p));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f2v u = unpack2(Src{}, w[j]);
+            x[2 * j] = u[0];
+            x[2 * j + 1] = u[1];
+        }
+    }
+}
+
+// TOK tokens per workgroup.  A thread keeps one place of the rows (k or v, head, eight dims) and
+// moves it for every token, the loads of all of them in flight together.
+template <int TOK, class Src, class Dst>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+    __shared__ int64_t rows[TOK];
+    const int64_t t0 = (int64_t)blockIdx.x * TOK;
+    if (threadIdx.x < TOK) rows[threadIdx.x] = t0 + threadIdx.x < a.tokens ? token_row(a, t0 + threadIdx.x) : -1;
+    __syncthreads();
+    const uint32_t hd8 = (uint32_t)a.hd >> 3, per = (uint32_t)a.Hkv * hd8;
+    for (uint32_t e = threadIdx.x; e < 2 * per; e += 256) {
+        const bool is_v = e >= per;
+        const uint32_t w = is_v ? e - per : e, h = w / hd8, d = (w - h * hd8) * 8;
+        const typename Src::T* src = static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t0 * a.ld + (int64_t)w * 8;
+        typename Dst::T* dst = static_cast<typename Dst::T*>(is_v ? a.vp : a.kp) + (int64_t)h * a.page * a.hd + d;
+        float x[TOK][8];
+#pragma unroll
+        for (int i = 0; i < TOK; ++i)
+            if (rows[i] >= 0) load8<Src>(src + i * a.ld, x[i]);
+#pragma unroll
+        for (int i = 0; i < TOK; ++i)
+            if (rows[i] >= 0) {
+                u4v o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = pack2(Dst{}, x[i][2 * j], x[i][2 * j + 1]);
+                *reinterpret_cast<u4v*>(dst + rows[i] * a.hd) = o;
+            }
+    }
+}
+
+// int8 rows: scale = max|x| / 127, code = rne(x * (127 / max|x|)); a row whose largest magnitude is below
+// 127 / FLT_MAX (or 0) is stored as zeros; one that holds an infinity or NaN gets a scale that is not
+// finite, so that it reads back as NaN or infinity.
+struct RowScale {
+    float inv, scale;
+    __device__ __forceinline__ explicit RowScale(int32_t top) {  // the largest |x| as bits (NaN above infinity)
+        const float amax = __builtin_bit_cast(float, top);
+        inv = 127.0f / amax;
+        const bool zero = amax == amax && !(inv < INFINITY);
+        scale = zero ? 0.0f : amax / 127.0f;
+        if (zero) inv = 0.0f;
+    }
+    __device__ __forceinline__ int code(float x) const {
+        const float c = rne(x * inv);
+        return c == c ? (int)fminf(fmaxf(c, -127.0f), 127.0f) : 0;
+    }
+};
+__device__ __forceinline__ int32_t magnitude(float x) { return __builtin_bit_cast(int32_t, x) & 0x7fffffff; }
+
+// One wave per (token, head, k or v), element by element.
+template <class Src>
+__global__ __launch_bounds__(64) void append_i8_any_kernel(AppendArgs a) {
     const int64_t t = blockIdx.x;
     const int64_t row = token_row(a, t);
     if (row < 0) return;
@@ -66,19 +134,41 @@ __global__ __launch_bounds__(64) void append_i8_kernel(AppendArgs a) {
     const bool is_v = blockIdx.y & 1;
     const typename Src::T* src = static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t * a.ld + h * a.hd;
     const int64_t r = row + h * a.page;
-    int32_t top = 0;  // integer order of |x| bits; NaN above infinity
-    for (int64_t d = threadIdx.x; d < a.hd; d += 64)
-        top = max(top, __builtin_bit_cast(int32_t, Src::load(src[d])) & 0x7fffffff);
-    top = wave_max(top);
-    const float amax = __builtin_bit_cast(float, top);
-    const float inv = 127.0f / amax;
-    const bool zero = !(inv < INFINITY) && amax == amax;
+    int32_t top = 0;
+    for (int64_t d = threadIdx.x; d < a.hd; d += 64) top = max(top, magnitude(Src::load(src[d])));
+    const RowScale rs(wave_max(top));
     int8_t* dst = static_cast<int8_t*>(is_v ? a.vp : a.kp) + r * a.hd;
-    for (int64_t d = threadIdx.x; d < a.hd; d += 64) {
-        const float c = rne(Src::load(src[d]) * inv);
-        dst[d] = zero || c != c ? 0 : (int8_t)fminf(fmaxf(c, -127.0f), 127.0f);
+    for (int64_t d = threadIdx.x; d < a.hd; d += 64) dst[d] = (int8_t)rs.code(Src::load(src[d]));
+    if (threadIdx.x == 0) (is_v ? a.vs : a.ks)[r] = rs.scale;
+}
+
+// LPR lanes per row of hd <= 8 LPR values, eight values a lane; one workgroup per token.
+template <int LPR, class Src>
+__global__ __launch_bounds__(256) void append_i8_kernel(AppendArgs a) {
+    const int64_t t = blockIdx.x;
+    const int64_t row = token_row(a, t);
+    if (row < 0) return;
+    const uint32_t d = (threadIdx.x % LPR) * 8;
+    // every lane of a wave takes the same number of rounds: the exchange below needs them all
+    for (uint32_t e = threadIdx.x / LPR; e < ((uint32_t)a.Hkv * 2 + 64 / LPR - 1) / (64 / LPR) * (64 / LPR); e += 256 / LPR) {
+        const bool is_v = e & 1, mine = e < (uint32_t)a.Hkv * 2 && d < (uint32_t)a.hd;
+        const uint32_t h = e >> 1;
+        float x[8] = {};
+        if (mine) load8<Src>(static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t * a.ld + (int64_t)h * a.hd + d, x);
+        int32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[j]));
+#pragma unroll
+        for (int off = LPR / 2; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
+        const RowScale rs(top);
+        if (!mine) continue;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(rs.code(x[j]) & 0xff) << (8 * (j & 3));
+        const int64_t r = row + (int64_t)h * a.page;
+        *reinterpret_cast<u2v*>(static_cast<int8_t*>(is_v ? a.vp : a.kp) + r * a.hd + d) = u2v{w[0], w[1]};
+        if (d == 0) (is_v ? a.vs : a.ks)[r] = rs.scale;
     }
-    if (threadIdx.x == 0) (is_v ? a.vs : a.ks)[r] = zero ? 0.0f : amax / 127.0f;
 }
 
 // ------------------------------------------------------------------------------ attention
@@ -468,15 +558,26 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
     const AppendArgs a{d_k, d_v, ld, tokens, d_starts, seqs, Hkv, hd, d_table, table_stride, d_lengths,
                        d_k_pages, d_v_pages, d_k_scale, d_v_scale, pages, page};
     const hipStream_t st = as_stream(stream);
+    // eight values of a row at a time: heads of whole eights, bases and rows 16-byte aligned
+    const uintptr_t ends = reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v) |
+                           reinterpret_cast<uintptr_t>(d_k_pages) | reinterpret_cast<uintptr_t>(d_v_pages);
+    const bool vec = hd % 8 == 0 && (ends & 15) == 0 && ld * elem_size(src_type) % 16 == 0 && Hkv * hd < (1 << 28);
     with_float(src_type, [&](auto s) {
         using S = decltype(s);
+        const dim3 one((unsigned)tokens);
         if (cache_type == LQ_I8) {
-            hipLaunchKernelGGL((append_i8_kernel<S>), dim3((unsigned)tokens, (unsigned)(2 * Hkv)), dim3(64), 0, st, a);
-        } else {
-            with_half(cache_type, [&](auto c) {
-                hipLaunchKernelGGL((append_kernel<S, decltype(c)>), dim3((unsigned)tokens), dim3(256), 0, st, a);
-            });
+            if (vec && hd <= 64) hipLaunchKernelGGL((append_i8_kernel<8, S>), one, dim3(256), 0, st, a);
+            else if (vec && hd <= 128) hipLaunchKernelGGL((append_i8_kernel<16, S>), one, dim3(256), 0, st, a);
+            else if (vec && hd <= 256) hipLaunchKernelGGL((append_i8_kernel<32, S>), one, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((append_i8_any_kernel<S>), dim3((unsigned)tokens, (unsigned)(2 * Hkv)), dim3(64), 0, st, a);
+            return;
         }
+        with_half(cache_type, [&](auto c) {
+            using C = decltype(c);
+            if (!vec) hipLaunchKernelGGL((append_any_kernel<S, C>), one, dim3(256), 0, st, a);
+            else if (tokens <= 4 * 1024) hipLaunchKernelGGL((append_kernel<1, S, C>), one, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((append_kernel<4, S, C>), dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, st, a);
+        });
     });
     return launch_status("lq_paged_kv_append");
 }

@@ -121,11 +121,30 @@ __device__ __forceinline__ float quarter_sum(float v) {
     return half_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
 }
 
-// Four int8 codes of a word as two words of 16-bit values, exact in both types.
-template <class E>
-__device__ __forceinline__ u2v widen4(uint32_t w) {
-    const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8), c = (float)(int8_t)(w >> 16), d = (float)(int8_t)(w >> 24);
-    return u2v{pack2(E{}, a, b), pack2(E{}, c, d)};
+// Byte I of a word as a signed integer in float32.
+template <int I>
+__device__ __forceinline__ float byte_to_f32(uint32_t w) {
+    float f;
+    if constexpr (I == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+    if constexpr (I == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    if constexpr (I == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    if constexpr (I == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
+// Four int8 codes of a word as two words of 16-bit values, exact in both types.  fp16: the code + 128
+// under the exponent of 1024 is 1152 + code; bfloat16: the upper halves of the float32 values (eight
+// significant bits hold any code).
+__device__ __forceinline__ u2v widen4(ElemF16, uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u;
+    const h2v bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const h2v lo = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias;
+    const h2v hi = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias;
+    return u2v{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+__device__ __forceinline__ u2v widen4(ElemBF16, uint32_t w) {
+    const uint32_t a = __float_as_uint(byte_to_f32<0>(w)), b = __float_as_uint(byte_to_f32<1>(w));
+    const uint32_t c = __float_as_uint(byte_to_f32<2>(w)), d = __float_as_uint(byte_to_f32<3>(w));
+    return u2v{__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
 }
 
 // LDS reads at a byte offset of the workgroup's LDS (written by copies the compiler does not see).

@@ -62,4 +62,11 @@ __device__ __forceinline__ void lds_dma16(v4i rsrc, uint32_t voff, uint32_t soff
                  : "memory");
 }
 
+// 16 bytes per lane from the lane's own address into LDS at lds_addr + 16 * lane (lanes switched off copy
+// nothing), past the caches: for what is read once.  No bounds check: every active lane's address must
+// be valid.
+__device__ __forceinline__ void lds_copy16(const void* src, uint32_t lds_addr) {
+    asm volatile("global_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
+}
+
 }  // namespace lq

@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "lq_attn.h"
+#include "lq_dma.h"
 #include "lq_place.h"
 
 namespace lq {
@@ -188,349 +189,602 @@ struct PagedArgs {
     void* out;
     int out_f32;
     int q_vec;          // q may be read 16 bytes at a time
-    int chunk, splits;  // positions of a workgroup; chunk 0 .. splits - 1 (the last takes the rest)
+    int groups;         // workgroups that share all positions evenly; 0: one per sequence and key head
+    int64_t* bases;     // [B + 1] first step of each sequence, then the steps of a workgroup
     float *part_o, *part_ml;
 };
 
-constexpr int PG_WAVES = 4, PG_K = 32;  // waves of a workgroup, keys of a wave's tile
+constexpr int PG_K = 32;        // positions of a wave's tile
+constexpr int PG_I8_WAVES = 4;  // waves of a workgroup over an int8 cache
 
-// Length of sequence b within its table (positions past it are an error: `over`), and the number
-// of chunks it takes (the last one takes what the plan did not foresee).
-__device__ __forceinline__ int sequence_length(const PagedArgs& a, int b, bool& over, int& used) {
+// Length of sequence b within its table (positions past it are an error: `over`).
+__device__ __forceinline__ int sequence_length(const PagedArgs& a, int b, bool& over) {
     const int64_t cap = min(a.table_stride * a.page, (int64_t)(INT32_MAX - 4096));
     const int len = max(a.lengths[b], 0);
     over = len > cap;
-    const int n = over ? (int)cap : len;
-    used = min(a.splits, (int)(((int64_t)n + a.chunk - 1) / a.chunk));
-    return n;
+    return over ? (int)cap : len;
 }
 
-// Workgroup (key head and tile of 16 query heads, sequence, chunk of positions).  Each wave takes
-// every fourth tile of 32 positions with a maximum, sum and accumulators of its own, and the
-// waves meet at the end: no barrier inside the loop.
-//   S^T = K Q^T (v_mfma 16x16x32): lane (l, g) loads the rows l and 16 + l of K straight into the A
-//   operand and receives positions 4 g + i (and 16 + 4 g + i) of query l;
-//   O^T += V^T P^T: those weights are the B operand as they are; V passes through the wave's LDS,
-//   whose transposing read gives lane (l, g) dim l of the same positions.
+// The two kernels share this plan.  The work is a line of steps (WAVES tiles of 32 positions): all steps
+// of the first sequence's first key head (and tile of 16 query heads), then of its next one, and so
+// on.  Each workgroup takes an equal part of the line, whatever the sequences' lengths, and works
+// through the pieces of sequences in it one after the other: a piece costs some microseconds of
+// dependent loads before its first tile (512 positions a workgroup took 109 us where 1024 took 102,
+// 64 sequences of 2048), and unequal parts leave the chip waiting for the longest.  A piece that is
+// a whole sequence is written at once, others go to the workspace (a workgroup has two at most, its first
+// and its last) and are joined by a second launch.  With short sequences (`groups` 0) a workgroup takes
+// one of them whole and there is no second launch.
+//
+// Within a piece each wave takes every WAVES-th tile with a maximum, sum and accumulators of its own, and
+// the waves meet at the end: no barrier inside the loop.
+//   S^T = K Q^T (v_mfma 16x16x32): K is the A operand, row l (and 16 + l) in lane (l, g), which receives
+//   positions 4 g + i (and 16 + 4 g + i) of query l;
+//   O^T += V^T P^T: those weights are the B operand as they are; V comes from the wave's LDS, whose
+//   transposing read gives lane (l, g) dim l of the same positions.
 // A weight enters as two 16-bit terms (about 16 significant bits): the products are free beside the
-// loads.  An int8 cache's codes are exact in 16 bits; the key's scale multiplies the score, the
-// value's scale the weight, which is then bfloat16 for its range.
-template <int HDP, bool EXACT, class Q, class C>
-__global__ __launch_bounds__(64 * PG_WAVES) void paged_tile_kernel(PagedArgs a) {
-    constexpr bool I8 = C::code == LQ_I8;
-    using P = std::conditional_t<I8, ElemBF16, Q>;  // type of the second product
-    constexpr int KS = HDP / 32, DT = HDP / 16;
-    constexpr int VROW = HDP * 2, VTILE = PG_K * VROW;            // bytes of a V row / tile in LDS
-    constexpr int OROW = HDP + 4, OTILE = 16 * OROW * 4;          // floats of a query's row, bytes of a wave's sums
-    constexpr int SLOT = (VTILE > OTILE ? VTILE : OTILE) + 256;   // + 64 scales
-    __shared__ __attribute__((aligned(16))) uint8_t lds[PG_WAVES * SLOT];
-    __shared__ float mls[PG_WAVES][2][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x / a.qtiles, qt = blockIdx.x - hk * a.qtiles, b = blockIdx.y, split = blockIdx.z;
-    const int hd = EXACT ? HDP : a.hd, heads = min(16, a.group - 16 * qt);
-    const int h0 = hk * a.group + 16 * qt;
-    bool bad;  // a position that has no page
-    int used;
-    const int len = sequence_length(a, b, bad, used);
-    const int64_t first = (int64_t)split * a.chunk;
-    if (split > 0 && split >= used) return;
-    const int end = split == a.splits - 1 ? len : (int)min((int64_t)len, first + a.chunk);
-    const int begin = (int)first;
+// loads.
+struct Piece {
+    int b, h0, hk, heads, begin, end, len;
+    bool over, whole;
+    int64_t slot;
+};
 
-    // dims of this lane's eight slots in step s of the first product
-    auto dims = [&](int s) { return I8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
-    u4v qf[KS];
-    {
-        const uint16_t* qr = static_cast<const uint16_t*>(a.q) + b * a.ldq + (int64_t)(h0 + min(l16, heads - 1)) * hd;
+// The line of steps as a workgroup walks it.
+template <int WAVES>
+struct Line {
+    static constexpr int STEP = WAVES * PG_K, NT = 64 * WAVES, LEAST = 512 / STEP;
+    int64_t at, stop, start, base;  // next step, end and start of this part; first step of sequence b
+    int b, len, steps, heads;       // heads: key heads times tiles of 16 query heads
+    bool over;
+
+    __device__ __forceinline__ void sequence(const PagedArgs& a, int i) {
+        b = i;
+        len = sequence_length(a, i, over);
+        steps = (len + STEP - 1) / STEP;
+    }
+    // Finds the part of workgroup blockIdx.x; `scan` holds NT + 1 numbers.
+    __device__ __forceinline__ void init(const PagedArgs& a, int64_t* scan) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        heads = a.Hkv * a.qtiles;
+        if (a.groups == 0) {
+            const int i = blockIdx.x / heads;
+            sequence(a, i);
+            base = 0;
+            start = at = (int64_t)(blockIdx.x - i * heads) * steps;
+            stop = at + steps;
+            return;
+        }
+        const int per = (a.B + NT - 1) / NT, first = min(tid * per, a.B), last = min(first + per, a.B);
+        int64_t mine = 0;
+        for (int i = first; i < last; ++i) {
+            sequence(a, i);
+            mine += (int64_t)heads * steps;
+        }
+        int64_t upto = mine;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            qf[s] = u4v{0, 0, 0, 0};
-            if (EXACT || dims(s) < hd) {
-                if (a.q_vec) {
-                    qf[s] = *reinterpret_cast<const u4v*>(qr + dims(s));
-                } else {
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+        scan[tid] = upto;
+        __syncthreads();
+        int64_t before = upto - mine;
+        for (int w = 0; w < wave; ++w) before += scan[64 * w + 63];
+        int64_t total = 0;
+        for (int w = 0; w < WAVES; ++w) total += scan[64 * w + 63];
+        __syncthreads();
+        scan[tid] = before;
+        if (tid == 0) scan[NT] = total;
+        int64_t share = (total + a.groups - 1) / a.groups;
+        share = share < LEAST ? LEAST : share;
+        if (blockIdx.x == 0) {
+            for (int i = first; i < last; ++i) {
+                a.bases[i] = before;
+                sequence(a, i);
+                before += (int64_t)heads * steps;
+            }
+            if (tid == 0) {
+                a.bases[a.B] = total;
+                a.bases[a.B + 1] = share;
+            }
+        }
+        __syncthreads();
+        start = at = min((int64_t)blockIdx.x * share, total);
+        stop = min(at + share, total);
+        if (at >= stop) return;
+        int lo = 0, hi = NT;  // the last thread whose sequences begin at or before `at`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (scan[mid] <= at) lo = mid; else hi = mid;
+        }
+        base = scan[lo];
+        sequence(a, lo * per);
+        while (at >= base + (int64_t)heads * steps) {
+            base += (int64_t)heads * steps;
+            sequence(a, b + 1);
+        }
+    }
+    // The next piece; false when the part is done.  Uniform over the workgroup.
+    __device__ __forceinline__ bool next(const PagedArgs& a, Piece& p) {
+        if (at >= stop) return false;
+        while (at >= base + (int64_t)heads * steps) {
+            base += (int64_t)heads * steps;
+            sequence(a, b + 1);
+        }
+        const int hq = (int)((at - base) / steps), s0 = (int)(at - base - (int64_t)hq * steps);
+        const int n = (int)min((int64_t)(steps - s0), stop - at);
+        const int qt = hq % a.qtiles;
+        p.b = b;
+        p.hk = hq / a.qtiles;
+        p.heads = min(16, a.group - 16 * qt);
+        p.h0 = p.hk * a.group + 16 * qt;
+        p.len = len;
+        p.over = over;
+        p.begin = s0 * STEP;
+        p.end = min((s0 + n) * STEP, len);
+        p.whole = n == steps;
+        p.slot = 2 * (int64_t)blockIdx.x + (at == start ? 0 : 1);
+        at += n;
+        return true;
+    }
+};
+
+// Sequences without a position: 0, or NaN where only the table is missing.
+template <int WAVES, class Q>
+__device__ __forceinline__ void paged_empty(const PagedArgs& a) {
+    const int64_t row = (int64_t)a.H * a.hd;
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+        bool over;
+        if (sequence_length(a, b, over) > 0) continue;
+        const float y = over ? __builtin_nanf("") : 0.0f;
+        for (int64_t e = threadIdx.x; e < row; e += 64 * WAVES) {
+            if (a.out_f32) static_cast<float*>(a.out)[b * row + e] = y;
+            else static_cast<typename Q::T*>(a.out)[b * row + e] = Q::store(y);
+        }
+    }
+}
+
+// Eight dims from d on of query head h0 + min(l, heads - 1), zeros past the head dim.
+__device__ __forceinline__ u4v paged_query(const PagedArgs& a, const Piece& w, int l, int d, int hd) {
+    u4v f = {0, 0, 0, 0};
+    if (d >= hd) return f;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + w.b * a.ldq + (int64_t)(w.h0 + min(l, w.heads - 1)) * hd + d;
+    if (a.q_vec) return *reinterpret_cast<const u4v*>(q);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) qf[s][j >> 1] |= (uint32_t)qr[dims(s) + j] << (16 * (j & 1));
-                }
+    for (int j = 0; j < 8; ++j) f[j >> 1] |= (uint32_t)q[j] << (16 * (j & 1));
+    return f;
+}
+
+// Statistics and accumulators of a wave: 16 queries, DT * 16 dims.
+template <int DT, class P>
+struct Sums {
+    vf4 o[DT];
+    float m, l;
+    __device__ __forceinline__ Sums() : m(-INFINITY), l(0.0f) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
+    }
+    // Scores (of n positions from this lane's 4 g on, -inf past them) to weights relative to the
+    // running maximum; the accumulators follow it only when it has risen by more than 2^RESCALE_AT.
+    __device__ __forceinline__ void weights(vf4 (&sc)[2], float sl2, bool whole, int n) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!whole && 16 * T + i >= n) sc[T][i] = -INFINITY;
+                mx = fmaxf(mx, sc[T][i]);
+            }
+        mx = quarter_max(mx) * sl2;
+        if (__any(mx > m + RESCALE_AT)) {
+            const float mn = fmaxf(m, mx);
+            const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= corr;
+        }
+        const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<P>;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[T][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -base));
+                l += sc[T][i];
+            }
+    }
+    // O^T += V^T P^T, V at LDS `v_at` with rows of VROW bytes swizzled by swz
+    template <int VROW, class F>
+    __device__ __forceinline__ void accumulate(const vf4 (&w)[2], uint32_t v_at, F swz) {
+        u4v ph, pl;
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t u = pack2(P{}, w[T][2 * i], w[T][2 * i + 1]);
+                const f2v r = unpack2(P{}, u);
+                ph[2 * T + i] = u;
+                pl[2 * T + i] = pack2(P{}, w[T][2 * i] - r[0], w[T][2 * i + 1] - r[1]);
+            }
+        const int lane = threadIdx.x & 63, vi = lane & 15, row = 4 * (lane >> 4) + (vi >> 2);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const uint32_t at = v_at + row * VROW + (((2 * d + ((vi & 3) >> 1)) ^ swz(row)) << 4) + 8 * (vi & 1);
+            const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * VROW);
+            const u4v v = {lo[0], lo[1], hi[0], hi[1]};
+            o[d] = mfma_16x16x32(P{}, v, ph, o[d]);
+            o[d] = mfma_16x16x32(P{}, v, pl, o[d]);
+        }
+    }
+};
+
+// The waves' sums meet: wave w's lie at LDS lds + w * SLOT (16 queries of OROW floats each), and the
+// workgroup writes the output or its part of it.
+template <int WAVES, int SLOT, int DT, class Q, class P>
+__device__ __forceinline__ void paged_finish(const PagedArgs& a, const Piece& w, uint8_t* lds, float (*ml)[2][16],
+                                             Sums<DT, P>& s, bool bad) {
+    constexpr int OROW = 16 * DT + 4;
+    static_assert(16 * OROW * 4 <= SLOT, "the sums fit the wave's LDS");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4, hd = a.hd;
+    float l = quarter_sum(s.l);
+    if (__any(bad)) l = __builtin_nanf("");
+    float* so = reinterpret_cast<float*>(lds + wave * SLOT);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<vf4*>(so + l16 * OROW + 16 * d + 4 * g) = s.o[d];
+    if (g == 0) {
+        ml[wave][0][l16] = s.m;
+        ml[wave][1][l16] = l;
+    }
+    __syncthreads();
+    for (int e = tid; e < w.heads * hd; e += 64 * WAVES) {
+        const int r = e / hd, d = e - r * hd;
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) M = fmaxf(M, ml[v][0][r]);
+        const float base = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            const float f = __builtin_amdgcn_exp2f(ml[v][0][r] - base);
+            L = __builtin_fmaf(f, ml[v][1][r], L);
+            x = __builtin_fmaf(f, reinterpret_cast<const float*>(lds + v * SLOT)[r * OROW + d], x);
+        }
+        if (w.whole) {
+            const int64_t at = ((int64_t)w.b * a.H + w.h0 + r) * hd + d;
+            if (a.out_f32) static_cast<float*>(a.out)[at] = x / L;
+            else static_cast<typename Q::T*>(a.out)[at] = Q::store(x / L);
+        } else {
+            a.part_o[(16 * w.slot + r) * hd + d] = x;
+            if (d == 0) {
+                a.part_ml[2 * (16 * w.slot + r)] = M;
+                a.part_ml[2 * (16 * w.slot + r) + 1] = L;
             }
         }
     }
-    const int32_t* table = a.table + (int64_t)b * a.table_stride;
-    // page number of a position (-1: none), and the row of a position in the pool
-    auto page_of = [&](int key) -> int {
-        const uint32_t col = (uint32_t)key / (uint32_t)a.page;
-        return key < end && col < a.table_stride ? table[col] : -1;
+    __syncthreads();  // the next piece fills this LDS again
+}
+
+// V rows in LDS: 16-byte chunk c of row r lies at chunk c ^ v_swz(r), so that the transposing reads (4 rows,
+// 2 chunks for 16 lanes) and the writes spread over the banks; K rows (8 lanes read 8 rows): c ^ (r & 7).
+template <int HDP>
+__device__ __forceinline__ int v_swz(int r) {
+    return HDP == 64 ? 2 * ((r >> 1) & 3) : HDP % 128 == 0 ? 2 * (r & 7) : 2 * (r & 3);
+}
+
+constexpr int PG_IDS = 512;  // positions of a wave between two looks into the table
+
+// fp16 / bfloat16 cache.  K and V tiles are copied to the wave's LDS 16 bytes a lane, NST tiles deep: the
+// copies of a row are one contiguous access, they need no registers, and a wave waits only for
+// its oldest tile.  The byte offsets of PG_IDS positions at a time are looked up before their copies.
+template <int HDP, int WAVES, int NST, bool EXACT, class Q>
+__global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
+    constexpr int CPR = HDP / 8, COPIES = PG_K * CPR / 64, KS = HDP / 32, DT = HDP / 16;
+    constexpr int ROW = HDP * 2, TILE = PG_K * ROW, SLOT = 2 * NST * TILE;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOT];
+    __shared__ int64_t offsets[WAVES][PG_IDS];
+    __shared__ float ml[WAVES][2][16];
+    __shared__ int64_t scan[64 * WAVES + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int hd = EXACT ? HDP : a.hd;
+    Line<WAVES> line;
+    line.init(a, scan);
+    paged_empty<WAVES, Q>(a);
+    const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
+    // copy i of a tile: LDS chunk 64 i + lane, row (64 i + lane) / CPR
+    int kch[COPIES], vch[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        const int r = (64 * i + lane) / CPR, x = (64 * i + lane) % CPR;
+        kch[i] = (x ^ (r & 7)) * 16;
+        vch[i] = (x ^ v_swz<HDP>(r)) * 16;
+    }
+    const char* kp = static_cast<const char*>(a.k);
+    const char* vp = static_cast<const char*>(a.v);
+    auto issue = [&](int t) __attribute__((always_inline)) {
+        const uint32_t to = slot + (t % NST) * 2 * TILE;
+        int64_t off[COPIES];
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) off[i] = offsets[wave][t * PG_K + (64 * i + lane) / CPR];
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i)
+            if (EXACT || kch[i] < 2 * hd) lds_copy16(kp + off[i] + kch[i], to + i * 1024);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i)
+            if (EXACT || vch[i] < 2 * hd) lds_copy16(vp + off[i] + vch[i], to + TILE + i * 1024);
     };
-    auto row_of = [&](int key, int id) -> int64_t {
-        return ((int64_t)id * a.Hkv + hk) * a.page + (uint32_t)key % (uint32_t)a.page;
-    };
-    // a tile in registers: K (and V) rows l16 and 16 + l16, and their scales
-    u4v kr[2][I8 ? KS / 2 : KS], vr[2][I8 ? KS / 2 : KS];
+    const float sl2 = a.scale * LOG2E;
+    for (Piece w; line.next(a, w);) {
+    if (!EXACT) {  // chunks past the head dim are never copied and stay zeros
+        for (int i = lane; i < SLOT / 16; i += 64) reinterpret_cast<u4v*>(lds + wave * SLOT)[i] = u4v{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    u4v qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, 32 * s + 8 * g, hd);
+    const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+    Sums<DT, Q> sums;
+    bool bad = w.over || a.pages == 0;
+    constexpr int STEP = WAVES * PG_K;
+    for (int sub = w.begin; sub < w.end && a.pages > 0; sub += WAVES * PG_IDS) {
+        const int stop = min(sub + WAVES * PG_IDS, w.end);
+        const int first = sub + wave * PG_K;
+        const int tiles = first < stop ? (stop - first + STEP - 1) / STEP : 0;
+        for (int e = lane; e < tiles * PG_K; e += 64) {
+            const int key = first + (e / PG_K) * STEP + (e % PG_K);
+            int64_t off = 0;  // row 0 stands in past the end and for a bad page: its score and values are dropped
+            if (key < stop) {
+                const uint32_t col = (uint32_t)key / (uint32_t)a.page;
+                const int id = table[col];  // the length lies within the table
+                if (id >= 0 && id < a.pages)
+                    off = (((int64_t)id * a.Hkv + w.hk) * a.page + (key - (int)(col * (uint32_t)a.page))) * (2 * hd);
+                else
+                    bad = true;
+            }
+            offsets[wave][e] = off;
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < NST; ++t)
+            if (t < tiles) issue(t);
+        for (int t = 0; t < tiles; ++t) {
+            // the copies of later tiles may still be under way
+            const int later = min(NST - 1, tiles - 1 - t);
+            if (later == 0) wait_vmcnt<0>();
+            else if (later == 1) wait_vmcnt<2 * COPIES>();
+            else if (later == 2) wait_vmcnt<(NST > 2 ? 4 : 0) * COPIES>();
+            else wait_vmcnt<(NST > 3 ? 6 : 0) * COPIES>();
+            asm volatile("" ::: "memory");
+            const uint32_t kt = slot + (t % NST) * 2 * TILE, vt = kt + TILE;
+            const int left = stop - (first + t * STEP);  // positions of this tile that exist
+            vf4 sc[2];
+#pragma unroll
+            for (int T = 0; T < 2; ++T) {
+                sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    sc[T] = mfma_16x16x32(Q{}, lds_read16(kt + (16 * T + l16) * ROW + (((4 * s + g) ^ (l16 & 7)) << 4)),
+                                          qf[s], sc[T]);
+            }
+            const bool whole = left >= PG_K;
+            if (!whole) {  // values past the end as zeros: their weight 0 must meet no infinity or NaN
+                const int r = lane & 31;
+                if (r >= left)
+                    for (int c = lane >> 5; c < CPR; c += 2)
+                        *reinterpret_cast<lds_u4v*>(vt + r * ROW + c * 16) = u4v{0, 0, 0, 0};
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+            sums.weights(sc, sl2, whole, left - 4 * g);
+            sums.template accumulate<ROW>(sc, vt, v_swz<HDP>);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
+            if (t + NST < tiles) issue(t + NST);
+        }
+    }
+    paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
+    }
+}
+
+// int8 cache.  Codes are exact in 16 bits: they are loaded to registers (a tile ahead), widened there,
+// and V goes to the wave's LDS as bfloat16.  The key's scale multiplies the score, the value's scale
+// the weight, which is bfloat16 for its range.  The widening bounds it: one and a half vector
+// instructions a code.
+template <int HDP, bool EXACT, class Q>
+__global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8_kernel(PagedArgs a) {
+    using P = ElemBF16;
+    constexpr int WAVES = PG_I8_WAVES, KS = HDP / 32, HALF = HDP / 64, DT = HDP / 16;
+    constexpr int ROW = HDP * 2, TILE = PG_K * ROW, OTILE = 16 * (HDP + 4) * 4;
+    constexpr int SLOT = (TILE > OTILE ? TILE : OTILE) + 256;  // + 64 scales
+    __shared__ __attribute__((aligned(16))) uint8_t lds[WAVES * SLOT];
+    __shared__ float ml[WAVES][2][16];
+    __shared__ int64_t scan[64 * WAVES + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int hd = EXACT ? HDP : a.hd;
+    Line<WAVES> line;
+    line.init(a, scan);
+    paged_empty<WAVES, Q>(a);
+    const float sl2 = a.scale * LOG2E;
+    uint8_t* slot = lds + wave * SLOT;
+    float* scales = reinterpret_cast<float*>(slot + SLOT - 256);
+    const uint32_t slot_at = (uint32_t)reinterpret_cast<uintptr_t>(slot);
+    for (Piece w; line.next(a, w);) {
+    // dims of this lane's eight slots in step s of the first product: a load brings 16 codes
+    auto dims = [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
+    u4v qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, dims(s), hd);
+    const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+    // page number of a position, -1 past the end
+    auto page_of = [&](int key) -> int { return key < w.end ? table[(uint32_t)key / (uint32_t)a.page] : -1; };
+    bool bad = w.over || a.pages == 0;
+    // a tile in registers: rows l16 and 16 + l16 of K and V, and their scales
+    u4v kr[2][HALF], vr[2][HALF];
     float ksc[2], vsc[2];
     auto fetch = [&](int key0, const int (&id)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
             const int key = key0 + 16 * T + l16;
             const bool ok = id[T] >= 0 && id[T] < a.pages;
-            bad |= key < end && !ok;
-            const int64_t row = ok ? row_of(key, id[T]) : 0;  // row 0 stands in: its scores and values are dropped
-            if constexpr (I8) {
-                const int8_t* kp = static_cast<const int8_t*>(a.k) + row * hd;
-                const int8_t* vp = static_cast<const int8_t*>(a.v) + row * hd;
-                ksc[T] = a.ks[row];
-                vsc[T] = a.vs[row];
+            bad |= key < w.end && !ok;
+            // row 0 stands in: its scores and values are dropped
+            const int64_t row = ok ? ((int64_t)id[T] * a.Hkv + w.hk) * a.page + (uint32_t)key % (uint32_t)a.page : 0;
+            const int8_t* kp = static_cast<const int8_t*>(a.k) + row * hd;
+            const int8_t* vp = static_cast<const int8_t*>(a.v) + row * hd;
+            ksc[T] = a.ks[row];
+            vsc[T] = a.vs[row];
+            auto load = [&](const int8_t* p, int d) {
+                if constexpr (EXACT) return *reinterpret_cast<const u4v*>(p + d);
+                const u2v lo = *reinterpret_cast<const u2v*>(p + (d < hd ? d : 0));
+                const u2v hi = *reinterpret_cast<const u2v*>(p + (d + 8 < hd ? d + 8 : 0));
+                return u4v{lo[0], lo[1], hi[0], hi[1]};
+            };
 #pragma unroll
-                for (int s = 0; s < KS / 2; ++s) {
-                    const int d = 64 * s + 16 * g;
-                    if constexpr (EXACT) {
-                        kr[T][s] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(kp + d));
-                        vr[T][s] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(vp + d));
-                    } else {
-                        const u2v k0 = *reinterpret_cast<const u2v*>(kp + (d < hd ? d : 0));
-                        const u2v k1 = *reinterpret_cast<const u2v*>(kp + (d + 8 < hd ? d + 8 : 0));
-                        const u2v v0 = *reinterpret_cast<const u2v*>(vp + (d < hd ? d : 0));
-                        const u2v v1 = *reinterpret_cast<const u2v*>(vp + (d + 8 < hd ? d + 8 : 0));
-                        kr[T][s] = u4v{k0[0], k0[1], k1[0], k1[1]};
-                        vr[T][s] = u4v{v0[0], v0[1], v1[0], v1[1]};
-                    }
-                }
-            } else {
-                const uint16_t* kp = static_cast<const uint16_t*>(a.k) + row * hd;
-                const uint16_t* vp = static_cast<const uint16_t*>(a.v) + row * hd;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int d = EXACT || dims(s) < hd ? dims(s) : 0;
-                    kr[T][s] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(kp + d));
-                    vr[T][s] = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(vp + d));
-                }
+            for (int s = 0; s < HALF; ++s) {
+                kr[T][s] = load(kp, 64 * s + 16 * g);
+                vr[T][s] = load(vp, 64 * s + 16 * g);
             }
         }
     };
-
-    vf4 o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.0f;
-    const float sl2 = a.scale * LOG2E;
-    uint8_t* slot = lds + wave * SLOT;
-    float* scales = reinterpret_cast<float*>(slot + SLOT - 256);
-    const uint32_t slot_at = (uint32_t)reinterpret_cast<uintptr_t>(slot);
-    // 16-byte chunk c of V row r lies at chunk c ^ swz(r): the writes (16 rows, 4 chunks) and the
-    // transposing reads (4 rows, 2 chunks a group) spread over the banks
-    auto swz = [](int r) { return HDP == 64 ? 2 * ((r >> 1) & 3) : HDP % 128 == 0 ? 2 * (r & 7) : 2 * (r & 3); };
-    const int vi = lane & 15, trow = 4 * g + (vi >> 2);
-    constexpr float SHIFT = WEIGHT_SHIFT<P>;
-
-    const int stride = PG_WAVES * PG_K;
-    int key0 = begin + wave * PG_K;
-    if (a.pages > 0 && key0 < end) {
+    Sums<DT, P> sums;
+    constexpr int STEP = WAVES * PG_K;
+    int key0 = w.begin + wave * PG_K;
+    if (a.pages > 0 && key0 < w.end) {
         int id[2], next[2];
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
             id[T] = page_of(key0 + 16 * T + l16);
-            next[T] = page_of(key0 + stride + 16 * T + l16);
+            next[T] = page_of(key0 + STEP + 16 * T + l16);
         }
         fetch(key0, id);
-        for (; key0 < end; key0 += stride) {
-            const bool whole = key0 + PG_K <= end && __all(!bad);
-            // scores
+        for (; key0 < w.end; key0 += STEP) {
+            const int left = w.end - key0;
+            const bool whole = left >= PG_K;
             vf4 sc[2];
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
                 sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    u4v kf;
-                    if constexpr (I8) {
-                        const u2v lo = widen4<Q>(kr[T][s >> 1][2 * (s & 1)]), hi = widen4<Q>(kr[T][s >> 1][2 * (s & 1) + 1]);
-                        kf = u4v{lo[0], lo[1], hi[0], hi[1]};
-                    } else {
-                        kf = kr[T][s];
-                    }
-                    if (!EXACT && dims(s) >= hd) kf = u4v{0, 0, 0, 0};
-                    sc[T] = mfma_16x16x32(Q{}, kf, qf[s], sc[T]);
+                    const uint32_t lo = kr[T][s >> 1][2 * (s & 1)], hi = kr[T][s >> 1][2 * (s & 1) + 1];
+                    const u2v x = widen4(Q{}, lo), y = widen4(Q{}, hi);
+                    sc[T] = mfma_16x16x32(Q{}, u4v{x[0], x[1], y[0], y[1]}, qf[s], sc[T]);  // codes past hd meet zeros
                 }
             }
-            // V into the wave's LDS (rows past the end as zeros)
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
                 const int r = 16 * T + l16;
-                const bool gone = !whole && (key0 + r >= end);
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    u4v w;
-                    if constexpr (I8) {
-                        const u2v lo = widen4<P>(vr[T][s >> 1][2 * (s & 1)]), hi = widen4<P>(vr[T][s >> 1][2 * (s & 1) + 1]);
-                        w = u4v{lo[0], lo[1], hi[0], hi[1]};
-                    } else {
-                        w = vr[T][s];
-                    }
-                    if (gone || (!EXACT && dims(s) >= hd)) w = u4v{0, 0, 0, 0};
-                    *reinterpret_cast<u4v*>(slot + r * VROW + (((dims(s) >> 3) ^ swz(r)) << 4)) = w;
+                    const uint32_t lo = vr[T][s >> 1][2 * (s & 1)], hi = vr[T][s >> 1][2 * (s & 1) + 1];
+                    const u2v x = widen4(P{}, lo), y = widen4(P{}, hi);
+                    *reinterpret_cast<u4v*>(slot + r * ROW + (((dims(s) >> 3) ^ v_swz<HDP>(r)) << 4)) =
+                        u4v{x[0], x[1], y[0], y[1]};
                 }
-                if constexpr (I8) {
-                    scales[r] = ksc[T];
-                    scales[32 + r] = gone ? 0.0f : vsc[T];
-                }
+                scales[r] = ksc[T];
+                scales[32 + r] = r < left ? vsc[T] : 0.0f;  // codes are finite: a weight of 0 drops them
             }
             // the next tile, and the page numbers of the one after it
-            if (key0 + stride < end) {
+            if (key0 + STEP < w.end) {
                 id[0] = next[0];
                 id[1] = next[1];
 #pragma unroll
-                for (int T = 0; T < 2; ++T) next[T] = page_of(key0 + 2 * stride + 16 * T + l16);
-                fetch(key0 + stride, id);
+                for (int T = 0; T < 2; ++T) next[T] = page_of(key0 + 2 * STEP + 16 * T + l16);
+                fetch(key0 + STEP, id);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's LDS writes, before any lane reads them
-            // weights
-            float mx = -INFINITY;
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
-                if constexpr (I8) sc[T] *= *reinterpret_cast<const vf4*>(scales + 16 * T + 4 * g);
+                const vf4 f = *reinterpret_cast<const vf4*>(scales + 16 * T + 4 * g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!whole && key0 + 16 * T + 4 * g + i >= end) sc[T][i] = -INFINITY;
-                    mx = fmaxf(mx, sc[T][i]);
-                }
+                for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
             }
-            mx = quarter_max(mx) * sl2;
-            if (__any(mx > m + RESCALE_AT)) {
-                const float mn = fmaxf(m, mx);
-                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
-                m = mn;
-                l *= corr;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= corr;
-            }
-            const float base = m == -INFINITY ? 0.0f : m - SHIFT;
-            u4v ph, pl;
+            sums.weights(sc, sl2, whole, left - 4 * g);
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
-                vf4 w;
+                const vf4 f = *reinterpret_cast<const vf4*>(scales + 32 + 16 * T + 4 * g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -base));
-                    l += w[i];
-                }
-                if constexpr (I8) w *= *reinterpret_cast<const vf4*>(scales + 32 + 16 * T + 4 * g);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t u = pack2(P{}, w[2 * i], w[2 * i + 1]);
-                    const f2v r = unpack2(P{}, u);
-                    ph[2 * T + i] = u;
-                    pl[2 * T + i] = pack2(P{}, w[2 * i] - r[0], w[2 * i + 1] - r[1]);
-                }
+                for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
             }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const uint32_t at = slot_at + trow * VROW + (((2 * d + ((vi & 3) >> 1)) ^ swz(trow)) << 4) + 8 * (vi & 1);
-                const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * VROW);
-                const u4v v = {lo[0], lo[1], hi[0], hi[1]};
-                o[d] = mfma_16x16x32(P{}, v, ph, o[d]);
-                o[d] = mfma_16x16x32(P{}, v, pl, o[d]);
-            }
+            sums.template accumulate<ROW>(sc, slot_at, v_swz<HDP>);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads, before the next tile's writes
         }
     }
-    l = quarter_sum(l);
-    if (__any(bad || (a.pages == 0 && begin < end))) l = __builtin_nanf("");
-    // the waves' sums meet
-    float* so = reinterpret_cast<float*>(slot);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<vf4*>(so + l16 * OROW + 16 * d + 4 * g) = o[d];
-    if (g == 0) {
-        mls[wave][0][l16] = m;
-        mls[wave][1][l16] = l;
-    }
-    __syncthreads();
-    for (int e = tid; e < heads * hd; e += 64 * PG_WAVES) {
-        const int r = e / hd, d = e - r * hd;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < PG_WAVES; ++w) M = fmaxf(M, mls[w][0][r]);
-        const float base = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f, x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < PG_WAVES; ++w) {
-            const float f = __builtin_amdgcn_exp2f(mls[w][0][r] - base);
-            L = __builtin_fmaf(f, mls[w][1][r], L);
-            x = __builtin_fmaf(f, reinterpret_cast<const float*>(lds + w * SLOT)[r * OROW + d], x);
-        }
-        const int64_t at = (int64_t)b * a.H + h0 + r;
-        if (used > 1) {
-            const int64_t pt = at * a.splits + split;
-            a.part_o[pt * hd + d] = x;
-            if (d == 0) {
-                a.part_ml[2 * pt] = M;
-                a.part_ml[2 * pt + 1] = L;
-            }
-        } else {
-            const float y = len || bad ? x / L : 0.0f;
-            if (a.out_f32) static_cast<float*>(a.out)[at * hd + d] = y;
-            else static_cast<typename Q::T*>(a.out)[at * hd + d] = Q::store(y);
-        }
+    paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
 }
 
-// The chunks of one (sequence, query head) joined: one workgroup, a thread per dim, the chunks' factors in
-// LDS 256 at a time.
+// The pieces of one (sequence, query head) joined by one workgroup: hd / 4 lanes take four dims each
+// of every (256 / (hd / 4))-th piece, and these sums meet in LDS.
 template <class Q>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     __shared__ float f[256], red[4];
+    __shared__ vf4 sums[256];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, b = blockIdx.y;
-    bool over;
-    int used;
-    sequence_length(a, b, over, used);
-    if (used <= 1) return;  // written by its one chunk
+    const int heads = a.Hkv * a.qtiles, hk = h / a.group, hq = hk * a.qtiles + (h - hk * a.group) / 16;
+    const int64_t steps = (a.bases[b + 1] - a.bases[b]) / heads, share = a.bases[a.B + 1];
+    if (steps == 0) return;
+    const int64_t first = a.bases[b] + hq * steps, w0 = first / share, w1 = (first + steps - 1) / share;
+    if (w0 == w1) return;  // one piece, written already
+    const int used = (int)(w1 - w0 + 1), row = (h - hk * a.group) % 16;
+    // piece s lies with workgroup w0 + s: its first one, unless that begins before this head does
+    auto piece = [&](int s) {
+        const int64_t w = w0 + s;
+        return 16 * (2 * w + (w * share < first ? 1 : 0)) + row;
+    };
     const int64_t at = (int64_t)b * a.H + h;
-    const float* ml = a.part_ml + 2 * at * a.splits;
-    const float* po = a.part_o + at * a.splits * a.hd;
+    const float* ml = a.part_ml;
+    const float* po = a.part_o;
+    const int quads = a.hd / 4, teams = 256 / quads, team = tid / quads, d = (tid - team * quads) * 4;
     float M = -INFINITY;
-    for (int s = tid; s < used; s += 256) M = fmaxf(M, ml[2 * s]);
+    for (int s = tid; s < used; s += 256) M = fmaxf(M, ml[2 * piece(s)]);
     for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
     if (lane == 0) red[tid >> 6] = M;
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, x = 0.0f;
+    float L = 0.0f;
+    vf4 x = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < used; s0 += 256) {
         const int n = min(256, used - s0);
         __syncthreads();
         float w = 0.0f;
         if (tid < n) {
-            const float e = __builtin_amdgcn_exp2f(ml[2 * (s0 + tid)] - base);
+            const float e = __builtin_amdgcn_exp2f(ml[2 * piece(s0 + tid)] - base);
             f[tid] = e;
-            w = e * ml[2 * (s0 + tid) + 1];
+            w = e * ml[2 * piece(s0 + tid) + 1];
         }
         w = ln_wave_sum(w);
         if (lane == 0) red[tid >> 6] = w;
         __syncthreads();
         L += (red[0] + red[1]) + (red[2] + red[3]);
-        if (tid < a.hd)
-            for (int s = 0; s < n; ++s) x = __builtin_fmaf(f[s], po[(int64_t)(s0 + s) * a.hd + tid], x);
+        if (team < teams) {
+#pragma unroll 8
+            for (int s = team; s < n; s += teams) {
+                const vf4 p = *reinterpret_cast<const vf4*>(po + piece(s0 + s) * a.hd + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(f[s], p[i], x[i]);
+            }
+        }
     }
-    if (tid < a.hd) {
-        const float y = x / L;
-        if (a.out_f32) static_cast<float*>(a.out)[at * a.hd + tid] = y;
-        else static_cast<typename Q::T*>(a.out)[at * a.hd + tid] = Q::store(y);
+    sums[tid] = x;
+    __syncthreads();
+    if (team == 0) {
+        for (int t = 1; t < teams; ++t) x += sums[t * quads + tid];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y = x[i] / L;
+            if (a.out_f32) static_cast<float*>(a.out)[at * a.hd + d + i] = y;
+            else static_cast<typename Q::T*>(a.out)[at * a.hd + d + i] = Q::store(y);
+        }
     }
 }
 
-// Positions of a workgroup and number of chunks: enough workgroups for the chip, whole tiles of
-// every wave, and no more chunks than the bound of the lengths asks for.
-struct Split {
-    int chunk, splits;
-};
-Split plan_split(int64_t B, int64_t H, int64_t Hkv, int64_t max_length) {
-    const int64_t rows = B * Hkv * ((H / Hkv + 15) / 16);
-    constexpr int64_t STEP = PG_WAVES * PG_K, WANT = 2048, LEAST = 4 * STEP;
-    int64_t chunk = rows > 0 ? (max_length * rows + WANT - 1) / WANT : 0;
-    chunk = (chunk + STEP - 1) / STEP * STEP;
-    if (chunk < LEAST) chunk = LEAST;
-    if (chunk > (1 << 30)) chunk = 1 << 30;
-    int64_t splits = (max_length + chunk - 1) / chunk;
-    return {(int)chunk, (int)(splits < 1 ? 1 : splits)};
-}
+// Workgroups of a call over long sequences: as many as run at a time (two to a CU; three of the int8
+// kernel's, one past 128 dims).  Up to PG_ALONE positions each workgroup takes a sequence whole: the
+// second launch would cost more than it gives (8 sequences of 640: 9.1 us against 12.5).
+constexpr int PG_GROUPS = 512, PG_GROUPS_I8 = 768, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
+int64_t paged_bases(int64_t B) { return (B + 3) / 2 * 2; }
+int paged_groups(int64_t hd, bool i8) { return i8 ? PG_GROUPS_I8 : hd <= 128 ? PG_GROUPS : PG_GROUPS_WIDE; }
 
 }  // namespace
 }  // namespace lq
@@ -583,9 +837,8 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
 }
 
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length) {
-    if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || max_length <= 0 || max_length > 0x7fffffff) return 0;
-    const Split s = plan_split(B, H, Hkv, max_length);
-    return s.splits > 1 ? (size_t)(B * H) * s.splits * (hd + 2) * sizeof(float) : 0;
+    if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || max_length <= PG_ALONE) return 0;
+    return (size_t)paged_bases(B) * sizeof(int64_t) + (size_t)2 * PG_GROUPS_I8 * 16 * (hd + 2) * sizeof(float);
 }
 
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
@@ -609,35 +862,61 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
     LQ_REQUIRE(cache_type != LQ_I8 || pages == 0 || (d_k_scale && d_v_scale),
                "lq_paged_attention: an int8 cache needs scales");
     LQ_REQUIRE(aligned16(d_k_pages) && aligned16(d_v_pages), "lq_paged_attention: pages must be 16-byte aligned");
-    const Split sp = plan_split(B, H, Hkv, max_length);
-    LQ_REQUIRE(sp.splits == 1 || (d_workspace && workspace_bytes >=
-                                      lq_paged_attention_workspace_size(B, H, Hkv, hd, max_length)),
-               "lq_paged_attention: workspace too small");
-    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16;
-    float* part_o = static_cast<float*>(d_workspace);
+    const bool alone = max_length <= PG_ALONE, i8_cache = cache_type == LQ_I8;
+    LQ_REQUIRE(alone || (d_workspace && aligned16(d_workspace) &&
+                         workspace_bytes >= lq_paged_attention_workspace_size(B, H, Hkv, hd, max_length)),
+               "lq_paged_attention: workspace too small or not 16-byte aligned");
+    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16, groups = alone ? 0 : paged_groups(hd, i8_cache);
+    const int64_t units = B * Hkv * qtiles;
+    LQ_REQUIRE(units <= 0x7fffffff, "lq_paged_attention: too many workgroups");
+    int64_t* bases = static_cast<int64_t*>(d_workspace);
+    float* part_o = alone ? nullptr : reinterpret_cast<float*>(bases + paged_bases(B));
     const PagedArgs a{d_q, ldq, (int)B, (int)H, (int)Hkv, (int)hd, group, qtiles, d_k_pages, d_v_pages, d_k_scale,
                       d_v_scale, pages, (int)page, d_table, table_stride, d_lengths, scale, d_out, out_type == LQ_F32,
-                      aligned16(d_q) && ldq % 8 == 0, sp.chunk, sp.splits, part_o, part_o ? part_o + B * H * sp.splits * hd : nullptr};
-    const dim3 grid((unsigned)(Hkv * qtiles), (unsigned)B, (unsigned)sp.splits), wg(64 * PG_WAVES);
+                      aligned16(d_q) && ldq % 8 == 0, groups, bases, part_o,
+                      alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
+    const dim3 grid((unsigned)(alone ? units : groups));
     const hipStream_t st = as_stream(stream);
+    // a few short sequences: four waves each, to hide more of the latency; else two, two workgroups to a CU
+    const bool few = alone && units <= 256;
     with_half(q_type, [&](auto q) {
         using Q = decltype(q);
-        auto go = [&](auto w, auto exact, auto c) {
-            hipLaunchKernelGGL((paged_tile_kernel<decltype(w)::value, decltype(exact)::value, Q, decltype(c)>), grid, wg,
-                               0, st, a);
+        auto i8 = [&](auto w, auto exact) {
+            hipLaunchKernelGGL((paged_i8_kernel<decltype(w)::value, decltype(exact)::value, Q>), grid,
+                               dim3(64 * PG_I8_WAVES), 0, st, a);
         };
-        auto width = [&](auto c) {
-            if (hd == 64) go(std::integral_constant<int, 64>{}, std::true_type{}, c);
-            else if (hd == 128) go(std::integral_constant<int, 128>{}, std::true_type{}, c);
-            else if (hd < 64) go(std::integral_constant<int, 64>{}, std::false_type{}, c);
-            else if (hd < 128) go(std::integral_constant<int, 128>{}, std::false_type{}, c);
-            else if (hd <= 192) go(std::integral_constant<int, 192>{}, std::false_type{}, c);
-            else go(std::integral_constant<int, 256>{}, std::false_type{}, c);
+        auto copy = [&](auto w, auto waves, auto nst, auto exact) {
+            hipLaunchKernelGGL((paged_copy_kernel<decltype(w)::value, decltype(waves)::value, decltype(nst)::value,
+                                                  decltype(exact)::value, Q>),
+                               grid, dim3(64 * decltype(waves)::value), 0, st, a);
         };
-        if (cache_type == LQ_I8) width(ElemI8{});
-        else width(Q{});
-        if (sp.splits > 1)
-            hipLaunchKernelGGL((paged_join_kernel<Q>), dim3((unsigned)H, (unsigned)B), dim3(256), 0, st, a);
+        const std::integral_constant<int, 2> two{};
+        const std::integral_constant<int, 4> four{};
+        const std::integral_constant<int, 64> w64{};
+        const std::integral_constant<int, 128> w128{};
+        const std::integral_constant<int, 192> w192{};
+        const std::integral_constant<int, 256> w256{};
+        if (cache_type == LQ_I8) {
+            if (hd == 64) i8(w64, std::true_type{});
+            else if (hd == 128) i8(w128, std::true_type{});
+            else if (hd < 64) i8(w64, std::false_type{});
+            else if (hd < 128) i8(w128, std::false_type{});
+            else if (hd <= 192) i8(w192, std::false_type{});
+            else i8(w256, std::false_type{});
+        } else if (hd <= 64) {
+            if (few) hd == 64 ? copy(w64, four, four, std::true_type{}) : copy(w64, four, four, std::false_type{});
+            else hd == 64 ? copy(w64, two, four, std::true_type{}) : copy(w64, two, four, std::false_type{});
+        } else if (hd <= 128) {
+            if (few) hd == 128 ? copy(w128, four, two, std::true_type{}) : copy(w128, four, two, std::false_type{});
+            else hd == 128 ? copy(w128, two, two, std::true_type{}) : copy(w128, two, two, std::false_type{});
+        } else if (hd <= 192) {
+            copy(w192, two, two, std::false_type{});
+        } else {
+            copy(w256, two, two, std::false_type{});
+        }
+        if (alone) return;
+        const dim3 rows((unsigned)H, (unsigned)B);
+        hipLaunchKernelGGL((paged_join_kernel<Q>), rows, dim3(256), 0, st, a);
     });
     return launch_status("lq_paged_attention");
 }

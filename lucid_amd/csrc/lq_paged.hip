@@ -190,7 +190,7 @@ struct PagedArgs {
     int out_f32;
     int q_vec;          // q may be read 16 bytes at a time
     int groups;         // workgroups that share all positions evenly; 0: one per sequence and key head
-    int64_t* bases;     // [B + 1] first step of each sequence, then the steps of a workgroup
+    int2* pieces;       // [B][key head and tile of query heads]: first piece's slot, number of pieces
     float *part_o, *part_ml;
 };
 
@@ -208,9 +208,10 @@ __device__ __forceinline__ int sequence_length(const PagedArgs& a, int b, bool& 
 // The two kernels share this plan.  The work is a line of steps (WAVES tiles of 32 positions): all steps
 // of the first sequence's first key head (and tile of 16 query heads), then of its next one, and so
 // on.  Each workgroup takes an equal part of the line, whatever the sequences' lengths, and works
-// through the pieces of sequences in it one after the other: a piece costs some microseconds of
-// dependent loads before its first tile (512 positions a workgroup took 109 us where 1024 took 102,
-// 64 sequences of 2048), and unequal parts leave the chip waiting for the longest.  A piece that is
+// through the pieces of sequences in it one after the other.  A piece costs some microseconds of dependent
+// loads before its first tile, which counts as START steps on the line (without it 64 sequences of 256 to
+// 8191 positions took 128 us, with it 110).  Where parts of 256 or 512 positions are enough for all, each
+// lies within one sequence instead.  A piece that is
 // a whole sequence is written at once, others go to the workspace (a workgroup has two at most, its first
 // and its last) and are joined by a second launch.  With short sequences (`groups` 0) a workgroup takes
 // one of them whole and there is no second launch.
@@ -232,33 +233,59 @@ struct Piece {
 // The line of steps as a workgroup walks it.
 template <int WAVES>
 struct Line {
-    static constexpr int STEP = WAVES * PG_K, NT = 64 * WAVES, LEAST = 512 / STEP;
-    int64_t at, stop, start, base;  // next step, end and start of this part; first step of sequence b
-    int b, len, steps, heads;       // heads: key heads times tiles of 16 query heads
+    static constexpr int STEP = WAVES * PG_K, NT = 64 * WAVES, START = 256 / STEP;
+    int64_t share, at, stop, start, base;  // steps of a workgroup; next step, end and start of this part; first step of sequence b
+    int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
+    int cost;                  // places of one head of sequence b on the line
+    int unit, lead;            // steps that a part is a multiple of (0: any), places before a head's first step
     bool over;
 
     __device__ __forceinline__ void sequence(const PagedArgs& a, int i) {
         b = i;
         len = sequence_length(a, i, over);
         steps = (len + STEP - 1) / STEP;
+        cost = unit ? (steps + unit - 1) / unit * unit : steps ? steps + START : 0;
     }
-    // Finds the part of workgroup blockIdx.x; `scan` holds NT + 1 numbers.
+    // Sum over the workgroup's threads; `sums` holds WAVES numbers.
+    __device__ __forceinline__ static int64_t add_all(int64_t v, int64_t* sums) {
+        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0;
+        for (int w = 0; w < WAVES; ++w) v += sums[w];
+        return v;
+    }
+    // Finds the part of workgroup blockIdx.x; `scan` holds NT numbers.
     __device__ __forceinline__ void init(const PagedArgs& a, int64_t* scan) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         heads = a.Hkv * a.qtiles;
+        unit = 0;
         if (a.groups == 0) {
+            lead = START;
             const int i = blockIdx.x / heads;
             sequence(a, i);
             base = 0;
-            start = at = (int64_t)(blockIdx.x - i * heads) * steps;
-            stop = at + steps;
+            start = at = (int64_t)(blockIdx.x - i * heads) * cost;
+            stop = at + cost;
             return;
         }
         const int per = (a.B + NT - 1) / NT, first = min(tid * per, a.B), last = min(first + per, a.B);
+        // parts of 256 or 512 positions, if the workgroups suffice: none then has two pieces
+        int64_t small = 0, large = 0;
+        for (int i = first; i < last; ++i) {
+            sequence(a, i);
+            small += (int64_t)heads * ((steps + 256 / STEP - 1) / (256 / STEP));
+            large += (int64_t)heads * ((steps + 512 / STEP - 1) / (512 / STEP));
+        }
+        small = add_all(small, scan);
+        large = add_all(large, scan);
+        unit = small <= a.groups ? 256 / STEP : large <= a.groups ? 512 / STEP : 0;
+        lead = unit ? 0 : START;
         int64_t mine = 0;
         for (int i = first; i < last; ++i) {
             sequence(a, i);
-            mine += (int64_t)heads * steps;
+            mine += (int64_t)heads * cost;
         }
         int64_t upto = mine;
 #pragma unroll
@@ -266,6 +293,7 @@ struct Line {
             const int64_t o = __shfl_up(upto, d, 64);
             if (lane >= d) upto += o;
         }
+        __syncthreads();
         scan[tid] = upto;
         __syncthreads();
         int64_t before = upto - mine;
@@ -274,20 +302,7 @@ struct Line {
         for (int w = 0; w < WAVES; ++w) total += scan[64 * w + 63];
         __syncthreads();
         scan[tid] = before;
-        if (tid == 0) scan[NT] = total;
-        int64_t share = (total + a.groups - 1) / a.groups;
-        share = share < LEAST ? LEAST : share;
-        if (blockIdx.x == 0) {
-            for (int i = first; i < last; ++i) {
-                a.bases[i] = before;
-                sequence(a, i);
-                before += (int64_t)heads * steps;
-            }
-            if (tid == 0) {
-                a.bases[a.B] = total;
-                a.bases[a.B + 1] = share;
-            }
-        }
+        share = unit ? unit : (total + a.groups - 1) / a.groups;
         __syncthreads();
         start = at = min((int64_t)blockIdx.x * share, total);
         stop = min(at + share, total);
@@ -299,33 +314,43 @@ struct Line {
         }
         base = scan[lo];
         sequence(a, lo * per);
-        while (at >= base + (int64_t)heads * steps) {
-            base += (int64_t)heads * steps;
+        advance(a);
+    }
+    __device__ __forceinline__ void advance(const PagedArgs& a) {
+        while (at >= base + (int64_t)heads * cost) {
+            base += (int64_t)heads * cost;
             sequence(a, b + 1);
         }
     }
     // The next piece; false when the part is done.  Uniform over the workgroup.
     __device__ __forceinline__ bool next(const PagedArgs& a, Piece& p) {
-        if (at >= stop) return false;
-        while (at >= base + (int64_t)heads * steps) {
-            base += (int64_t)heads * steps;
-            sequence(a, b + 1);
+        while (at < stop) {
+            advance(a);
+            const int hq = (int)((at - base) / cost), x0 = (int)(at - base - (int64_t)hq * cost);
+            const int x1 = (int)min((int64_t)cost, x0 + (stop - at));
+            const int s0 = max(x0 - lead, 0), s1 = min(x1 - lead, steps);
+            const bool first = at == start;
+            at += x1 - x0;
+            if (s1 <= 0) continue;  // nothing but the start of a sequence whose steps come in the next part
+            const int qt = hq % a.qtiles;
+            p.b = b;
+            p.hk = hq / a.qtiles;
+            p.heads = min(16, a.group - 16 * qt);
+            p.h0 = p.hk * a.group + 16 * qt;
+            p.len = len;
+            p.over = over;
+            p.begin = s0 * STEP;
+            p.end = min(s1 * STEP, len);
+            p.whole = s1 - s0 == steps;
+            p.slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+            if (a.groups && s0 == 0 && threadIdx.x == 0) {  // for the join
+                const int64_t end = base + (int64_t)hq * cost + lead + steps - 1;  // its last step
+                const int more = p.whole ? 0 : (int)(end / share) - (int)blockIdx.x;
+                a.pieces[(int64_t)b * heads + hq] = make_int2((int)p.slot, more + 1);
+            }
+            return true;
         }
-        const int hq = (int)((at - base) / steps), s0 = (int)(at - base - (int64_t)hq * steps);
-        const int n = (int)min((int64_t)(steps - s0), stop - at);
-        const int qt = hq % a.qtiles;
-        p.b = b;
-        p.hk = hq / a.qtiles;
-        p.heads = min(16, a.group - 16 * qt);
-        p.h0 = p.hk * a.group + 16 * qt;
-        p.len = len;
-        p.over = over;
-        p.begin = s0 * STEP;
-        p.end = min((s0 + n) * STEP, len);
-        p.whole = n == steps;
-        p.slot = 2 * (int64_t)blockIdx.x + (at == start ? 0 : 1);
-        at += n;
-        return true;
+        return false;
     }
 };
 
@@ -337,6 +362,9 @@ __device__ __forceinline__ void paged_empty(const PagedArgs& a) {
         bool over;
         if (sequence_length(a, b, over) > 0) continue;
         const float y = over ? __builtin_nanf("") : 0.0f;
+        const int heads = a.Hkv * a.qtiles;
+        if (a.groups)
+            for (int e = threadIdx.x; e < heads; e += 64 * WAVES) a.pieces[(int64_t)b * heads + e] = make_int2(0, 0);
         for (int64_t e = threadIdx.x; e < row; e += 64 * WAVES) {
             if (a.out_f32) static_cast<float*>(a.out)[b * row + e] = y;
             else static_cast<typename Q::T*>(a.out)[b * row + e] = Q::store(y);
@@ -485,7 +513,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOT];
     __shared__ int64_t offsets[WAVES][PG_IDS];
     __shared__ float ml[WAVES][2][16];
-    __shared__ int64_t scan[64 * WAVES + 1];
+    __shared__ int64_t scan[64 * WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;
@@ -502,6 +530,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     }
     const char* kp = static_cast<const char*>(a.k);
     const char* vp = static_cast<const char*>(a.v);
+    // every copy instruction covers a whole row at least, so that some lane of it is on whatever the head
+    // dim: the waits below count instructions
     auto issue = [&](int t) __attribute__((always_inline)) {
         const uint32_t to = slot + (t % NST) * 2 * TILE;
         int64_t off[COPIES];
@@ -549,8 +579,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
         for (int t = 0; t < NST; ++t)
             if (t < tiles) issue(t);
         for (int t = 0; t < tiles; ++t) {
-            // the copies of later tiles may still be under way
-            const int later = min(NST - 1, tiles - 1 - t);
+            const int later = min(NST - 1, tiles - 1 - t);  // tiles that may still be on their way
+            static_assert(NST <= 4 && 2 * (NST - 1) * COPIES < 64, "the counter's range");
             if (later == 0) wait_vmcnt<0>();
             else if (later == 1) wait_vmcnt<2 * COPIES>();
             else if (later == 2) wait_vmcnt<(NST > 2 ? 4 : 0) * COPIES>();
@@ -568,6 +598,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
                                           qf[s], sc[T]);
             }
             const bool whole = left >= PG_K;
+            sums.weights(sc, sl2, whole, left - 4 * g);
             if (!whole) {  // values past the end as zeros: their weight 0 must meet no infinity or NaN
                 const int r = lane & 31;
                 if (r >= left)
@@ -575,7 +606,6 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
                         *reinterpret_cast<lds_u4v*>(vt + r * ROW + c * 16) = u4v{0, 0, 0, 0};
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
-            sums.weights(sc, sl2, whole, left - 4 * g);
             sums.template accumulate<ROW>(sc, vt, v_swz<HDP>);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
             if (t + NST < tiles) issue(t + NST);
@@ -597,7 +627,7 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8
     constexpr int SLOT = (TILE > OTILE ? TILE : OTILE) + 256;  // + 64 scales
     __shared__ __attribute__((aligned(16))) uint8_t lds[WAVES * SLOT];
     __shared__ float ml[WAVES][2][16];
-    __shared__ int64_t scan[64 * WAVES + 1];
+    __shared__ int64_t scan[64 * WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;
@@ -721,16 +751,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     __shared__ vf4 sums[256];
     const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.x, b = blockIdx.y;
     const int heads = a.Hkv * a.qtiles, hk = h / a.group, hq = hk * a.qtiles + (h - hk * a.group) / 16;
-    const int64_t steps = (a.bases[b + 1] - a.bases[b]) / heads, share = a.bases[a.B + 1];
-    if (steps == 0) return;
-    const int64_t first = a.bases[b] + hq * steps, w0 = first / share, w1 = (first + steps - 1) / share;
-    if (w0 == w1) return;  // one piece, written already
-    const int used = (int)(w1 - w0 + 1), row = (h - hk * a.group) % 16;
-    // piece s lies with workgroup w0 + s: its first one, unless that begins before this head does
-    auto piece = [&](int s) {
-        const int64_t w = w0 + s;
-        return 16 * (2 * w + (w * share < first ? 1 : 0)) + row;
-    };
+    const int2 info = a.pieces[(int64_t)b * heads + hq];
+    const int used = info.y, row = (h - hk * a.group) % 16;
+    if (used <= 1) return;  // written already
+    // the first piece, then the first ones of the workgroups that follow
+    auto piece = [&](int s) { return (int64_t)16 * (s == 0 ? info.x : (info.x & ~1) + 2 * s) + row; };
     const int64_t at = (int64_t)b * a.H + h;
     const float* ml = a.part_ml;
     const float* po = a.part_o;
@@ -779,12 +804,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     }
 }
 
-// Workgroups of a call over long sequences: as many as run at a time (two to a CU; three of the int8
-// kernel's, one past 128 dims).  Up to PG_ALONE positions each workgroup takes a sequence whole: the
+// Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims).  Up to PG_ALONE positions each workgroup takes a sequence whole: the
 // second launch would cost more than it gives (8 sequences of 640: 9.1 us against 12.5).
-constexpr int PG_GROUPS = 512, PG_GROUPS_I8 = 768, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
-int64_t paged_bases(int64_t B) { return (B + 3) / 2 * 2; }
-int paged_groups(int64_t hd, bool i8) { return i8 ? PG_GROUPS_I8 : hd <= 128 ? PG_GROUPS : PG_GROUPS_WIDE; }
+constexpr int PG_GROUPS = 512, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
+// bytes of the table of pieces, and the slots of a call (two to a workgroup)
+int64_t pieces_bytes(int64_t units) { return (units * (int64_t)sizeof(int2) + 15) / 16 * 16; }
+int paged_groups(int64_t hd) { return hd <= 128 ? PG_GROUPS : PG_GROUPS_WIDE; }
 
 }  // namespace
 }  // namespace lq
@@ -838,7 +863,7 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
 
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length) {
     if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || max_length <= PG_ALONE) return 0;
-    return (size_t)paged_bases(B) * sizeof(int64_t) + (size_t)2 * PG_GROUPS_I8 * 16 * (hd + 2) * sizeof(float);
+    return (size_t)pieces_bytes(B * Hkv * ((H / Hkv + 15) / 16)) + (size_t)2 * paged_groups(hd) * 16 * (hd + 2) * sizeof(float);
 }
 
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
@@ -862,18 +887,18 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
     LQ_REQUIRE(cache_type != LQ_I8 || pages == 0 || (d_k_scale && d_v_scale),
                "lq_paged_attention: an int8 cache needs scales");
     LQ_REQUIRE(aligned16(d_k_pages) && aligned16(d_v_pages), "lq_paged_attention: pages must be 16-byte aligned");
-    const bool alone = max_length <= PG_ALONE, i8_cache = cache_type == LQ_I8;
+    const bool alone = max_length <= PG_ALONE;
     LQ_REQUIRE(alone || (d_workspace && aligned16(d_workspace) &&
                          workspace_bytes >= lq_paged_attention_workspace_size(B, H, Hkv, hd, max_length)),
                "lq_paged_attention: workspace too small or not 16-byte aligned");
-    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16, groups = alone ? 0 : paged_groups(hd, i8_cache);
+    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16, groups = alone ? 0 : paged_groups(hd);
     const int64_t units = B * Hkv * qtiles;
     LQ_REQUIRE(units <= 0x7fffffff, "lq_paged_attention: too many workgroups");
-    int64_t* bases = static_cast<int64_t*>(d_workspace);
-    float* part_o = alone ? nullptr : reinterpret_cast<float*>(bases + paged_bases(B));
+    char* ws = static_cast<char*>(d_workspace);
+    float* part_o = alone ? nullptr : reinterpret_cast<float*>(ws + pieces_bytes(units));
     const PagedArgs a{d_q, ldq, (int)B, (int)H, (int)Hkv, (int)hd, group, qtiles, d_k_pages, d_v_pages, d_k_scale,
                       d_v_scale, pages, (int)page, d_table, table_stride, d_lengths, scale, d_out, out_type == LQ_F32,
-                      aligned16(d_q) && ldq % 8 == 0, groups, bases, part_o,
+                      aligned16(d_q) && ldq % 8 == 0, groups, reinterpret_cast<int2*>(ws), part_o,
                       alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
     const dim3 grid((unsigned)(alone ? units : groups));
     const hipStream_t st = as_stream(stream);

@@ -82,16 +82,38 @@ __global__ __launch_bounds__(64) void prompt_rows_kernel(PromptArgs a) {
 
 constexpr int PT_WAVES = 4, PT_Q = 32 * PT_WAVES, PT_K = 64;  // queries of a workgroup, keys of a tile
 
-// Sequence and query block of workgroup index n (blocks of a sequence last to first: under the
-// causal mask the later ones have more keys, and the longest work starts first); false past the
-// last block.  Every wave finds it by a scan over 64 sequences at a time.
+// Sequence and query block of workgroup index n; false past the last block.  Under the causal mask later
+// blocks have more keys, and the longest work starts first: up to 64 sequences, block L of every
+// sequence that has one before any block L - 1 (at the count of blocks from L on, which a search
+// finds); with more, blocks last to first within each sequence.  Every wave finds it by itself, a lane
+// for each of 64 sequences.
 __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64_t& seq, int64_t& blk) {
     const int lane = threadIdx.x & 63;
+    auto blocks = [&](int64_t s) {
+        return s < a.seqs ? (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + PT_Q - 1) / PT_Q) : 0;
+    };
+    if (a.seqs <= 64) {
+        const int cnt = blocks(lane);
+        auto from = [&](int level) {  // blocks at or past a level
+            int v = max(cnt - level, 0);
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+            return v;
+        };
+        if (n >= from(0)) return false;
+        int lo = 0, hi = wave_max(cnt);  // from(lo) > n >= from(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (from(mid) > n) lo = mid; else hi = mid;
+        }
+        uint64_t has = __ballot(cnt > lo);
+        for (int64_t k = n - from(lo + 1); k > 0; --k) has &= has - 1;
+        seq = __builtin_ctzll(has);
+        blk = lo;
+        return true;
+    }
     for (int64_t base = 0; base < a.seqs; base += 64) {
-        const int64_t s = base + lane;
-        int cnt = 0;
-        if (s < a.seqs) cnt = (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + PT_Q - 1) / PT_Q);
-        int upto = cnt;
+        int upto = blocks(base + lane);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(upto, d, 64);
@@ -153,11 +175,13 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
     uint32_t koff[COPIES], voff[COPIES];
     const uint32_t ldk = (uint32_t)a.ldk * 2, ldv = (uint32_t)a.ldv * 2;
-    auto vswz = [](int r) { return CPR == 8 ? 2 * ((r >> 1) & 3) : CPR % 16 == 0 ? 2 * (r & 7) : 2 * (r & 3); };
+    // (64 banks: 16 rows' 16-byte chunks at a time for K, 4 rows' 64 bytes for V; no conflicts at 64, 128 and 256)
+    auto k_swz = [](int r) { return CPR == 8 ? (r >> 1) & 7 : CPR % 16 == 0 ? r & 15 : r & 7; };
+    auto v_swz = [](int r) { return CPR == 8 ? 4 * ((r >> 1) & 1) : CPR % 16 == 0 ? 4 * (r & 3) : 4 * (r & 1); };
 #pragma unroll
     for (int j = 0; j < COPIES; ++j) {
         const int slot = (j * PT_WAVES + wave) * 64 + lane, r = slot / CPR, x = slot % CPR;
-        const int ck = x ^ (r & 7), cv = x ^ vswz(r);
+        const int ck = x ^ k_swz(r), cv = x ^ v_swz(r);
         koff[j] = 8 * ck < hd ? r * ldk + ck * 16 : 0x80000000u;  // past the head dim: out of range, read as 0
         voff[j] = 8 * cv < hd ? r * ldv + cv * 16 : 0x80000000u;
     }
@@ -198,14 +222,15 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
         const uint32_t buf = (t & 1) * 2 * TILE;
         f16v sc[KT];
 #pragma unroll
-        for (int b = 0; b < KT; ++b) {
+        for (int b = 0; b < KT; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ (col & 7)) << 4)),
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int b = 0; b < KT; ++b)
+                sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)),
                                       qf[s], sc[b]);
-        }
         if constexpr (MASKED) {
             const int left = lim - kb - 4 * hh;
 #pragma unroll
@@ -248,7 +273,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 }
             }
         auto value = [&](int d, int ks) __attribute__((always_inline)) {
-            const uint32_t at = vrow + buf + ks * 16 * HDP * 2 + (((4 * d + vc) ^ vswz(vr)) << 4);
+            const uint32_t at = vrow + buf + ks * 16 * HDP * 2 + (((4 * d + vc) ^ v_swz(vr)) << 4);
             const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * HDP * 2);
             return u4v{lo[0], lo[1], hi[0], hi[1]};
         };
@@ -265,9 +290,9 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
             careful |= odd & 0x80008000u;
         }
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int ks = 0; ks < 2 * KT; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < 2 * KT; ++ks) {
+            for (int d = 0; d < DT; ++d) {
                 const u4v v = value(d, ks);
                 o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
                 if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);

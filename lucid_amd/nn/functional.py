@@ -14,6 +14,7 @@ from lucid_amd._tensor import Tensor, empty, float32
 from lucid_amd.nn.generation import (  # noqa: F401  (part of this module's surface)
     paged_attention,
     paged_kv_append,
+    paged_kv_append_qkv,
     prompt_attention,
     prompt_attention_qkv,
     token_logprobs,

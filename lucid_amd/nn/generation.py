@@ -100,6 +100,27 @@ def paged_kv_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, tabl
             _CACHE_TYPE[k_pages.dtype], _opt(k_scale), _opt(v_scale), pages, page, stream)
 
 
+def paged_kv_append_qkv(qkv: Tensor, heads: int, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
+                        starts: Tensor | None = None, k_scale: Tensor | None = None, v_scale: Tensor | None = None,
+                        stream=None) -> None:
+    """:func:`paged_kv_append` of a fused projection's rows ``[tokens, heads + 2 kv_heads,
+    head_dim]`` (queries, keys, values), read in place."""
+    op = "paged_kv_append_qkv"
+    pages, hkv, page, hd = _pages(op, k_pages, v_pages, k_scale, v_scale, table, lengths)
+    dt = _need(qkv, op, "qkv", 3, tuple(FLOAT_TYPE_CODE))
+    if heads < 1 or tuple(qkv.shape[1:]) != (heads + 2 * hkv, hd):
+        raise ValueError(f"{op}: qkv {tuple(qkv.shape)} for {heads} heads and {hkv} key heads of {hd}")
+    seqs, tokens = int(table.shape[0]), int(qkv.shape[0])
+    if starts is not None:
+        _ints(starts, op, "starts", seqs + 1)
+    elif tokens != seqs:
+        raise ValueError(f"{op}: {tokens} tokens for {seqs} sequences need starts")
+    k = qkv.data_ptr() + heads * hd * dt.itemsize
+    _C.call("lq_paged_kv_append", k, k + hkv * hd * dt.itemsize, FLOAT_TYPE_CODE[dt], (heads + 2 * hkv) * hd, tokens,
+            _opt(starts), seqs, hkv, hd, table.data_ptr(), table.shape[1], lengths.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), _CACHE_TYPE[k_pages.dtype], _opt(k_scale), _opt(v_scale), pages, page, stream)
+
+
 def _out_type(out_dtype, dt, op: str) -> np.dtype:
     out = np.dtype(out_dtype) if out_dtype is not None else dt
     if out not in (dt, float32):
@@ -116,20 +137,24 @@ def _scale(scale, hd: int, op: str) -> float:
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, max_length: int,
                     scale: float | None = None, k_scale: Tensor | None = None, v_scale: Tensor | None = None,
-                    out_dtype=None, stream=None) -> Tensor:
+                    out_dtype=None, stream=None, heads: int | None = None) -> Tensor:
     """Attention of one new token per sequence, ``q`` [seqs, heads, head_dim], over its pages;
-    ``max_length`` is the host's bound of ``lengths``.  See ``lq_paged_attention``."""
+    ``max_length`` is the host's bound of ``lengths``.  With ``heads`` the queries are the first
+    heads of wider rows (a fused projection's).  See ``lq_paged_attention``."""
     op = "paged_attention"
     pages, hkv, page, hd = _pages(op, k_pages, v_pages, k_scale, v_scale, table, lengths)
     dt = _need(q, op, "q", 3, (float16, bfloat16))
-    B, h = int(q.shape[0]), int(q.shape[1])
+    B, ldq = int(q.shape[0]), int(q.shape[1]) * hd
+    h = int(q.shape[1]) if heads is None else heads
+    if not 0 < h <= q.shape[1]:
+        raise ValueError(f"{op}: {h} heads of q {tuple(q.shape)}")
     if q.shape[2] != hd or B != table.shape[0] or h % hkv:
         raise ValueError(f"{op}: q {tuple(q.shape)} does not fit {table.shape[0]} sequences, {hkv} key heads of {hd}")
     if k_pages.dtype not in (dt, np.dtype(np.int8)):
         raise TypeError(f"{op}: a cache of {k_pages.dtype} for queries of {dt}")
     out = empty((B, h, hd), _out_type(out_dtype, dt, op), "gpu")
     size = _C.lib().lq_paged_attention_workspace_size(B, h, hkv, hd, max_length)
-    _C.call("lq_paged_attention", q.data_ptr(), FLOAT_TYPE_CODE[dt], h * hd, B, h, hkv, hd, k_pages.data_ptr(),
+    _C.call("lq_paged_attention", q.data_ptr(), FLOAT_TYPE_CODE[dt], ldq, B, h, hkv, hd, k_pages.data_ptr(),
             v_pages.data_ptr(), _CACHE_TYPE[k_pages.dtype], _opt(k_scale), _opt(v_scale), pages, page, table.data_ptr(),
             table.shape[1], lengths.data_ptr(), max_length, _scale(scale, hd, op), out.data_ptr(),
             FLOAT_TYPE_CODE[out.dtype], workspace.get(size), size, stream)
@@ -251,6 +276,11 @@ class PageTable:
     def host_lengths(self) -> np.ndarray:
         return self._lengths.copy()
 
+    def rows(self, seqs) -> tuple[Tensor, Tensor]:
+        """Copies of some sequences' table rows and lengths."""
+        return (tensor(np.ascontiguousarray(self._table[seqs]), device="gpu"),
+                tensor(np.ascontiguousarray(self._lengths[seqs]), device="gpu"))
+
     def grow(self, counts) -> None:
         """``counts[s]`` more positions for every sequence: takes pages as needed and uploads the
         table and the lengths.  Nothing changes when the free pages do not suffice."""
@@ -304,8 +334,12 @@ class PagedKVCache:
         paged_kv_append(k, v, self.k, self.v, self.pages.table, self.pages.lengths, starts, self.k_scale, self.v_scale,
                         stream)
 
+    def append_qkv(self, qkv: Tensor, heads: int, starts: Tensor | None = None, stream=None) -> None:
+        paged_kv_append_qkv(qkv, heads, self.k, self.v, self.pages.table, self.pages.lengths, starts, self.k_scale,
+                            self.v_scale, stream)
+
     def attend(self, q: Tensor, scale: float | None = None, out_dtype=None, max_length: int | None = None,
-               stream=None) -> Tensor:
+               stream=None, heads: int | None = None) -> Tensor:
         return paged_attention(q, self.k, self.v, self.pages.table, self.pages.lengths,
                                self.pages.max_length if max_length is None else max_length, scale, self.k_scale,
-                               self.v_scale, out_dtype, stream)
+                               self.v_scale, out_dtype, stream, heads)

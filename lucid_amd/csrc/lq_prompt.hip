@@ -80,17 +80,18 @@ __global__ __launch_bounds__(64) void prompt_rows_kernel(PromptArgs a) {
 
 // ------------------------------------------------------------------------- the tile kernel
 
-constexpr int PT_WAVES = 4, PT_Q = 32 * PT_WAVES, PT_K = 64;  // queries of a workgroup, keys of a tile
+constexpr int PT_WAVES = 4, PT_K = 64;  // waves of a workgroup, keys of a tile
 
 // Sequence and query block of workgroup index n; false past the last block.  Under the causal mask later
 // blocks have more keys, and the longest work starts first: up to 64 sequences, block L of every
 // sequence that has one before any block L - 1 (at the count of blocks from L on, which a search
 // finds); with more, blocks last to first within each sequence.  Every wave finds it by itself, a lane
 // for each of 64 sequences.
+template <int QB>
 __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64_t& seq, int64_t& blk) {
     const int lane = threadIdx.x & 63;
     auto blocks = [&](int64_t s) {
-        return s < a.seqs ? (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + PT_Q - 1) / PT_Q) : 0;
+        return s < a.seqs ? (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + QB - 1) / QB) : 0;
     };
     if (a.seqs <= 64) {
         const int cnt = blocks(lane);
@@ -131,14 +132,26 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64
     return false;
 }
 
-template <int HDP, class E, class Out>
+// A workgroup of four waves; SPLIT of them share 32 queries and take 64 / SPLIT keys of a tile each, so
+// that it has QB = 128 / SPLIT queries.  K and V tiles are copied to LDS one ahead (three ahead, with one
+// workgroup to a CU, was no faster where few workgroups run and slower elsewhere).
+//   S^T = K Q^T (v_mfma 32x32x16): a lane receives 16 keys of one query, so the softmax statistics are one
+//   number a lane;
+//   O^T += V^T P^T: those weights are the B operand as they are (no exchange between lanes), and V^T is
+//   what the transposing read of the V rows gives.  A rescale is one factor a lane.
+// What bounds it: the matrix cores are busy half of the time at the 1.9 GHz that the card keeps under
+// this load, the vector unit's work on the weights (exponential, sum, rounding) the other half; the
+// two waves of a SIMD overlap them only in part.
+template <int HDP, int SPLIT, class E, class Out>
 __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile_kernel(PromptArgs a) {
+    constexpr int QB = 32 * PT_WAVES / SPLIT;
     constexpr int CPR = HDP / 8;                                // 16-byte chunks of a row
     constexpr int TILE = PT_K * HDP * 2;                        // bytes of a K (or V) tile
     constexpr int COPIES = PT_K * CPR / (64 * PT_WAVES);        // 16-byte copies of a lane per tile
-    constexpr int KS = HDP / 16, DT = HDP / 32, KT = PT_K / 32;
+    constexpr int KS = HDP / 16, DT = HDP / 32, KT = PT_K / 32 / SPLIT;
     constexpr bool TWO = Out::code == LQ_F32;                   // weights as two terms
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];
+    __shared__ int odd_values[PT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, hh = lane >> 5;
     const uint32_t group = (uint32_t)(a.H / a.Hkv);
     const uint32_t n = blockIdx.x / (uint32_t)a.H, hx = blockIdx.x - n * (uint32_t)a.H;
@@ -146,10 +159,11 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     // serves few of them
     const int hk = hx % (uint32_t)a.Hkv, h = hk * group + hx / (uint32_t)a.Hkv;
     int64_t seq, blk;
-    if (!find_block(a, n, seq, blk)) return;
+    if (!find_block<QB>(a, n, seq, blk)) return;
     const Packed pk = packed_sequence(a.qs, a.ks, seq, a.total_q, a.total_k);
     const bool causal = a.causal != 0;
-    const int64_t qb = blk * PT_Q, qw = qb + 32 * wave;  // first query of the workgroup, of the wave
+    const int kg = wave % SPLIT, k32 = 64 / SPLIT * kg;  // this wave's keys of a tile begin at k32
+    const int64_t qb = blk * QB, qw = qb + 32 * (wave / SPLIT);  // first query of the workgroup, of the wave
     const int hd = (int)a.hd;
 
     // B operand of S^T = K Q^T: query qw + col, dims 16 s + 8 hh ..
@@ -167,7 +181,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     const int lim = (int)keys_seen(pk, qw + col, causal);
     const int seen_first = (int)keys_seen(pk, qw, causal);
     const int seen_wave = qw < pk.nq ? (int)keys_seen(pk, qw + 31, causal) : 0;
-    const int seen_all = (int)keys_seen(pk, min(qb + PT_Q, pk.nq) - 1, causal);
+    const int seen_all = (int)keys_seen(pk, min(qb + QB, pk.nq) - 1, causal);
     const int tiles = (seen_all + PT_K - 1) / PT_K;
 
     // copies: lane of copy j of its wave fills LDS slot (j * waves + wave) * 64 + lane; slot x of row
@@ -207,9 +221,9 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     uint32_t careful = 0;
     const float sl2 = a.scale * LOG2E;
     // reads of K: row col of a 32-key block, chunk 2 s + hh; of V: rows 4 hh + (i >> 2) (+ 8), see lds_read_tr
-    const uint32_t krow = lds0 + col * HDP * 2;
+    const uint32_t krow = lds0 + (k32 + col) * HDP * 2;
     const int vi = lane & 15, vr = 4 * hh + (vi >> 2), vc = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
-    const uint32_t vrow = lds0 + TILE + vr * HDP * 2 + 8 * (vi & 1);
+    const uint32_t vrow = lds0 + TILE + (k32 + vr) * HDP * 2 + 8 * (vi & 1);
 
     // one tile: MASKED where some query of the wave does not see some of its keys
     auto step = [&](int t, auto masked) __attribute__((always_inline)) {
@@ -232,7 +246,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)),
                                       qf[s], sc[b]);
         if constexpr (MASKED) {
-            const int left = lim - kb - 4 * hh;
+            const int left = lim - kb - k32 - 4 * hh;
 #pragma unroll
             for (int b = 0; b < KT; ++b)
 #pragma unroll
@@ -302,12 +316,44 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     if (tiles > 0) issue(0);
     for (int t = 0; t < open; ++t) step(t, std::false_type{});
     for (int t = open; t < tiles; ++t) step(t, std::true_type{});
-    if (__any(careful != 0)) {  // the wave's queries again, one by one
+    bool again = __any(careful != 0);
+    l = half_sum(l);
+    if constexpr (SPLIT > 1) {  // the waves of a query meet in the first of them
+        constexpr int WORDS = (16 * DT + 2) * 64;
+        static_assert(PT_WAVES / SPLIT * (SPLIT - 1) * WORDS * 4 <= 4 * TILE, "the sums fit the tiles' LDS");
+        float* sums = reinterpret_cast<float*>(lds) + wave / SPLIT * (SPLIT - 1) * WORDS + lane;
+        block_barrier();  // every wave is done with the tiles
+        if (kg > 0) {
+            float* mine = sums + (kg - 1) * WORDS;
+            mine[0] = m;
+            mine[64] = l;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[64 * (2 + 16 * d + i)] = o[d][i];
+        }
+        if (lane == 0) odd_values[wave] = again;
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int w = 1; w < SPLIT; ++w) {
+            const float* other = sums + (w - 1) * WORDS;
+            again |= odd_values[wave + w] != 0;
+            const float mn = fmaxf(m, other[0]), base = mn == -INFINITY ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(other[0] - base);
+            m = mn;
+            l = __builtin_fmaf(l, f, g * other[64]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = __builtin_fmaf(o[d][i], f, g * other[64 * (2 + 16 * d + i)]);
+        }
+    }
+    if (again) {  // the wave's queries once more, one by one
         for (int64_t i = qw; i < min(qw + 32, pk.nq); ++i)
             attend_row<E, Out>(a, pk.q0 + i, h, hk, pk.k0, keys_seen(pk, i, causal));
         return;
     }
-    l = half_sum(l);
     const float r = seen_all > 0 && lim > 0 ? 1.0f / l : 0.0f;
     const int64_t qi = qw + col;
     if (qi < pk.nq) {
@@ -358,13 +404,21 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
     // 16-byte copies and loads: bases and rows aligned to them, offsets of a tile's rows within 31 bits
     const bool vec = aligned16(d_q) && aligned16(d_k) && aligned16(d_v) && aligned16(d_out) && ldq % 8 == 0 &&
                      ldk % 8 == 0 && ldv % 8 == 0 && ldk < (1 << 23) && ldv < (1 << 23);
-    const int64_t blocks = (total_q + (PT_Q - 1) * (seqs < total_q ? seqs : total_q)) / PT_Q;
-    if (vec && blocks * H <= 0x7fffffff) {
-        const dim3 tiles((unsigned)(blocks * H)), wg(64 * PT_WAVES);
+    auto blocks = [&](int64_t qb) { return (total_q + (qb - 1) * (seqs < total_q ? seqs : total_q)) / qb * H; };
+    if (vec && blocks(64) <= 0x7fffffff) {
+        // Enough workgroups to fill the chip twice over: 128 queries each.  Fewer: 64 queries each with the keys
+        // split over two waves, which shortens the longest chain of tiles (one sequence of 3845 with 8 heads of
+        // 128: 87 us with 128 queries, 66 with 64; 34 of up to 3483 with 2 heads: 81 and 64; at twice as
+        // many workgroups no difference).
+        const bool many = blocks(128) >= 2 * 512;
+        const dim3 tiles((unsigned)blocks(many ? 128 : 64)), wg(64 * PT_WAVES);
         with_half(type, [&](auto e) {
             using E = decltype(e);
             auto go = [&](auto w, auto o) {
-                hipLaunchKernelGGL((prompt_tile_kernel<decltype(w)::value, E, decltype(o)>), tiles, wg, 0, st, a);
+                constexpr int W = decltype(w)::value;
+                using O = decltype(o);
+                if (many) hipLaunchKernelGGL((prompt_tile_kernel<W, 1, E, O>), tiles, wg, 0, st, a);
+                else hipLaunchKernelGGL((prompt_tile_kernel<W, 2, E, O>), tiles, wg, 0, st, a);
             };
             auto width = [&](auto o) {
                 if (hd <= 64) go(std::integral_constant<int, 64>{}, o);

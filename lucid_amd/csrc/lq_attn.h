@@ -147,6 +147,19 @@ __device__ __forceinline__ u2v widen4(ElemBF16, uint32_t w) {
     return u2v{__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
 }
 
+// Sum of an integer over the wave, the same in every lane, by register permutes (the pairings of
+// ln_wave_sum).
+__device__ __forceinline__ int wave_add(int v) {
+    v += __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, true);   // quad_perm [1,0,3,2]
+    v += __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, true);   // quad_perm [2,3,0,1]
+    v += __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, true);  // row_half_mirror
+    v += __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, true);  // row_mirror
+    const auto p16 = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = (int)(p16[0] + p16[1]);
+    const auto p32 = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    return (int)(p32[0] + p32[1]);
+}
+
 // LDS reads at a byte offset of the workgroup's LDS (written by copies the compiler does not see).
 typedef __attribute__((address_space(3))) u4v lds_u4v;
 typedef __attribute__((address_space(3))) s4v lds_s4v;

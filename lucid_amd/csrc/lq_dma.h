@@ -62,6 +62,16 @@ __device__ __forceinline__ void lds_dma16(v4i rsrc, uint32_t voff, uint32_t soff
                  : "memory");
 }
 
+// The same where the descriptor is made right before (v_readfirstlane): a load must not read a scalar
+// register within five wait states of a vector instruction's write to it, and the compiler, which
+// keeps that distance for loads of its own, does not see the load in the asm.
+__device__ __forceinline__ void lds_dma16_fresh(v4i rsrc, uint32_t voff, uint32_t lds_addr) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(voff), "s"(rsrc), "{m0}"(lds_addr)
+                 : "memory");
+}
+
 // 16 bytes per lane from the lane's own address into LDS at lds_addr + 16 * lane (lanes switched off copy
 // nothing), past the caches: for what is read once.  No bounds check: every active lane's address must
 // be valid.

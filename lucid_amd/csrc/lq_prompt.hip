@@ -95,12 +95,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64
     };
     if (a.seqs <= 64) {
         const int cnt = blocks(lane);
-        auto from = [&](int level) {  // blocks at or past a level
-            int v = max(cnt - level, 0);
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-            return v;
-        };
+        auto from = [&](int level) { return wave_add(max(cnt - level, 0)); };  // blocks at or past a level
         if (n >= from(0)) return false;
         int lo = 0, hi = wave_max(cnt);  // from(lo) > n >= from(hi)
         while (hi - lo > 1) {
@@ -139,11 +134,15 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64
 //   number a lane;
 //   O^T += V^T P^T: those weights are the B operand as they are (no exchange between lanes), and V^T is
 //   what the transposing read of the V rows gives.  A rescale is one factor a lane.
-// What bounds it: the matrix cores are busy half of the time at the 1.9 GHz that the card keeps under
-// this load, the vector unit's work on the weights (exponential, sum, rounding) the other half; the
-// two waves of a SIMD overlap them only in part.
+// The scores of the next tile are on the matrix cores while the vector unit makes this tile's weights (one
+// wave's exponentials beside its own products: 12288 tokens, 32 heads of 128 in bfloat16, 1192 -> 1135
+// us; an order of the two forced by scheduling hints 1155).
+// What bounds it: at that size 1090 TFLOP/s, where a library product of 16384^3 reaches 1326 on this
+// card; the card keeps 1.9 GHz under this load, at which the matrix cores are busy more than half of
+// the time, and the vector unit's work on the weights (exponential, sum, rounding) is only in
+// part beside them.  Short sequences add some 4 us of dependent loads to every workgroup.
 template <int HDP, int SPLIT, class E, class Out>
-__global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) void prompt_tile_kernel(PromptArgs a) {
     constexpr int QB = 32 * PT_WAVES / SPLIT;
     constexpr int CPR = HDP / 8;                                // 16-byte chunks of a row
     constexpr int TILE = PT_K * HDP * 2;                        // bytes of a K (or V) tile
@@ -152,7 +151,8 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     constexpr bool TWO = Out::code == LQ_F32;                   // weights as two terms
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];
     __shared__ int odd_values[PT_WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, hh = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hh = lane >> 5;
     const uint32_t group = (uint32_t)(a.H / a.Hkv);
     const uint32_t n = blockIdx.x / (uint32_t)a.H, hx = blockIdx.x - n * (uint32_t)a.H;
     // consecutive workgroups (on consecutive XCDs) take different key heads: an XCD's L2 then
@@ -160,6 +160,8 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     const int hk = hx % (uint32_t)a.Hkv, h = hk * group + hx / (uint32_t)a.Hkv;
     int64_t seq, blk;
     if (!find_block<QB>(a, n, seq, blk)) return;
+    seq = __builtin_amdgcn_readfirstlane((int)seq);  // what follows from it lies in scalar registers
+    blk = __builtin_amdgcn_readfirstlane((int)blk);
     const Packed pk = packed_sequence(a.qs, a.ks, seq, a.total_q, a.total_k);
     const bool causal = a.causal != 0;
     const int kg = wave % SPLIT, k32 = 64 / SPLIT * kg;  // this wave's keys of a tile begin at k32
@@ -201,16 +203,17 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     }
     const char* kbase = static_cast<const char*>(a.k) + (pk.k0 * a.ldk + (int64_t)hk * hd) * 2;
     const char* vbase = static_cast<const char*>(a.v) + (pk.k0 * a.ldv + (int64_t)hk * hd) * 2;
-    auto issue = [&](int t) __attribute__((always_inline)) {
+    auto issue = [&](int t, const char* src, uint32_t ld, const uint32_t (&off)[COPIES], uint32_t at)
+                     __attribute__((always_inline)) {
+        if (t >= tiles) return;
         const int rows = (int)min((int64_t)PT_K, pk.nk - (int64_t)t * PT_K);  // at least 1
-        const v4i rk = buffer_rsrc(kbase + (int64_t)t * PT_K * ldk, (uint32_t)((rows - 1) * ldk + 2 * hd));
-        const v4i rv = buffer_rsrc(vbase + (int64_t)t * PT_K * ldv, (uint32_t)((rows - 1) * ldv + 2 * hd));
-        const uint32_t to = lds0 + (t & 1) * 2 * TILE + wave * 1024;
+        const v4i r = buffer_rsrc(src + (int64_t)t * PT_K * ld, (uint32_t)((rows - 1) * ld + 2 * hd));
+        const uint32_t to = lds0 + (t & 1) * 2 * TILE + at + wave * 1024;
 #pragma unroll
-        for (int j = 0; j < COPIES; ++j) lds_dma16(rk, koff[j], 0u, to + j * PT_WAVES * 1024);
-#pragma unroll
-        for (int j = 0; j < COPIES; ++j) lds_dma16(rv, voff[j], 0u, to + TILE + j * PT_WAVES * 1024);
+        for (int j = 0; j < COPIES; ++j) lds_dma16_fresh(r, off[j], to + j * PT_WAVES * 1024);
     };
+    auto issue_k = [&](int t) __attribute__((always_inline)) { issue(t, kbase, ldk, koff, 0); };
+    auto issue_v = [&](int t) __attribute__((always_inline)) { issue(t, vbase, ldv, voff, TILE); };
 
     f16v o[DT];
 #pragma unroll
@@ -225,16 +228,10 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
     const int vi = lane & 15, vr = 4 * hh + (vi >> 2), vc = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
     const uint32_t vrow = lds0 + TILE + (k32 + vr) * HDP * 2 + 8 * (vi & 1);
 
-    // one tile: MASKED where some query of the wave does not see some of its keys
-    auto step = [&](int t, auto masked) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked)::value;
-        wait_vmcnt<0>();
-        block_barrier();  // tile t has landed, and every wave is done with the buffer of tile t + 1
-        if (t + 1 < tiles) issue(t + 1);
-        const int kb = t * PT_K;
-        if (MASKED && kb >= seen_wave) return;
-        const uint32_t buf = (t & 1) * 2 * TILE;
-        f16v sc[KT];
+    const int open = qw < pk.nq ? min(seen_first / PT_K, tiles) : 0;  // tiles whose keys every query of the wave sees
+    const int mine = (seen_wave + PT_K - 1) / PT_K;                   // tiles with a key that some query of it sees
+    auto scores = [&](int t, f16v (&sc)[KT]) __attribute__((always_inline)) {
+        const uint32_t at = krow + (t & 1) * 2 * TILE;
 #pragma unroll
         for (int b = 0; b < KT; ++b)
 #pragma unroll
@@ -243,23 +240,25 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int b = 0; b < KT; ++b)
-                sc[b] = mfma_32x32x16(E{}, lds_read16(krow + buf + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)),
-                                      qf[s], sc[b]);
-        if constexpr (MASKED) {
-            const int left = lim - kb - k32 - 4 * hh;
+                sc[b] = mfma_32x32x16(E{}, lds_read16(at + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)), qf[s], sc[b]);
+    };
+    auto mask = [&](int t, f16v (&sc)[KT]) __attribute__((always_inline)) {
+        const int left = lim - t * PT_K - k32 - 4 * hh;
 #pragma unroll
-            for (int b = 0; b < KT; ++b)
+        for (int b = 0; b < KT; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (32 * b + 8 * (i >> 2) + (i & 3) >= left) sc[b][i] = -INFINITY;
-        }
+            for (int i = 0; i < 16; ++i)
+                if (32 * b + 8 * (i >> 2) + (i & 3) >= left) sc[b][i] = -INFINITY;
+    };
+    // the running maximum over a tile's scores; the accumulators follow it only when it has risen by
+    // more than 2^RESCALE_AT
+    auto maximum = [&](const f16v (&sc)[KT]) __attribute__((always_inline)) {
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < KT; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
         mx = half_max(mx) * sl2;
-        // the accumulators follow the maximum only when it has risen by more than 2^RESCALE_AT
         if (__any(mx > m + RESCALE_AT)) {
             const float mn = fmaxf(m, mx);
             const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
@@ -270,15 +269,30 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
+    };
+    // Tile t, whose scores are `sc`: the scores of tile t + 1 go to the matrix cores while the vector unit makes
+    // this tile's weights, then the weights meet V.  MASKED where some query of the wave does not see
+    // some key of tile t or t + 1.
+    auto step = [&](int t, f16v (&sc)[KT], f16v (&next)[KT], auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
+        wait_vmcnt<0>();
+        block_barrier();  // K of t + 1 and V of t have landed; every wave is done with K of t and V of t - 1
+        issue_k(t + 2);
+        issue_v(t + 1);
+        if (MASKED && t >= mine) return;
+        const bool more = !MASKED || t + 1 < mine;
+        if (more) scores(t + 1, next);
         const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<E>;
         u4v p[2 * KT], pl[TWO ? 2 * KT : 1];
+        float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < KT; ++b)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
                 const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], sl2, -base));
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i + 1], sl2, -base));
-                l += x + y;
+                l += x;
+                sum += y;
                 const uint32_t w = pack2(E{}, x, y);
                 p[2 * b + (i >> 3)][(i & 7) >> 1] = w;
                 if constexpr (TWO) {
@@ -286,8 +300,10 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                     pl[2 * b + (i >> 3)][(i & 7) >> 1] = pack2(E{}, x - r[0], y - r[1]);
                 }
             }
+        l += sum;
+        const uint32_t vt = vrow + (t & 1) * 2 * TILE;
         auto value = [&](int d, int ks) __attribute__((always_inline)) {
-            const uint32_t at = vrow + buf + ks * 16 * HDP * 2 + (((4 * d + vc) ^ v_swz(vr)) << 4);
+            const uint32_t at = vt + ks * 16 * HDP * 2 + (((4 * d + vc) ^ v_swz(vr)) << 4);
             const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * HDP * 2);
             return u4v{lo[0], lo[1], hi[0], hi[1]};
         };
@@ -301,7 +317,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                     odd |= not_finite<E>(v[0]) | not_finite<E>(v[1]) | not_finite<E>(v[2]) | not_finite<E>(v[3]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            careful |= odd & 0x80008000u;
+            if (t >= open) careful |= odd & 0x80008000u;
         }
 #pragma unroll
         for (int ks = 0; ks < 2 * KT; ++ks)
@@ -311,11 +327,34 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 128 ? 2 : 1) void prompt_tile
                 o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
                 if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
             }
+        if (more) {
+            if (MASKED && t + 1 >= open) mask(t + 1, next);
+            maximum(next);
+        }
     };
-    const int open = qw < pk.nq ? min(seen_first / PT_K, tiles) : 0;  // tiles whose keys every query of the wave sees
-    if (tiles > 0) issue(0);
-    for (int t = 0; t < open; ++t) step(t, std::false_type{});
-    for (int t = open; t < tiles; ++t) step(t, std::true_type{});
+    f16v sa[KT], sb[KT];
+    if (tiles > 0) {
+        issue_k(0);
+        wait_vmcnt<0>();
+        block_barrier();
+        issue_k(1);
+        issue_v(0);
+        if (mine > 0) {
+            scores(0, sa);
+            if (open == 0) mask(0, sa);
+            maximum(sa);
+        }
+    }
+    int t = 0;
+    for (; t + 2 < open; t += 2) {
+        step(t, sa, sb, std::false_type{});
+        step(t + 1, sb, sa, std::false_type{});
+    }
+    for (; t < tiles; ++t) {
+        step(t, sa, sb, std::true_type{});
+#pragma unroll
+        for (int b = 0; b < KT; ++b) sa[b] = sb[b];
+    }
     bool again = __any(careful != 0);
     l = half_sum(l);
     if constexpr (SPLIT > 1) {  // the waves of a query meet in the first of them

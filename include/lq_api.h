@@ -804,7 +804,7 @@ int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_
  * d_starts[s] .. d_starts[s + 1] - 1 and they become its last positions; d_starts NULL: token s is
  * the one new token of sequence s (tokens == seqs).  A float cache gets each value rounded once
  * to nearest even.  An int8 cache gets scale = max|x| / 127 and code = rne(x * (127 / max|x|)) per
- * row of hd; a row with an infinity or NaN gets a scale that is not finite and reads back as
+ * row of hd; a row with an infinity or NaN gets a scale that is not finite and is attended as
  * NaN, one whose magnitudes are below 127 / FLT_MAX as zeros.  A token is left out when its
  * position is negative (a sequence of length 0), lies past the table, or its page number is
  * outside [0, pages).  Two tokens of one call must not share a place. */

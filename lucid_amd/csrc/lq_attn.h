@@ -91,12 +91,6 @@ template <class E>
 constexpr float WEIGHT_SHIFT = E::code == LQ_F16 ? 6.0f : 0.0f;
 constexpr float RESCALE_AT = 8.0f;
 
-// Bits 15 and 31 are set where a 16-bit value of the word is an infinity or NaN.
-template <class E>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    return E::code == LQ_F16 ? (w & 0x7c007c00u) + 0x04000400u : (w & 0x7f807f80u) + 0x00800080u;
-}
-
 // The larger / the sum of the values that lanes l and l ^ 32 hold.
 __device__ __forceinline__ float half_max(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);

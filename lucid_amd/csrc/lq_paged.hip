@@ -448,6 +448,25 @@ struct Sums {
     }
 };
 
+// Dim d of row r's sum over a piece, key by key: for values that hold an infinity, which the second term
+// of a weight turned into NaN.  M: the piece's maximum.
+template <class Q>
+__device__ __forceinline__ float paged_sum_again(const PagedArgs& a, const Piece& w, int r, int d, float M) {
+    const typename Q::T* q = static_cast<const typename Q::T*>(a.q) + w.b * a.ldq + (int64_t)(w.h0 + r) * a.hd;
+    float x = 0.0f;
+    for (int key = w.begin; key < w.end; ++key) {
+        const int64_t row0 = position_row(key, a.table + (int64_t)w.b * a.table_stride, a.table_stride, a.pages, a.Hkv, a.page);
+        if (row0 < 0) return __builtin_nanf("");
+        const int64_t row = row0 + (int64_t)w.hk * a.page;
+        const typename Q::T* k = static_cast<const typename Q::T*>(a.k) + row * a.hd;
+        float s = 0.0f;
+        for (int i = 0; i < a.hd; ++i) s = __builtin_fmaf(Q::load(q[i]), Q::load(k[i]), s);
+        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale * LOG2E, -(M == -INFINITY ? 0.0f : M - WEIGHT_SHIFT<Q>)));
+        x = __builtin_fmaf(f, Q::load(static_cast<const typename Q::T*>(a.v)[row * a.hd + d]), x);
+    }
+    return x;
+}
+
 // The waves' sums meet: wave w's lie at LDS lds + w * SLOT (16 queries of OROW floats each), and the
 // workgroup writes the output or its part of it.
 template <int WAVES, int SLOT, int DT, class Q, class P>
@@ -479,6 +498,8 @@ __device__ __forceinline__ void paged_finish(const PagedArgs& a, const Piece& w,
             L = __builtin_fmaf(f, ml[v][1][r], L);
             x = __builtin_fmaf(f, reinterpret_cast<const float*>(lds + v * SLOT)[r * OROW + d], x);
         }
+        if constexpr (std::is_same_v<Q, P>)  // the int8 cache's values are finite codes
+            if (!(fabsf(x) < INFINITY) && L == L) x = paged_sum_again<Q>(a, w, r, d, M);
         if (w.whole) {
             const int64_t at = ((int64_t)w.b * a.H + w.h0 + r) * hd + d;
             if (a.out_f32) static_cast<float*>(a.out)[at] = x / L;
@@ -904,6 +925,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
     const hipStream_t st = as_stream(stream);
     // a few short sequences: four waves each, to hide more of the latency; else two, two workgroups to a CU
     const bool few = alone && units <= 256;
+    note_path(!alone ? "paged shared" : few ? "paged whole 4 waves" : "paged whole");
     with_half(q_type, [&](auto q) {
         using Q = decltype(q);
         auto i8 = [&](auto w, auto exact) {

@@ -26,7 +26,7 @@ struct PromptArgs {
 // Query t of head h (key head hk) over keys k0 .. k0 + len - 1, by one wave: 64 keys at a time, a lane
 // scores one key, then adds its dims (lane, lane + 64, ...) of the weighted values.  Reads nothing
 // but the keys seen, element by element: for operands that no vector fits, and for queries whose
-// tiles hold infinities or NaN beyond what they see.
+// tiles hold infinities or NaN.
 template <class E, class Out>
 __device__ __forceinline__ void attend_row(const PromptArgs& a, int64_t t, int h, int hk, int64_t k0, int64_t len) {
     constexpr int PARTS = ATTN_MAX_HD / 64;
@@ -221,7 +221,6 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    uint32_t careful = 0;
     const float sl2 = a.scale * LOG2E;
     // reads of K: row col of a 32-key block, chunk 2 s + hh; of V: rows 4 hh + (i >> 2) (+ 8), see lds_read_tr
     const uint32_t krow = lds0 + (k32 + col) * HDP * 2;
@@ -307,18 +306,6 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
             const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * HDP * 2);
             return u4v{lo[0], lo[1], hi[0], hi[1]};
         };
-        if constexpr (MASKED) {  // a key not seen has the weight 0, which no infinity or NaN may meet
-            uint32_t odd = 0;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int ks = 0; ks < 2 * KT; ++ks) {
-                    const u4v v = value(d, ks);
-                    odd |= not_finite<E>(v[0]) | not_finite<E>(v[1]) | not_finite<E>(v[2]) | not_finite<E>(v[3]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            if (t >= open) careful |= odd & 0x80008000u;
-        }
 #pragma unroll
         for (int ks = 0; ks < 2 * KT; ++ks)
 #pragma unroll
@@ -355,7 +342,14 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
 #pragma unroll
         for (int b = 0; b < KT; ++b) sa[b] = sb[b];
     }
-    bool again = __any(careful != 0);
+    // An infinity or NaN among the values has met weights it must not meet: the 0 of a key that is not seen, the
+    // second term of a weight.  It left a sum that is not finite; such queries are computed again.
+    bool odd = false;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) odd |= !(fabsf(o[d][i]) < INFINITY);
+    bool again = __any(odd);
     l = half_sum(l);
     if constexpr (SPLIT > 1) {  // the waves of a query meet in the first of them
         constexpr int WORDS = (16 * DT + 2) * 64;
@@ -468,7 +462,7 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
             if (out_type == LQ_F32) width(ElemF32{});
             else width(E{});
         });
-        note_path("prompt tile");
+        note_path(many ? "prompt tile 128" : "prompt tile 64");
         return launch_status("lq_prompt_attention");
     }
     note_path("prompt rows");

@@ -335,6 +335,76 @@ def test_paged_attention_keeps_infinite_scores_like_the_formula(gpu):
     assert np.isnan(got[0, 1]).all()
 
 
+@pytest.mark.parametrize("cache,hd", [("float16", 64), ("float16", 128), ("int8", 128), ("float16", 40), ("int8", 64),
+                                      ("float16", 192)])
+@pytest.mark.parametrize("seqs,longest,h,hkv", [(150, 1400, 2, 1), (40, 3000, 4, 4), (3, 1100, 20, 1), (200, 1025, 1, 1)])
+def test_paged_attention_shared_positions(gpu, cache, hd, seqs, longest, h, hkv):
+    """Lengths of every kind on one line of work: more sequences than a workgroup has threads, parts
+    that begin and end inside sequences, empty ones between, two tiles of query heads."""
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(seqs + hd)
+    lens = [int(n) for n in np.exp(rng.uniform(0, np.log(longest), seqs))]
+    lens[seqs // 2], lens[-1], lens[0] = longest, 0, 0
+    lens[1:seqs // 3:7] = [0] * len(lens[1:seqs // 3:7])
+    _paged(rng, lens, h, hkv, hd, 16, "float16", cache, "float32")
+    assert _C.last_path() == "paged shared"
+
+
+def test_paged_attention_paths(gpu):
+    from lucid_amd import _C
+
+    for hd in (64, 128):
+        _paged(np.random.default_rng(1), [40, 1000], 2, 1, hd, 16, "float16", "float16", "float16")
+        assert _C.last_path() == "paged whole 4 waves"
+        _paged(np.random.default_rng(2), [int(n) for n in np.random.default_rng(2).integers(0, 90, 140)], 4, 2, hd, 16,
+               "bfloat16", "bfloat16", "bfloat16")
+        assert _C.last_path() == "paged whole"
+
+
+def test_paged_cache_past_32_bits(gpu):
+    """A pool of more than 2^32 bytes and 2^31 values: the last pages hold what was appended and are
+    attended."""
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+
+    hkv, page, hd = 8, 64, 64
+    pages = (1 << 31) // (hkv * page * hd) + 40
+    k, v = (L.empty((pages, hkv, page, hd), L.float16, "gpu") for _ in range(2))
+    assert k.nbytes > 1 << 32
+    rng = np.random.default_rng(0)
+    table = np.array([[pages - 1, 3, pages - 2]], np.int32)
+    x = rng.standard_normal((150, 2, hkv, hd)).astype(np.float16)
+    F.paged_kv_append(_dev(x[:, 0]), _dev(x[:, 1]), k, v, _i32(table), _i32([150]), _i32([0, 150]))
+    q = rng.standard_normal((1, hkv, hd)).astype(np.float16)
+    for bound in (150, 2000):
+        got = F.paged_attention(_dev(q), k, v, _i32(table), _i32([150]), bound, out_dtype=L.float32).numpy()
+        for j in range(hkv):
+            want, b = _attend(q[0, j].astype(np.float64), x[:, 0, j].astype(np.float64), x[:, 1, j].astype(np.float64),
+                              hd ** -0.5, 2.0 ** -16, U)
+            _check(got[0, j], want, b, f"head {j}")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 72])
+@pytest.mark.parametrize("n", [70, 1500])
+def test_paged_attention_of_infinite_values(gpu, hd, n):
+    """An infinity among the values gives an infinity in its dim (NaN where both signs meet) and
+    nothing elsewhere."""
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(n + hd)
+    pages = -(-n // 16)
+    k, v = (rng.standard_normal((pages, 1, 16, hd)).astype(np.float16) for _ in range(2))
+    v[1, 0, 3, 5], v[2, 0, 1, 6], v[3, 0, 0, 6], v[0, 0, 2, 9] = np.inf, np.inf, -np.inf, -np.inf
+    q = rng.standard_normal((1, 3, hd)).astype(np.float16)
+    table = np.arange(pages, dtype=np.int32)[None]
+    for dt in (L.float32, L.float16):
+        got = _values(F.paged_attention(_dev(q), _dev(k), _dev(v), _i32(table), _i32([n]), n, out_dtype=dt))[0]
+        assert (got[:, 5] == np.inf).all() and np.isnan(got[:, 6]).all() and (got[:, 9] == -np.inf).all()
+        assert np.isfinite(np.delete(got, [5, 6, 9], 1)).all()
+
+
 # ------------------------------------------------------------------------------ prompts
 
 
@@ -433,6 +503,70 @@ def test_prompt_attention_keys_not_seen_never_reach_a_query(gpu, hd, dtype):
         assert np.isfinite(got[:first]).all(), first
         assert np.abs(got[:first] - clean[:first]).max() <= 8 * weps * np.abs(v).max()
         assert not np.isfinite(got[first]).all()
+
+
+@pytest.mark.parametrize("dtype,out", [("float16", "float32"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("hd", [64, 128, 40, 192, 256])
+def test_prompt_attention_many_workgroups(gpu, dtype, out, hd):
+    """The kernel of 128 queries a workgroup, over 64 sequences at most and over more."""
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(hd)
+    lens = [300, 1, 0, 129, 128, 127, 64, 65, 200] + [int(n) for n in rng.integers(0, 40, 27)]
+    _prompt(rng, lens, lens, 32, 4, hd, dtype, out, fused=True)
+    assert _C.last_path() == "prompt tile 128"
+    more = [int(n) for n in rng.integers(0, 20, 90)] + [260]
+    _prompt(rng, more, [n + 30 for n in more], 16, 8, hd, dtype, out)
+    assert _C.last_path() == "prompt tile 128"
+    _prompt(rng, lens[:9], lens[:9], 2, 1, hd, dtype, out)
+    assert _C.last_path() == "prompt tile 64"
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_attention_keys_not_seen_many_workgroups(gpu, hd):
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(hd)
+    lens, h = [150] + [3] * 60, 32
+    total = sum(lens)
+    st = _i32(np.concatenate([[0], np.cumsum(lens)]))
+    q, k, v = (rng.standard_normal((total, n, hd)).astype(np.float16) for n in (h, 2, 2))
+    clean = F.prompt_attention(_dev(q), _dev(k), _dev(v), st, out_dtype=L.float32).numpy()
+    assert _C.last_path() == "prompt tile 128"
+    for first in (5, 70, 149):
+        vb = v.copy()
+        vb[first, 0, 1], vb[first, 1, 2] = np.inf, np.nan
+        got = F.prompt_attention(_dev(q), _dev(k), _dev(vb), st, out_dtype=L.float32).numpy()
+        ok = np.r_[0:first, 150:total]
+        assert np.abs(got[ok] - clean[ok]).max() <= 8 * 2.0 ** -15 * np.abs(v).max()
+        assert np.isinf(got[first:150, :h // 2, 1]).all() and np.isnan(got[first:150, h // 2:, 2]).all()
+        # the dims beside them are untouched
+        assert np.isfinite(np.delete(got, [1, 2], 2)).all()
+
+
+def test_prompt_attention_of_rows_no_vector_fits(gpu):
+    """Rows an odd number of elements apart, and a base that is not 16-byte aligned."""
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(2)
+    n, h, hd = 70, 2, 40
+    for ld, shift in ((h * hd + 3, 0), (h * hd + 8, 1)):
+        buf = rng.standard_normal((3, n * ld + 8)).astype(np.float16)
+        d = [_dev(b) for b in buf]
+        x = [b[shift:shift + n * ld].reshape(n, ld)[:, :h * hd].reshape(n, h, hd).astype(np.float64) for b in buf]
+        out, st = _dev(np.zeros((n, h, hd), np.float32)), _i32([0, 30, 70])
+        _C.call("lq_prompt_attention", d[0].data_ptr() + 2 * shift, ld, d[1].data_ptr() + 2 * shift, ld,
+                d[2].data_ptr() + 2 * shift, ld, _C.F16, st.data_ptr(), st.data_ptr(), 2, n, n, h, h, hd, 1, hd ** -0.5,
+                out.data_ptr(), _C.F32, None)
+        assert _C.last_path() == "prompt rows"
+        got = out.numpy()
+        for t in range(n):
+            a = 0 if t < 30 else 30
+            for j in range(h):
+                want, bound = _attend(x[0][t, j], x[1][a:t + 1, j], x[2][a:t + 1, j], hd ** -0.5, 2.0 ** -16, U)
+                _check(got[t, j], want, bound, f"row {t}")
 
 
 def test_prompt_attention_rows_of_no_sequence_are_left(gpu):
@@ -554,6 +688,28 @@ def test_token_logprobs_ties_and_rows_that_are_not_ordinary(gpu, dtype, vocab):
     assert np.isnan(lse[5]) and np.isnan(lp[5]) and np.isnan(ent[5])
     assert np.isnan(lp[6])
     assert np.isfinite(lse[8]) and abs(ent[8] - np.log(vocab)) <= tol * 15
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("top", [2, 64])
+def test_token_logprobs_best_in_few_threads(gpu, dtype, top):
+    """All large values within the chunks of eight neighbouring threads: more than are collected at
+    once, with and without ties."""
+    import lucid_amd.nn.functional as F
+
+    n = 4 if dtype == "float32" else 8
+    vocab = 200000
+    rng = np.random.default_rng(top)
+    chunk = np.arange(vocab) // n % 512
+    x = rng.standard_normal((2, vocab)).astype(np.float32)
+    large = chunk < 8
+    x[0, large] = 50 + rng.permutation(large.sum()) / 8
+    x[1, large] = 50
+    v, xh = _round(x, dtype)
+    lp, ent, lse, tlp, tid = (a.numpy() for a in F.token_logprobs(_dev(xh), _i32([0, 1]), top))
+    np.testing.assert_array_equal(tid, _order(v, top))
+    want = _logprob_want(v, np.array([0, 1]), top)
+    _check(lse, want[2], want[5] + 2 * U * np.abs(want[2]), "lse")
 
 
 def test_token_logprobs_strided_rows_and_optional_outputs(gpu):
@@ -744,6 +900,37 @@ def test_cache_classes_and_graph_replay(gpu):
     check(q, cache.attend(_dev(q), out_dtype=L.float32).numpy())
     del graph
     _C.call("lq_stream_destroy", stream)
+
+
+def test_ops_replayed_from_a_graph(gpu):
+    """Prompt attention, log probabilities and their gradient recorded once and replayed with new
+    inputs, eager work of the same ops and synchronizations between the replays."""
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+    from lucid_amd.graphs import CapturedForward
+
+    rng = np.random.default_rng(31)
+    st, t = _i32([0, 50, 130]), _i32([3, -100, 7, 500])
+    g = _dev(rng.standard_normal(4).astype(np.float32))
+
+    def fn(qkv, x):
+        lp, ent, lse, top, ids = F.token_logprobs(x, t, 6)
+        return (F.prompt_attention_qkv(qkv, 4, 2, st, out_dtype=L.float32), lp, ent, lse, top, ids,
+                F.token_logprobs_backward(x, t, lse, g, ent, g))
+
+    make = lambda: (rng.standard_normal((130, 8, 64)).astype(np.float16),  # noqa: E731
+                    (rng.standard_normal((4, 3001)) * 3).astype(np.float32))
+    a, b = make()
+    qkv, x = _dev(a), _dev(b)
+    cap = CapturedForward(fn, qkv, x)
+    for _ in range(4):
+        a, b = make()
+        cap.load(a, b)
+        got = [y.numpy() for y in cap()]
+        want = [y.numpy() for y in fn(_dev(a), _dev(b))]
+        L.synchronize()
+        for y, z in zip(got, want):
+            np.testing.assert_array_equal(y, z)
 
 
 def test_ops_on_a_stream_of_their_own(gpu):

@@ -119,10 +119,13 @@ __device__ __forceinline__ float quarter_sum(float v) {
 template <int I>
 __device__ __forceinline__ float byte_to_f32(uint32_t w) {
     float f;
-    if constexpr (I == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
-    if constexpr (I == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
-    if constexpr (I == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
-    if constexpr (I == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+#define LQ_BYTE(i)                                                                                        \
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_" #i : "=v"(f) : "v"(w))
+    if constexpr (I == 0) LQ_BYTE(0);
+    if constexpr (I == 1) LQ_BYTE(1);
+    if constexpr (I == 2) LQ_BYTE(2);
+    if constexpr (I == 3) LQ_BYTE(3);
+#undef LQ_BYTE
     return f;
 }
 // Four int8 codes of a word as two words of 16-bit values, exact in both types.  fp16: the code + 128

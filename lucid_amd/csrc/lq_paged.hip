@@ -78,7 +78,9 @@ __device__ __forceinline__ void load8(const typename Src::T* p, float (&x)[8]) {
 }
 
 // TOK tokens per workgroup.  A thread keeps one place of the rows (k or v, head, eight dims) and
-// moves it for every token, the loads of all of them in flight together.
+// moves it for every token, the loads of all of them in flight together.  Bound by HBM: 20452 tokens of
+// 8 heads of 128 in bfloat16 33 us, 5.0 TB/s read and written (one thread per value 87 us); up to 4096
+// tokens one a workgroup, so that there are workgroups enough.
 template <int TOK, class Src, class Dst>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     __shared__ int64_t rows[TOK];
@@ -151,11 +153,14 @@ __global__ __launch_bounds__(256) void append_i8_kernel(AppendArgs a) {
     if (row < 0) return;
     const uint32_t d = (threadIdx.x % LPR) * 8;
     // every lane of a wave takes the same number of rounds: the exchange below needs them all
-    for (uint32_t e = threadIdx.x / LPR; e < ((uint32_t)a.Hkv * 2 + 64 / LPR - 1) / (64 / LPR) * (64 / LPR); e += 256 / LPR) {
+    constexpr uint32_t PER = 64 / LPR;
+    const uint32_t rounded = ((uint32_t)a.Hkv * 2 + PER - 1) / PER * PER;
+    for (uint32_t e = threadIdx.x / LPR; e < rounded; e += 256 / LPR) {
         const bool is_v = e & 1, mine = e < (uint32_t)a.Hkv * 2 && d < (uint32_t)a.hd;
         const uint32_t h = e >> 1;
         float x[8] = {};
-        if (mine) load8<Src>(static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t * a.ld + (int64_t)h * a.hd + d, x);
+        const typename Src::T* src = static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t * a.ld;
+        if (mine) load8<Src>(src + (int64_t)h * a.hd + d, x);
         int32_t top = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[j]));
@@ -234,7 +239,8 @@ struct Piece {
 template <int WAVES>
 struct Line {
     static constexpr int STEP = WAVES * PG_K, NT = 64 * WAVES, START = 256 / STEP;
-    int64_t share, at, stop, start, base;  // steps of a workgroup; next step, end and start of this part; first step of sequence b
+    int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
+    int64_t base;                    // first step of sequence b
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
     int cost;                  // places of one head of sequence b on the line
     int unit, lead;            // steps that a part is a multiple of (0: any), places before a head's first step
@@ -453,15 +459,17 @@ struct Sums {
 template <class Q>
 __device__ __forceinline__ float paged_sum_again(const PagedArgs& a, const Piece& w, int r, int d, float M) {
     const typename Q::T* q = static_cast<const typename Q::T*>(a.q) + w.b * a.ldq + (int64_t)(w.h0 + r) * a.hd;
+    const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+    const float base = M == -INFINITY ? 0.0f : M - WEIGHT_SHIFT<Q>;
     float x = 0.0f;
     for (int key = w.begin; key < w.end; ++key) {
-        const int64_t row0 = position_row(key, a.table + (int64_t)w.b * a.table_stride, a.table_stride, a.pages, a.Hkv, a.page);
+        const int64_t row0 = position_row(key, table, a.table_stride, a.pages, a.Hkv, a.page);
         if (row0 < 0) return __builtin_nanf("");
         const int64_t row = row0 + (int64_t)w.hk * a.page;
         const typename Q::T* k = static_cast<const typename Q::T*>(a.k) + row * a.hd;
         float s = 0.0f;
         for (int i = 0; i < a.hd; ++i) s = __builtin_fmaf(Q::load(q[i]), Q::load(k[i]), s);
-        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale * LOG2E, -(M == -INFINITY ? 0.0f : M - WEIGHT_SHIFT<Q>)));
+        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale * LOG2E, -base));
         x = __builtin_fmaf(f, Q::load(static_cast<const typename Q::T*>(a.v)[row * a.hd + d]), x);
     }
     return x;
@@ -516,7 +524,11 @@ __device__ __forceinline__ void paged_finish(const PagedArgs& a, const Piece& w,
 }
 
 // V rows in LDS: 16-byte chunk c of row r lies at chunk c ^ v_swz(r), so that the transposing reads (4 rows,
-// 2 chunks for 16 lanes) and the writes spread over the banks; K rows (8 lanes read 8 rows): c ^ (r & 7).
+// 2 chunks for 16 lanes) and the writes spread over the banks; K rows (16 lanes read 16 rows): c ^ k_swz(r).
+template <int HDP>
+__device__ __forceinline__ int k_swz(int r) {
+    return HDP == 64 ? (r >> 1) & 7 : HDP % 128 == 0 ? r & 15 : r & 7;
+}
 template <int HDP>
 __device__ __forceinline__ int v_swz(int r) {
     return HDP == 64 ? 2 * ((r >> 1) & 3) : HDP % 128 == 0 ? 2 * (r & 7) : 2 * (r & 3);
@@ -527,6 +539,9 @@ constexpr int PG_IDS = 512;  // positions of a wave between two looks into the t
 // fp16 / bfloat16 cache.  K and V tiles are copied to the wave's LDS 16 bytes a lane, NST tiles deep: the
 // copies of a row are one contiguous access, they need no registers, and a wave waits only for
 // its oldest tile.  The byte offsets of PG_IDS positions at a time are looked up before their copies.
+// Bound by HBM: 64 sequences of 256 to 8191 positions, 8 heads of 128, 108 us with the join (5.5 TB/s); of
+// 8192 each 336 us (6.4 TB/s).  Rows loaded to registers, 64 bytes of each at a time: 130 us, the
+// first.
 template <int HDP, int WAVES, int NST, bool EXACT, class Q>
 __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     constexpr int CPR = HDP / 8, COPIES = PG_K * CPR / 64, KS = HDP / 32, DT = HDP / 16;
@@ -546,7 +561,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
         const int r = (64 * i + lane) / CPR, x = (64 * i + lane) % CPR;
-        kch[i] = (x ^ (r & 7)) * 16;
+        kch[i] = (x ^ k_swz<HDP>(r)) * 16;
         vch[i] = (x ^ v_swz<HDP>(r)) * 16;
     }
     const char* kp = static_cast<const char*>(a.k);
@@ -567,79 +582,81 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     };
     const float sl2 = a.scale * LOG2E;
     for (Piece w; line.next(a, w);) {
-    if (!EXACT) {  // chunks past the head dim are never copied and stay zeros
-        for (int i = lane; i < SLOT / 16; i += 64) reinterpret_cast<u4v*>(lds + wave * SLOT)[i] = u4v{0, 0, 0, 0};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    u4v qf[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, 32 * s + 8 * g, hd);
-    const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
-    Sums<DT, Q> sums;
-    bool bad = w.over || a.pages == 0;
-    constexpr int STEP = WAVES * PG_K;
-    for (int sub = w.begin; sub < w.end && a.pages > 0; sub += WAVES * PG_IDS) {
-        const int stop = min(sub + WAVES * PG_IDS, w.end);
-        const int first = sub + wave * PG_K;
-        const int tiles = first < stop ? (stop - first + STEP - 1) / STEP : 0;
-        for (int e = lane; e < tiles * PG_K; e += 64) {
-            const int key = first + (e / PG_K) * STEP + (e % PG_K);
-            int64_t off = 0;  // row 0 stands in past the end and for a bad page: its score and values are dropped
-            if (key < stop) {
-                const uint32_t col = (uint32_t)key / (uint32_t)a.page;
-                const int id = table[col];  // the length lies within the table
-                if (id >= 0 && id < a.pages)
-                    off = (((int64_t)id * a.Hkv + w.hk) * a.page + (key - (int)(col * (uint32_t)a.page))) * (2 * hd);
-                else
-                    bad = true;
-            }
-            offsets[wave][e] = off;
+        if (!EXACT) {  // chunks past the head dim are never copied and stay zeros
+            for (int i = lane; i < SLOT / 16; i += 64) reinterpret_cast<u4v*>(lds + wave * SLOT)[i] = u4v{0, 0, 0, 0};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        u4v qf[KS];
 #pragma unroll
-        for (int t = 0; t < NST; ++t)
-            if (t < tiles) issue(t);
-        for (int t = 0; t < tiles; ++t) {
-            const int later = min(NST - 1, tiles - 1 - t);  // tiles that may still be on their way
-            static_assert(NST <= 4 && 2 * (NST - 1) * COPIES < 64, "the counter's range");
-            if (later == 0) wait_vmcnt<0>();
-            else if (later == 1) wait_vmcnt<2 * COPIES>();
-            else if (later == 2) wait_vmcnt<(NST > 2 ? 4 : 0) * COPIES>();
-            else wait_vmcnt<(NST > 3 ? 6 : 0) * COPIES>();
-            asm volatile("" ::: "memory");
-            const uint32_t kt = slot + (t % NST) * 2 * TILE, vt = kt + TILE;
-            const int left = stop - (first + t * STEP);  // positions of this tile that exist
-            vf4 sc[2];
-#pragma unroll
-            for (int T = 0; T < 2; ++T) {
-                sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    sc[T] = mfma_16x16x32(Q{}, lds_read16(kt + (16 * T + l16) * ROW + (((4 * s + g) ^ (l16 & 7)) << 4)),
-                                          qf[s], sc[T]);
+        for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, 32 * s + 8 * g, hd);
+        const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+        Sums<DT, Q> sums;
+        bool bad = w.over || a.pages == 0;
+        constexpr int STEP = WAVES * PG_K;
+        for (int sub = w.begin; sub < w.end && a.pages > 0; sub += WAVES * PG_IDS) {
+            const int stop = min(sub + WAVES * PG_IDS, w.end);
+            const int first = sub + wave * PG_K;
+            const int tiles = first < stop ? (stop - first + STEP - 1) / STEP : 0;
+            for (int e = lane; e < tiles * PG_K; e += 64) {
+                const int key = first + (e / PG_K) * STEP + (e % PG_K);
+                int64_t off = 0;  // row 0 stands in past the end and for a bad page: its score and values are dropped
+                if (key < stop) {
+                    const uint32_t col = (uint32_t)key / (uint32_t)a.page;
+                    const int id = table[col];  // the length lies within the table
+                    if (id >= 0 && id < a.pages)
+                        off = (((int64_t)id * a.Hkv + w.hk) * a.page + (key - (int)(col * (uint32_t)a.page))) * (2 * hd);
+                    else
+                        bad = true;
+                }
+                offsets[wave][e] = off;
             }
-            const bool whole = left >= PG_K;
-            sums.weights(sc, sl2, whole, left - 4 * g);
-            if (!whole) {  // values past the end as zeros: their weight 0 must meet no infinity or NaN
-                const int r = lane & 31;
-                if (r >= left)
-                    for (int c = lane >> 5; c < CPR; c += 2)
-                        *reinterpret_cast<lds_u4v*>(vt + r * ROW + c * 16) = u4v{0, 0, 0, 0};
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < NST; ++t)
+                if (t < tiles) issue(t);
+            for (int t = 0; t < tiles; ++t) {
+                const int later = min(NST - 1, tiles - 1 - t);  // tiles that may still be on their way
+                static_assert(NST <= 4 && 2 * (NST - 1) * COPIES < 64, "the counter's range");
+                if (later == 0) wait_vmcnt<0>();
+                else if (later == 1) wait_vmcnt<2 * COPIES>();
+                else if (later == 2) wait_vmcnt<(NST > 2 ? 4 : 0) * COPIES>();
+                else wait_vmcnt<(NST > 3 ? 6 : 0) * COPIES>();
+                asm volatile("" ::: "memory");
+                const uint32_t kt = slot + (t % NST) * 2 * TILE, vt = kt + TILE;
+                const int left = stop - (first + t * STEP);  // positions of this tile that exist
+                vf4 sc[2];
+#pragma unroll
+                for (int T = 0; T < 2; ++T) {
+                    sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+                        sc[T] = mfma_16x16x32(Q{}, lds_read16(kt + (16 * T + l16) * ROW +
+                                                              (((4 * s + g) ^ k_swz<HDP>(l16)) << 4)),
+                                              qf[s], sc[T]);
+                }
+                const bool whole = left >= PG_K;
+                sums.weights(sc, sl2, whole, left - 4 * g);
+                if (!whole) {  // values past the end as zeros: their weight 0 must meet no infinity or NaN
+                    const int r = lane & 31;
+                    if (r >= left)
+                        for (int c = lane >> 5; c < CPR; c += 2)
+                            *reinterpret_cast<lds_u4v*>(vt + r * ROW + c * 16) = u4v{0, 0, 0, 0};
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+                sums.template accumulate<ROW>(sc, vt, v_swz<HDP>);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
+                if (t + NST < tiles) issue(t + NST);
             }
-            sums.template accumulate<ROW>(sc, vt, v_swz<HDP>);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
-            if (t + NST < tiles) issue(t + NST);
         }
-    }
-    paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
+        paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
 }
 
 // int8 cache.  Codes are exact in 16 bits: they are loaded to registers (a tile ahead), widened there,
 // and V goes to the wave's LDS as bfloat16.  The key's scale multiplies the score, the value's scale
-// the weight, which is bfloat16 for its range.  The widening bounds it: one and a half vector
-// instructions a code.
+// the weight, which is bfloat16 for its range.  The widening bounds it, one and a half vector
+// instructions a code: 131071 positions and a second sequence, 8 heads of 128, 81 us with the join (4.8
+// TB/s; 125 us with the compiler's own conversions).
 template <int HDP, bool EXACT, class Q>
 __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8_kernel(PagedArgs a) {
     using P = ElemBF16;
@@ -659,108 +676,109 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8
     float* scales = reinterpret_cast<float*>(slot + SLOT - 256);
     const uint32_t slot_at = (uint32_t)reinterpret_cast<uintptr_t>(slot);
     for (Piece w; line.next(a, w);) {
-    // dims of this lane's eight slots in step s of the first product: a load brings 16 codes
-    auto dims = [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
-    u4v qf[KS];
+        // dims of this lane's eight slots in step s of the first product: a load brings 16 codes
+        auto dims = [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
+        u4v qf[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, dims(s), hd);
-    const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
-    // page number of a position, -1 past the end
-    auto page_of = [&](int key) -> int { return key < w.end ? table[(uint32_t)key / (uint32_t)a.page] : -1; };
-    bool bad = w.over || a.pages == 0;
-    // a tile in registers: rows l16 and 16 + l16 of K and V, and their scales
-    u4v kr[2][HALF], vr[2][HALF];
-    float ksc[2], vsc[2];
-    auto fetch = [&](int key0, const int (&id)[2]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-            const int key = key0 + 16 * T + l16;
-            const bool ok = id[T] >= 0 && id[T] < a.pages;
-            bad |= key < w.end && !ok;
-            // row 0 stands in: its scores and values are dropped
-            const int64_t row = ok ? ((int64_t)id[T] * a.Hkv + w.hk) * a.page + (uint32_t)key % (uint32_t)a.page : 0;
-            const int8_t* kp = static_cast<const int8_t*>(a.k) + row * hd;
-            const int8_t* vp = static_cast<const int8_t*>(a.v) + row * hd;
-            ksc[T] = a.ks[row];
-            vsc[T] = a.vs[row];
-            auto load = [&](const int8_t* p, int d) {
-                if constexpr (EXACT) return *reinterpret_cast<const u4v*>(p + d);
-                const u2v lo = *reinterpret_cast<const u2v*>(p + (d < hd ? d : 0));
-                const u2v hi = *reinterpret_cast<const u2v*>(p + (d + 8 < hd ? d + 8 : 0));
-                return u4v{lo[0], lo[1], hi[0], hi[1]};
-            };
-#pragma unroll
-            for (int s = 0; s < HALF; ++s) {
-                kr[T][s] = load(kp, 64 * s + 16 * g);
-                vr[T][s] = load(vp, 64 * s + 16 * g);
-            }
-        }
-    };
-    Sums<DT, P> sums;
-    constexpr int STEP = WAVES * PG_K;
-    int key0 = w.begin + wave * PG_K;
-    if (a.pages > 0 && key0 < w.end) {
-        int id[2], next[2];
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-            id[T] = page_of(key0 + 16 * T + l16);
-            next[T] = page_of(key0 + STEP + 16 * T + l16);
-        }
-        fetch(key0, id);
-        for (; key0 < w.end; key0 += STEP) {
-            const int left = w.end - key0;
-            const bool whole = left >= PG_K;
-            vf4 sc[2];
+        for (int s = 0; s < KS; ++s) qf[s] = paged_query(a, w, l16, dims(s), hd);
+        const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+        // page number of a position, -1 past the end
+        auto page_of = [&](int key) -> int { return key < w.end ? table[(uint32_t)key / (uint32_t)a.page] : -1; };
+        bool bad = w.over || a.pages == 0;
+        // a tile in registers: rows l16 and 16 + l16 of K and V, and their scales
+        u4v kr[2][HALF], vr[2][HALF];
+        float ksc[2], vsc[2];
+        auto fetch = [&](int key0, const int (&id)[2]) __attribute__((always_inline)) {
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
-                sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
+                const int key = key0 + 16 * T + l16;
+                const bool ok = id[T] >= 0 && id[T] < a.pages;
+                bad |= key < w.end && !ok;
+                // row 0 stands in: its scores and values are dropped
+                const int64_t row = ok ? ((int64_t)id[T] * a.Hkv + w.hk) * a.page + (uint32_t)key % (uint32_t)a.page : 0;
+                const int8_t* kp = static_cast<const int8_t*>(a.k) + row * hd;
+                const int8_t* vp = static_cast<const int8_t*>(a.v) + row * hd;
+                ksc[T] = a.ks[row];
+                vsc[T] = a.vs[row];
+                auto load = [&](const int8_t* p, int d) {
+                    if constexpr (EXACT) return *reinterpret_cast<const u4v*>(p + d);
+                    const u2v lo = *reinterpret_cast<const u2v*>(p + (d < hd ? d : 0));
+                    const u2v hi = *reinterpret_cast<const u2v*>(p + (d + 8 < hd ? d + 8 : 0));
+                    return u4v{lo[0], lo[1], hi[0], hi[1]};
+                };
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const uint32_t lo = kr[T][s >> 1][2 * (s & 1)], hi = kr[T][s >> 1][2 * (s & 1) + 1];
-                    const u2v x = widen4(Q{}, lo), y = widen4(Q{}, hi);
-                    sc[T] = mfma_16x16x32(Q{}, u4v{x[0], x[1], y[0], y[1]}, qf[s], sc[T]);  // codes past hd meet zeros
+                for (int s = 0; s < HALF; ++s) {
+                    kr[T][s] = load(kp, 64 * s + 16 * g);
+                    vr[T][s] = load(vp, 64 * s + 16 * g);
                 }
             }
+        };
+        Sums<DT, P> sums;
+        constexpr int STEP = WAVES * PG_K;
+        int key0 = w.begin + wave * PG_K;
+        if (a.pages > 0 && key0 < w.end) {
+            int id[2], next[2];
 #pragma unroll
             for (int T = 0; T < 2; ++T) {
-                const int r = 16 * T + l16;
+                id[T] = page_of(key0 + 16 * T + l16);
+                next[T] = page_of(key0 + STEP + 16 * T + l16);
+            }
+            fetch(key0, id);
+            for (; key0 < w.end; key0 += STEP) {
+                const int left = w.end - key0;
+                const bool whole = left >= PG_K;
+                vf4 sc[2];
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const uint32_t lo = vr[T][s >> 1][2 * (s & 1)], hi = vr[T][s >> 1][2 * (s & 1) + 1];
-                    const u2v x = widen4(P{}, lo), y = widen4(P{}, hi);
-                    *reinterpret_cast<u4v*>(slot + r * ROW + (((dims(s) >> 3) ^ v_swz<HDP>(r)) << 4)) =
-                        u4v{x[0], x[1], y[0], y[1]};
+                for (int T = 0; T < 2; ++T) {
+                    sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const uint32_t lo = kr[T][s >> 1][2 * (s & 1)], hi = kr[T][s >> 1][2 * (s & 1) + 1];
+                        const u2v x = widen4(Q{}, lo), y = widen4(Q{}, hi);
+                        // codes past hd meet zeros
+                        sc[T] = mfma_16x16x32(Q{}, u4v{x[0], x[1], y[0], y[1]}, qf[s], sc[T]);
+                    }
                 }
-                scales[r] = ksc[T];
-                scales[32 + r] = r < left ? vsc[T] : 0.0f;  // codes are finite: a weight of 0 drops them
+#pragma unroll
+                for (int T = 0; T < 2; ++T) {
+                    const int r = 16 * T + l16;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const uint32_t lo = vr[T][s >> 1][2 * (s & 1)], hi = vr[T][s >> 1][2 * (s & 1) + 1];
+                        const u2v x = widen4(P{}, lo), y = widen4(P{}, hi);
+                        *reinterpret_cast<u4v*>(slot + r * ROW + (((dims(s) >> 3) ^ v_swz<HDP>(r)) << 4)) =
+                            u4v{x[0], x[1], y[0], y[1]};
+                    }
+                    scales[r] = ksc[T];
+                    scales[32 + r] = r < left ? vsc[T] : 0.0f;  // codes are finite: a weight of 0 drops them
+                }
+                // the next tile, and the page numbers of the one after it
+                if (key0 + STEP < w.end) {
+                    id[0] = next[0];
+                    id[1] = next[1];
+#pragma unroll
+                    for (int T = 0; T < 2; ++T) next[T] = page_of(key0 + 2 * STEP + 16 * T + l16);
+                    fetch(key0 + STEP, id);
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's LDS writes, before any lane reads them
+#pragma unroll
+                for (int T = 0; T < 2; ++T) {
+                    const vf4 f = *reinterpret_cast<const vf4*>(scales + 16 * T + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
+                }
+                sums.weights(sc, sl2, whole, left - 4 * g);
+#pragma unroll
+                for (int T = 0; T < 2; ++T) {
+                    const vf4 f = *reinterpret_cast<const vf4*>(scales + 32 + 16 * T + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
+                }
+                sums.template accumulate<ROW>(sc, slot_at, v_swz<HDP>);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads, before the next tile's writes
             }
-            // the next tile, and the page numbers of the one after it
-            if (key0 + STEP < w.end) {
-                id[0] = next[0];
-                id[1] = next[1];
-#pragma unroll
-                for (int T = 0; T < 2; ++T) next[T] = page_of(key0 + 2 * STEP + 16 * T + l16);
-                fetch(key0 + STEP, id);
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's LDS writes, before any lane reads them
-#pragma unroll
-            for (int T = 0; T < 2; ++T) {
-                const vf4 f = *reinterpret_cast<const vf4*>(scales + 16 * T + 4 * g);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
-            }
-            sums.weights(sc, sl2, whole, left - 4 * g);
-#pragma unroll
-            for (int T = 0; T < 2; ++T) {
-                const vf4 f = *reinterpret_cast<const vf4*>(scales + 32 + 16 * T + 4 * g);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
-            }
-            sums.template accumulate<ROW>(sc, slot_at, v_swz<HDP>);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads, before the next tile's writes
         }
-    }
-    paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
+        paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
 }
 
@@ -825,8 +843,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     }
 }
 
-// Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims).  Up to PG_ALONE positions each workgroup takes a sequence whole: the
-// second launch would cost more than it gives (8 sequences of 640: 9.1 us against 12.5).
+// Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims).
+// Up to PG_ALONE positions each workgroup takes a sequence whole: the second launch would cost more
+// than it gives (8 sequences of 640: 9.1 us against 12.5).
 constexpr int PG_GROUPS = 512, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
 // bytes of the table of pieces, and the slots of a call (two to a workgroup)
 int64_t pieces_bytes(int64_t units) { return (units * (int64_t)sizeof(int2) + 15) / 16 * 16; }
@@ -869,7 +888,9 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
             if (vec && hd <= 64) hipLaunchKernelGGL((append_i8_kernel<8, S>), one, dim3(256), 0, st, a);
             else if (vec && hd <= 128) hipLaunchKernelGGL((append_i8_kernel<16, S>), one, dim3(256), 0, st, a);
             else if (vec && hd <= 256) hipLaunchKernelGGL((append_i8_kernel<32, S>), one, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((append_i8_any_kernel<S>), dim3((unsigned)tokens, (unsigned)(2 * Hkv)), dim3(64), 0, st, a);
+            else
+                hipLaunchKernelGGL((append_i8_any_kernel<S>), dim3((unsigned)tokens, (unsigned)(2 * Hkv)), dim3(64), 0,
+                                   st, a);
             return;
         }
         with_half(cache_type, [&](auto c) {
@@ -884,7 +905,8 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
 
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length) {
     if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || max_length <= PG_ALONE) return 0;
-    return (size_t)pieces_bytes(B * Hkv * ((H / Hkv + 15) / 16)) + (size_t)2 * paged_groups(hd) * 16 * (hd + 2) * sizeof(float);
+    return (size_t)pieces_bytes(B * Hkv * ((H / Hkv + 15) / 16)) +
+           (size_t)2 * paged_groups(hd) * 16 * (hd + 2) * sizeof(float);
 }
 
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,

@@ -239,7 +239,8 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int b = 0; b < KT; ++b)
-                sc[b] = mfma_32x32x16(E{}, lds_read16(at + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)), qf[s], sc[b]);
+                sc[b] = mfma_32x32x16(E{}, lds_read16(at + b * 32 * HDP * 2 + (((2 * s + hh) ^ k_swz(col)) << 4)),
+                                      qf[s], sc[b]);
     };
     auto mask = [&](int t, f16v (&sc)[KT]) __attribute__((always_inline)) {
         const int left = lim - t * PT_K - k32 - 4 * hh;
@@ -398,7 +399,8 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
                 const int dim = 32 * d + 2 * i + 4 * hh;
                 if (dim < hd) {
                     if constexpr (TWO) {
-                        *reinterpret_cast<vf4*>(orow + dim) = vf4{o[d][i] * r, o[d][i + 1] * r, o[d][i + 2] * r, o[d][i + 3] * r};
+                        *reinterpret_cast<vf4*>(orow + dim) = vf4{o[d][i] * r, o[d][i + 1] * r, o[d][i + 2] * r,
+                                                                  o[d][i + 3] * r};
                     } else {
                         *reinterpret_cast<u2v*>(orow + dim) = u2v{pack2(E{}, o[d][i] * r, o[d][i + 1] * r),
                                                                   pack2(E{}, o[d][i + 2] * r, o[d][i + 3] * r)};

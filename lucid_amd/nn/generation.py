@@ -74,6 +74,18 @@ def _pages(op, k_pages, v_pages, k_scale, v_scale, table, lengths):
     return tuple(int(n) for n in k_pages.shape)
 
 
+def _scratch(nbytes: int, stream):
+    """(address, holder) of workspace for one call: the thread's own on the default stream; on
+    another stream memory of its own, which is reused only after that stream's work."""
+    if nbytes == 0:
+        return None, None
+    if stream is None:
+        return workspace.get(nbytes), None
+    t = empty((nbytes,), np.uint8, "gpu")
+    t.record_stream(stream)
+    return t.data_ptr(), t
+
+
 def _opt(t) -> int | None:
     return t.data_ptr() if t is not None else None
 
@@ -154,10 +166,11 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
         raise TypeError(f"{op}: a cache of {k_pages.dtype} for queries of {dt}")
     out = empty((B, h, hd), _out_type(out_dtype, dt, op), "gpu")
     size = _C.lib().lq_paged_attention_workspace_size(B, h, hkv, hd, max_length)
+    ws, _held = _scratch(size, stream)
     _C.call("lq_paged_attention", q.data_ptr(), FLOAT_TYPE_CODE[dt], ldq, B, h, hkv, hd, k_pages.data_ptr(),
             v_pages.data_ptr(), _CACHE_TYPE[k_pages.dtype], _opt(k_scale), _opt(v_scale), pages, page, table.data_ptr(),
             table.shape[1], lengths.data_ptr(), max_length, _scale(scale, hd, op), out.data_ptr(),
-            FLOAT_TYPE_CODE[out.dtype], workspace.get(size), size, stream)
+            FLOAT_TYPE_CODE[out.dtype], ws, size, stream)
     return out
 
 
@@ -218,9 +231,10 @@ def token_logprobs(logits: Tensor, targets: Tensor, top: int = 0, stream=None):
     lp, ent, lse = (empty((rows,), float32, "gpu") for _ in range(3))
     top_lp, top_ids = empty((rows, top), float32, "gpu"), empty((rows, top), np.int32, "gpu")
     size = _C.lib().lq_token_logprobs_workspace_size(rows, vocab, top)
+    ws, _held = _scratch(size, stream)
     _C.call("lq_token_logprobs", logits.data_ptr(), FLOAT_TYPE_CODE[dt], vocab, rows, vocab, targets.data_ptr(), top,
-            lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(), workspace.get(size),
-            size, stream)
+            lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(), ws, size,
+            stream)
     return lp, ent, lse, top_lp, top_ids
 
 
@@ -290,8 +304,8 @@ class PageTable:
         new = self._lengths + counts
         need = [-(-int(n) // self.page) for n in new]
         if max(need) > self._table.shape[1]:
-            raise ValueError(f"PageTable.grow: a sequence of {int(new.max())} positions needs {max(need)} pages, its row "
-                             f"holds {self._table.shape[1]}")
+            raise ValueError(f"PageTable.grow: a sequence of {int(new.max())} positions needs {max(need)} pages, its "
+                             f"row holds {self._table.shape[1]}")
         more = sum(n - h for n, h in zip(need, self._held))
         if more > len(self._free):
             raise MemoryError(f"PageTable.grow: {more} pages needed, {len(self._free)} free")

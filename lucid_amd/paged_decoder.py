@@ -49,8 +49,8 @@ class PagedDecoder:
             _C.call("lq_layer_norm_f32", x.data_ptr(), D_MODEL, y.data_ptr(), D_MODEL, rows, D_MODEL, None, None,
                     np.float32(1e-5), None)
         else:
-            _C.call("lq_add_layer_norm_f32", x.data_ptr(), D_MODEL, res.data_ptr(), D_MODEL, y.data_ptr(), D_MODEL, rows,
-                    D_MODEL, None, None, np.float32(1e-5), None)
+            _C.call("lq_add_layer_norm_f32", x.data_ptr(), D_MODEL, res.data_ptr(), D_MODEL, y.data_ptr(), D_MODEL,
+                    rows, D_MODEL, None, None, np.float32(1e-5), None)
         return y
 
     def _hidden(self, ids: np.ndarray, positions: np.ndarray, attend) -> Tensor:
@@ -104,8 +104,8 @@ class PagedDecoder:
             self.cache[i].append_qkv(qkv, HEADS, starts)
             return F.prompt_attention_qkv(qkv, HEADS, HEADS, starts, out_dtype=float32)
 
-        h = self._hidden(np.concatenate([toks[s] for s in seqs]), np.concatenate([np.arange(len(toks[s])) for s in seqs]),
-                         attend)
+        h = self._hidden(np.concatenate([toks[s] for s in seqs]),
+                         np.concatenate([np.arange(len(toks[s])) for s in seqs]), attend)
         return self.qdec.head(self._rows(h, ends[seqs] - 1))
 
     def step(self, tokens: dict[int, int]) -> Tensor:
@@ -200,9 +200,9 @@ def _main(argv: list[str]) -> None:
     t0 = time.perf_counter()
     toks, scores, _ = rt.generate(prompts, steps)
     dt = time.perf_counter() - t0
-    print(f"{len(prompts)} prompts of {sum(map(len, prompts))} tokens and {toks.size} generated tokens: {dt * 1e3:.1f} ms; "
-          f"mean log probability {scores.mean():.3f}")
     rows = sum(map(len, prompts))
+    print(f"{len(prompts)} prompts of {rows} tokens and {toks.size} generated tokens: {dt * 1e3:.1f} ms; "
+          f"mean log probability {scores.mean():.3f}")
     value, _, bias = rt.tune(prompts, np.ones(rows) / rows, 0.01 / rows)
     print(f"objective {value:.4f}, largest bias gradient {np.abs(bias).max():.3e}")
 

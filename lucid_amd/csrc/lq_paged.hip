@@ -252,16 +252,6 @@ struct Line {
         steps = (len + STEP - 1) / STEP;
         cost = unit ? (steps + unit - 1) / unit * unit : steps ? steps + START : 0;
     }
-    // Sum over the workgroup's threads; `sums` holds WAVES numbers.
-    __device__ __forceinline__ static int64_t add_all(int64_t v, int64_t* sums) {
-        for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0;
-        for (int w = 0; w < WAVES; ++w) v += sums[w];
-        return v;
-    }
     // Finds the part of workgroup blockIdx.x; `scan` holds NT numbers.
     __device__ __forceinline__ void init(const PagedArgs& a, int64_t* scan) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -277,15 +267,22 @@ struct Line {
             return;
         }
         const int per = (a.B + NT - 1) / NT, first = min(tid * per, a.B), last = min(first + per, a.B);
-        // parts of 256 or 512 positions, if the workgroups suffice: none then has two pieces
-        int64_t small = 0, large = 0;
+        // parts of 256 or 512 positions, if the workgroups suffice: none then has two pieces (a thread counts no
+        // further than 2^20 parts, more than there are workgroups)
+        int64_t n256 = 0, n512 = 0;
         for (int i = first; i < last; ++i) {
             sequence(a, i);
-            small += (int64_t)heads * ((steps + 256 / STEP - 1) / (256 / STEP));
-            large += (int64_t)heads * ((steps + 512 / STEP - 1) / (512 / STEP));
+            n256 += (int64_t)heads * ((steps + 256 / STEP - 1) / (256 / STEP));
+            n512 += (int64_t)heads * ((steps + 512 / STEP - 1) / (512 / STEP));
         }
-        small = add_all(small, scan);
-        large = add_all(large, scan);
+        int small = wave_add((int)min(n256, (int64_t)1 << 20)), large = wave_add((int)min(n512, (int64_t)1 << 20));
+        if (lane == 0) scan[wave] = (int64_t)small << 32 | large;
+        __syncthreads();
+        small = large = 0;
+        for (int w = 0; w < WAVES; ++w) {
+            small += (int)(scan[w] >> 32);
+            large += (int)scan[w];
+        }
         unit = small <= a.groups ? 256 / STEP : large <= a.groups ? 512 / STEP : 0;
         lead = unit ? 0 : START;
         int64_t mine = 0;
@@ -554,7 +551,6 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;
     line.init(a, scan);
-    paged_empty<WAVES, Q>(a);
     const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
     // copy i of a tile: LDS chunk 64 i + lane, row (64 i + lane) / CPR
     int kch[COPIES], vch[COPIES];
@@ -650,6 +646,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
         }
         paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
+    paged_empty<WAVES, Q>(a);
 }
 
 // int8 cache.  Codes are exact in 16 bits: they are loaded to registers (a tile ahead), widened there,
@@ -670,7 +667,6 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;
     line.init(a, scan);
-    paged_empty<WAVES, Q>(a);
     const float sl2 = a.scale * LOG2E;
     uint8_t* slot = lds + wave * SLOT;
     float* scales = reinterpret_cast<float*>(slot + SLOT - 256);
@@ -780,6 +776,7 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8
         }
         paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
+    paged_empty<WAVES, Q>(a);
 }
 
 // The pieces of one (sequence, query head) joined by one workgroup: hd / 4 lanes take four dims each
@@ -796,12 +793,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     // the first piece, then the first ones of the workgroups that follow
     auto piece = [&](int s) { return (int64_t)16 * (s == 0 ? info.x : (info.x & ~1) + 2 * s) + row; };
     const int64_t at = (int64_t)b * a.H + h;
-    const float* ml = a.part_ml;
+    const f2v* ml = reinterpret_cast<const f2v*>(a.part_ml);  // maximum and sum of a piece's row
     const float* po = a.part_o;
     const int quads = a.hd / 4, teams = 256 / quads, team = tid / quads, d = (tid - team * quads) * 4;
-    float M = -INFINITY;
-    for (int s = tid; s < used; s += 256) M = fmaxf(M, ml[2 * piece(s)]);
-    for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    // a thread's first pieces and every piece's statistics are on their way before anything waits
+    constexpr int AHEAD = 8;
+    vf4 p[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int s = team + i * teams;
+        p[i] = team < teams && s < used ? *reinterpret_cast<const vf4*>(po + piece(s) * a.hd + d) : vf4{0.f, 0.f, 0.f, 0.f};
+    }
+    f2v mine = tid < used ? ml[piece(tid)] : f2v{-INFINITY, 0.0f};
+    float M = mine[0];
+    for (int s = tid + 256; s < used; s += 256) M = fmaxf(M, ml[piece(s)][0]);
+    M = unkey(wave_max(fkey(M)));
     if (lane == 0) red[tid >> 6] = M;
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -811,23 +817,27 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     for (int s0 = 0; s0 < used; s0 += 256) {
         const int n = min(256, used - s0);
         __syncthreads();
-        float w = 0.0f;
-        if (tid < n) {
-            const float e = __builtin_amdgcn_exp2f(ml[2 * piece(s0 + tid)] - base);
-            f[tid] = e;
-            w = e * ml[2 * piece(s0 + tid) + 1];
-        }
-        w = ln_wave_sum(w);
+        if (s0 > 0) mine = tid < n ? ml[piece(s0 + tid)] : f2v{-INFINITY, 0.0f};
+        const float e = tid < n ? __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
+        f[tid] = e;
+        const float w = ln_wave_sum(tid < n ? e * mine[1] : 0.0f);
         if (lane == 0) red[tid >> 6] = w;
         __syncthreads();
         L += (red[0] + red[1]) + (red[2] + red[3]);
-        if (team < teams) {
-#pragma unroll 8
-            for (int s = team; s < n; s += teams) {
-                const vf4 p = *reinterpret_cast<const vf4*>(po + piece(s0 + s) * a.hd + d);
+        if (team >= teams) continue;
+        int s = team;
+        if (s0 == 0) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(f[s], p[i], x[i]);
-            }
+            for (int i = 0; i < AHEAD; ++i, s += teams)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (s < n) x[j] = __builtin_fmaf(f[s], p[i][j], x[j]);
+        }
+#pragma unroll 4
+        for (; s < n; s += teams) {
+            const vf4 q = *reinterpret_cast<const vf4*>(po + piece(s0 + s) * a.hd + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(f[s], q[j], x[j]);
         }
     }
     sums[tid] = x;

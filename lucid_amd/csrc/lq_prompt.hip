@@ -86,12 +86,21 @@ constexpr int PT_WAVES = 4, PT_K = 64;  // waves of a workgroup, keys of a tile
 // blocks have more keys, and the longest work starts first: up to 64 sequences, block L of every
 // sequence that has one before any block L - 1 (at the count of blocks from L on, which a search
 // finds); with more, blocks last to first within each sequence.  Every wave finds it by itself, a lane
-// for each of 64 sequences.
+// for each of 64 sequences, and takes the sequence's rows from that lane.
 template <int QB>
-__device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64_t& seq, int64_t& blk) {
+__device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, Packed& pk, int64_t& blk) {
     const int lane = threadIdx.x & 63;
+    Packed mine{0, 0, 0, 0};  // this lane's sequence
     auto blocks = [&](int64_t s) {
-        return s < a.seqs ? (int)((packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k).nq + QB - 1) / QB) : 0;
+        if (s >= a.seqs) return 0;
+        mine = packed_sequence(a.qs, a.ks, s, a.total_q, a.total_k);
+        return (int)((mine.nq + QB - 1) / QB);
+    };
+    auto take = [&](int l) {  // the rows of lane l's sequence, in scalar registers
+        pk.q0 = __builtin_amdgcn_readlane((int)mine.q0, l);
+        pk.nq = __builtin_amdgcn_readlane((int)mine.nq, l);
+        pk.k0 = __builtin_amdgcn_readlane((int)mine.k0, l);
+        pk.nk = __builtin_amdgcn_readlane((int)mine.nk, l);
     };
     if (a.seqs <= 64) {
         const int cnt = blocks(lane);
@@ -104,7 +113,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64
         }
         uint64_t has = __ballot(cnt > lo);
         for (int64_t k = n - from(lo + 1); k > 0; --k) has &= has - 1;
-        seq = __builtin_ctzll(has);
+        take(__builtin_ctzll(has));
         blk = lo;
         return true;
     }
@@ -118,7 +127,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, int64
         const int all = __builtin_amdgcn_readlane(upto, 63);
         if (n < all) {
             const int l = __builtin_ctzll(__ballot(upto > n));
-            seq = base + l;
+            take(l);
             blk = __builtin_amdgcn_readlane(upto, l) - 1 - n;
             return true;
         }
@@ -158,11 +167,10 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
     // consecutive workgroups (on consecutive XCDs) take different key heads: an XCD's L2 then
     // serves few of them
     const int hk = hx % (uint32_t)a.Hkv, h = hk * group + hx / (uint32_t)a.Hkv;
-    int64_t seq, blk;
-    if (!find_block<QB>(a, n, seq, blk)) return;
-    seq = __builtin_amdgcn_readfirstlane((int)seq);  // what follows from it lies in scalar registers
+    Packed pk;
+    int64_t blk;
+    if (!find_block<QB>(a, n, pk, blk)) return;
     blk = __builtin_amdgcn_readfirstlane((int)blk);
-    const Packed pk = packed_sequence(a.qs, a.ks, seq, a.total_q, a.total_k);
     const bool causal = a.causal != 0;
     const int kg = wave % SPLIT, k32 = 64 / SPLIT * kg;  // this wave's keys of a tile begin at k32
     const int64_t qb = blk * QB, qw = qb + 32 * (wave / SPLIT);  // first query of the workgroup, of the wave

@@ -712,6 +712,57 @@ def test_token_logprobs_best_in_few_threads(gpu, dtype, top):
     _check(lse, want[2], want[5] + 2 * U * np.abs(want[2]), "lse")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 200003, 64), (3, 70001, 5), (128, 140000, 1), (5, 150001, 0)])
+def test_token_logprobs_rows_in_parts(gpu, dtype, rows, vocab, top):
+    """Rows shared by several workgroups: odd part boundaries, rows whose allowed tokens lie in one
+    part, ties across parts, NaN and a row that allows nothing."""
+    import lucid_amd.nn.functional as F
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32) * 2
+    if rows > 2:
+        x[0, :-40] = -np.inf       # fewer allowed than alternatives, all at the end
+        x[1, ::1000] = 30          # ties in every part
+        x[2] = -np.inf
+    if rows > 4:
+        x[3, vocab // 2] = np.nan
+    v, xh = _round(x, dtype)
+    t = rng.integers(vocab - 30, vocab, rows).astype(np.int32)
+    lp, ent, lse, tlp, tid = (a.numpy() for a in F.token_logprobs(_dev(xh), _i32(t), top))
+    assert _C.last_path() == "logprobs parts"
+    keep = np.arange(min(rows, 6))
+    wlp, went, wlse, wtlp, wids, rel = _logprob_want(v[keep], t[keep], top)
+    np.testing.assert_array_equal(tid[keep], wids)
+    some = ~np.isneginf(wlse)  # a row that allows nothing is looked at below
+    for got, want, bound in ((lse, wlse, rel + 2 * U * np.abs(wlse)), (lp, wlp, rel + 3 * U * np.abs(wlse)),
+                             (ent, went, rel * (2 + np.abs(went)) + 4 * U * np.abs(went))):
+        fin = np.isfinite(want)
+        _check(got[keep][fin & some], want[fin & some], bound[fin & some])
+        np.testing.assert_array_equal(np.isnan(got[keep][~fin & some]), np.isnan(want[~fin & some]))
+    if rows > 2:
+        assert lse[2] == -np.inf and ent[2] == 0 and lp[2] == -np.inf
+
+
+def test_token_logprobs_one_by_one(gpu):
+    """Many rows (one workgroup each) with more candidates above the cut than are collected."""
+    import lucid_amd.nn.functional as F
+    from lucid_amd import _C
+
+    rows, vocab, top = 130, 200000, 7
+    rng = np.random.default_rng(8)
+    large = np.arange(vocab) // 8 % 512 < 8
+    x = np.zeros((rows, vocab), np.float32)
+    x[0, large] = 50 + rng.permutation(large.sum()) % 256 / 4
+    x[129, large] = 50
+    v, xh = _round(x, "bfloat16")
+    _, _, _, tlp, tid = (a.numpy() for a in F.token_logprobs(_dev(xh), _i32(np.zeros(rows)), top))
+    assert _C.last_path() == "logprobs rows"
+    for r in (0, 1, 129):
+        np.testing.assert_array_equal(tid[r], _order(v[r:r + 1], top)[0])
+
+
 def test_token_logprobs_strided_rows_and_optional_outputs(gpu):
     from lucid_amd import _C
 

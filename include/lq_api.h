@@ -846,8 +846,9 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
  * tokens in order (ties: the lower index; NaN above everything) with their log probabilities, in
  * [rows][top].  d_logprobs, d_entropy, d_lse may be NULL; top 0 .. 64, at most vocab (2^30).  A logit of
  * -inf is a token that is not allowed (probability 0); a row without any allowed token has lse =
- * -inf, entropy 0 and log probabilities of -inf.  Workspace: lq_token_logprobs_workspace_size
- * bytes, no contents kept from call to call. */
+ * -inf, entropy 0 and log probabilities of -inf; a row with NaN or +inf has NaN.  Workspace:
+ * lq_token_logprobs_workspace_size bytes, 16-byte aligned (0 but for at most 128 long rows), no
+ * contents kept from call to call. */
 size_t lq_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int64_t top);
 int lq_token_logprobs(const void* d_x, int type, int64_t ldx, int64_t rows, int64_t vocab, const int32_t* d_targets,
                       int64_t top, float* d_logprobs, float* d_entropy, float* d_lse, float* d_top_logprobs,

@@ -531,7 +531,9 @@ __device__ __forceinline__ int v_swz(int r) {
     return HDP == 64 ? 2 * ((r >> 1) & 3) : HDP % 128 == 0 ? 2 * (r & 7) : 2 * (r & 3);
 }
 
-constexpr int PG_IDS = 512;  // positions of a wave between two looks into the table
+// positions of a wave between two looks into the table
+template <int WAVES>
+constexpr int PG_IDS = WAVES > 4 ? 128 : 512;
 
 // fp16 / bfloat16 cache.  K and V tiles are copied to the wave's LDS 16 bytes a lane, NST tiles deep: the
 // copies of a row are one contiguous access, they need no registers, and a wave waits only for
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     constexpr int CPR = HDP / 8, COPIES = PG_K * CPR / 64, KS = HDP / 32, DT = HDP / 16;
     constexpr int ROW = HDP * 2, TILE = PG_K * ROW, SLOT = 2 * NST * TILE;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOT];
-    __shared__ int64_t offsets[WAVES][PG_IDS];
+    __shared__ int64_t offsets[WAVES][PG_IDS<WAVES>];
     __shared__ float ml[WAVES][2][16];
     __shared__ int64_t scan[64 * WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
@@ -589,8 +591,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
         Sums<DT, Q> sums;
         bool bad = w.over || a.pages == 0;
         constexpr int STEP = WAVES * PG_K;
-        for (int sub = w.begin; sub < w.end && a.pages > 0; sub += WAVES * PG_IDS) {
-            const int stop = min(sub + WAVES * PG_IDS, w.end);
+        for (int sub = w.begin; sub < w.end && a.pages > 0; sub += WAVES * PG_IDS<WAVES>) {
+            const int stop = min(sub + WAVES * PG_IDS<WAVES>, w.end);
             const int first = sub + wave * PG_K;
             const int tiles = first < stop ? (stop - first + STEP - 1) / STEP : 0;
             for (int e = lane; e < tiles * PG_K; e += 64) {
@@ -655,7 +657,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
 // instructions a code: 131071 positions and a second sequence, 8 heads of 128, 81 us with the join (4.8
 // TB/s; 125 us with the compiler's own conversions).
 template <int HDP, bool EXACT, class Q>
-__global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 128 ? 2 : 1) void paged_i8_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) void paged_i8_kernel(PagedArgs a) {
     using P = ElemBF16;
     constexpr int WAVES = PG_I8_WAVES, KS = HDP / 32, HALF = HDP / 64, DT = HDP / 16;
     constexpr int ROW = HDP * 2, TILE = PG_K * ROW, OTILE = 16 * (HDP + 4) * 4;
@@ -802,7 +804,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
         const int s = team + i * teams;
-        p[i] = team < teams && s < used ? *reinterpret_cast<const vf4*>(po + piece(s) * a.hd + d) : vf4{0.f, 0.f, 0.f, 0.f};
+        p[i] = vf4{0.f, 0.f, 0.f, 0.f};
+        if (team < teams && s < used) p[i] = *reinterpret_cast<const vf4*>(po + piece(s) * a.hd + d);
     }
     f2v mine = tid < used ? ml[piece(tid)] : f2v{-INFINITY, 0.0f};
     float M = mine[0];
@@ -853,13 +856,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     }
 }
 
-// Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims).
+// Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims; three of
+// the int8 kernel up to 64: 69 sequences of up to 39768, 2 heads of 64, 59 -> 55 us).
 // Up to PG_ALONE positions each workgroup takes a sequence whole: the second launch would cost more
 // than it gives (8 sequences of 640: 9.1 us against 12.5).
-constexpr int PG_GROUPS = 512, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
+constexpr int PG_GROUPS = 512, PG_GROUPS_I8_64 = 768, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
 // bytes of the table of pieces, and the slots of a call (two to a workgroup)
 int64_t pieces_bytes(int64_t units) { return (units * (int64_t)sizeof(int2) + 15) / 16 * 16; }
-int paged_groups(int64_t hd) { return hd <= 128 ? PG_GROUPS : PG_GROUPS_WIDE; }
+int paged_groups(int64_t hd, bool i8) {
+    return hd <= 64 && i8 ? PG_GROUPS_I8_64 : hd <= 128 ? PG_GROUPS : PG_GROUPS_WIDE;
+}
 
 }  // namespace
 }  // namespace lq
@@ -916,7 +922,7 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length) {
     if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || max_length <= PG_ALONE) return 0;
     return (size_t)pieces_bytes(B * Hkv * ((H / Hkv + 15) / 16)) +
-           (size_t)2 * paged_groups(hd) * 16 * (hd + 2) * sizeof(float);
+           (size_t)2 * paged_groups(hd, true) * 16 * (hd + 2) * sizeof(float);  // of either kind of cache
 }
 
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
@@ -944,7 +950,8 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
     LQ_REQUIRE(alone || (d_workspace && aligned16(d_workspace) &&
                          workspace_bytes >= lq_paged_attention_workspace_size(B, H, Hkv, hd, max_length)),
                "lq_paged_attention: workspace too small or not 16-byte aligned");
-    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16, groups = alone ? 0 : paged_groups(hd);
+    const int group = (int)(H / Hkv), qtiles = (group + 15) / 16;
+    const int groups = alone ? 0 : paged_groups(hd, cache_type == LQ_I8);
     const int64_t units = B * Hkv * qtiles;
     LQ_REQUIRE(units <= 0x7fffffff, "lq_paged_attention: too many workgroups");
     char* ws = static_cast<char*>(d_workspace);
@@ -955,9 +962,10 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
                       alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
     const dim3 grid((unsigned)(alone ? units : groups));
     const hipStream_t st = as_stream(stream);
-    // a few short sequences: four waves each, to hide more of the latency; else two, two workgroups to a CU
+    // A few short sequences: as many waves each as the LDS holds tiles for, to hide more of the latency (8 sequences
+    // of up to 640, 8 heads of 64: 9.9 us with four waves, 8.8 with eight); else two, two workgroups to a CU.
     const bool few = alone && units <= 256;
-    note_path(!alone ? "paged shared" : few ? "paged whole 4 waves" : "paged whole");
+    note_path(!alone ? "paged shared" : few ? "paged whole few" : "paged whole");
     with_half(q_type, [&](auto q) {
         using Q = decltype(q);
         auto i8 = [&](auto w, auto exact) {
@@ -971,6 +979,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
         };
         const std::integral_constant<int, 2> two{};
         const std::integral_constant<int, 4> four{};
+        const std::integral_constant<int, 8> eight{};
         const std::integral_constant<int, 64> w64{};
         const std::integral_constant<int, 128> w128{};
         const std::integral_constant<int, 192> w192{};
@@ -983,7 +992,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
             else if (hd <= 192) i8(w192, std::false_type{});
             else i8(w256, std::false_type{});
         } else if (hd <= 64) {
-            if (few) hd == 64 ? copy(w64, four, four, std::true_type{}) : copy(w64, four, four, std::false_type{});
+            if (few) hd == 64 ? copy(w64, eight, two, std::true_type{}) : copy(w64, eight, two, std::false_type{});
             else hd == 64 ? copy(w64, two, four, std::true_type{}) : copy(w64, two, four, std::false_type{});
         } else if (hd <= 128) {
             if (few) hd == 128 ? copy(w128, four, two, std::true_type{}) : copy(w128, four, two, std::false_type{});

@@ -356,7 +356,7 @@ def test_paged_attention_paths(gpu):
 
     for hd in (64, 128):
         _paged(np.random.default_rng(1), [40, 1000], 2, 1, hd, 16, "float16", "float16", "float16")
-        assert _C.last_path() == "paged whole 4 waves"
+        assert _C.last_path() == "paged whole few"
         _paged(np.random.default_rng(2), [int(n) for n in np.random.default_rng(2).integers(0, 90, 140)], 4, 2, hd, 16,
                "bfloat16", "bfloat16", "bfloat16")
         assert _C.last_path() == "paged whole"

@@ -54,9 +54,11 @@ __device__ __forceinline__ v4i operand_rsrc(const void* base, int64_t rows, int6
 
 // 16 bytes per lane from rsrc + voff + soff into LDS at lds_addr + 16 * lane.  The LDS
 // destination travels in M0 as an input operand ("{m0}"): the compiler writes M0 itself and
-// knows the instruction reads it, so M0 is never changed behind its back.
+// knows the instruction reads it, so M0 is never changed behind its back.  A load into LDS must
+// not follow a scalar write of M0 at once: the compiler keeps that one wait state for loads of its
+// own but does not see the load in the asm, which therefore begins with it (here and below).
 __device__ __forceinline__ void lds_dma16(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds_addr) {
-    asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds"
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds_addr)
                  : "memory");
@@ -64,7 +66,7 @@ __device__ __forceinline__ void lds_dma16(v4i rsrc, uint32_t voff, uint32_t soff
 
 // The same where the descriptor is made right before (v_readfirstlane): a load must not read a scalar
 // register within five wait states of a vector instruction's write to it, and the compiler, which
-// keeps that distance for loads of its own, does not see the load in the asm.
+// keeps that distance for loads of its own, does not see the load in the asm.  The wait covers M0 too.
 __device__ __forceinline__ void lds_dma16_fresh(v4i rsrc, uint32_t voff, uint32_t lds_addr) {
     asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :
@@ -76,7 +78,7 @@ __device__ __forceinline__ void lds_dma16_fresh(v4i rsrc, uint32_t voff, uint32_
 // nothing), past the caches: for what is read once.  No bounds check: every active lane's address must
 // be valid.
 __device__ __forceinline__ void lds_copy16(const void* src, uint32_t lds_addr) {
-    asm volatile("global_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
 }
 
 }  // namespace lq

@@ -87,15 +87,22 @@ _held: list | None = None  # every buffer allocated while a capture records (luc
 
 
 class _DeviceBuffer:
-    """An ``lq_malloc`` allocation, returned to the cache when collected."""
+    """An ``lq_malloc`` allocation, returned to the cache when collected.  With ``stream`` it may be
+    written on that stream at once (``lq_malloc_async``), and after its free it is not handed out
+    before the stream's work is done (``lq_record_stream``)."""
 
     __slots__ = ("ptr", "nbytes", "__weakref__")
 
-    def __init__(self, nbytes: int) -> None:
+    def __init__(self, nbytes: int, stream: Any = None) -> None:
         p = ctypes.c_void_p()
-        _C.check(_C.lib().lq_malloc(ctypes.byref(p), max(int(nbytes), 1)), "lq_malloc")
+        if stream is None:
+            _C.check(_C.lib().lq_malloc(ctypes.byref(p), max(int(nbytes), 1)), "lq_malloc")
+        else:
+            _C.check(_C.lib().lq_malloc_async(ctypes.byref(p), max(int(nbytes), 1), stream), "lq_malloc_async")
         self.ptr = p.value
         self.nbytes = int(nbytes)
+        if stream is not None:
+            _C.check(_C.lib().lq_record_stream(self.ptr, stream), "lq_record_stream")
         if _held is not None:
             _held.append(self)
 
@@ -149,7 +156,7 @@ class Tensor:
         return t
 
     @classmethod
-    def _empty(cls, shape: Sequence[int], dt: np.dtype, device: str) -> "Tensor":
+    def _empty(cls, shape: Sequence[int], dt: np.dtype, device: str, stream: Any = None) -> "Tensor":
         t = cls()
         t._shape = tuple(int(s) for s in shape)
         t._dtype = np.dtype(dt)
@@ -158,7 +165,7 @@ class Tensor:
             t._device = "cpu"
         else:
             t._device = "gpu"
-            t._buf = _DeviceBuffer(t.nbytes)
+            t._buf = _DeviceBuffer(t.nbytes, stream)
         return t
 
     @classmethod
@@ -410,10 +417,12 @@ def from_numpy(arr: np.ndarray, device: Any = "cpu") -> Tensor:
     return Tensor._from_numpy(arr, normalize_device(device))
 
 
-def empty(shape: Sequence[int] | int, dtype: Any = float32, device: Any = "cpu") -> Tensor:
+def empty(shape: Sequence[int] | int, dtype: Any = float32, device: Any = "cpu", stream: Any = None) -> Tensor:
+    """An uninitialised tensor; with ``stream`` (of ``lq_stream_create``) its device memory is for work
+    queued on that stream from now on."""
     if isinstance(shape, int):
         shape = (shape,)
-    return Tensor._empty(shape, np.dtype(dtype), normalize_device(device))
+    return Tensor._empty(shape, np.dtype(dtype), normalize_device(device), stream)
 
 
 def full(shape: Sequence[int] | int, value: float, dtype: Any = float32, device: Any = "cpu") -> Tensor:

@@ -5,8 +5,11 @@ The functions are part of ``lucid_amd.nn.functional``; :class:`PagedKVCache` kee
 page table and the lengths of one layer's cache, :class:`PageTable` shares a table between the
 layers of a model.  No counterpart in the reference, whose decode attends a dense cache
 (lucid/nn/functional/attention.py, ``scaled_dot_product_attention``).  Everything runs on the
-default stream (``stream=None``) or on a stream of ``lq_stream_create``; a tensor used on another
-stream than it is freed on is marked with ``Tensor.record_stream`` by the caller.
+default stream (``stream=None``) or on a stream of ``lq_stream_create``.  Results and workspace are
+allocated for the stream of the call; that the operands are ready there is the caller's to order,
+and an operand that may be dropped before that stream's work is done is marked with
+``Tensor.record_stream`` by the caller.  A call is captured into a graph through
+``lucid_amd.graphs.CapturedForward``, which keeps what the call allocates.
 """
 
 from __future__ import annotations
@@ -74,15 +77,27 @@ def _pages(op, k_pages, v_pages, k_scale, v_scale, table, lengths):
     return tuple(int(n) for n in k_pages.shape)
 
 
+def _stream(stream, *operands):
+    """``stream``, the default one as None.  An operand behind codes gets its values on the default
+    stream; another stream's work waits for them."""
+    if not getattr(stream, "value", stream):
+        return None
+    behind = [t for t in operands if t is not None and t.is_code_backed and t._buf is None]
+    for t in behind:
+        t.data_ptr()
+    if behind:
+        _C.call("lq_stream_synchronize", None)
+    return stream
+
+
 def _scratch(nbytes: int, stream):
     """(address, holder) of workspace for one call: the thread's own on the default stream; on
-    another stream memory of its own, which is reused only after that stream's work."""
+    another stream memory of its own, allocated for that stream."""
     if nbytes == 0:
         return None, None
     if stream is None:
         return workspace.get(nbytes), None
-    t = empty((nbytes,), np.uint8, "gpu")
-    t.record_stream(stream)
+    t = empty((nbytes,), np.uint8, "gpu", stream)
     return t.data_ptr(), t
 
 
@@ -107,6 +122,7 @@ def paged_kv_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, tabl
         _ints(starts, op, "starts", seqs + 1)
     elif tokens != seqs:
         raise ValueError(f"{op}: {tokens} tokens for {seqs} sequences need starts")
+    stream = _stream(stream, k, v, k_scale, v_scale)
     _C.call("lq_paged_kv_append", k.data_ptr(), v.data_ptr(), FLOAT_TYPE_CODE[dt], hkv * hd, tokens, _opt(starts), seqs,
             hkv, hd, table.data_ptr(), table.shape[1], lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             _CACHE_TYPE[k_pages.dtype], _opt(k_scale), _opt(v_scale), pages, page, stream)
@@ -127,6 +143,7 @@ def paged_kv_append_qkv(qkv: Tensor, heads: int, k_pages: Tensor, v_pages: Tenso
         _ints(starts, op, "starts", seqs + 1)
     elif tokens != seqs:
         raise ValueError(f"{op}: {tokens} tokens for {seqs} sequences need starts")
+    stream = _stream(stream, qkv, k_scale, v_scale)
     k = qkv.data_ptr() + heads * hd * dt.itemsize
     _C.call("lq_paged_kv_append", k, k + hkv * hd * dt.itemsize, FLOAT_TYPE_CODE[dt], (heads + 2 * hkv) * hd, tokens,
             _opt(starts), seqs, hkv, hd, table.data_ptr(), table.shape[1], lengths.data_ptr(), k_pages.data_ptr(),
@@ -164,7 +181,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
         raise ValueError(f"{op}: q {tuple(q.shape)} does not fit {table.shape[0]} sequences, {hkv} key heads of {hd}")
     if k_pages.dtype not in (dt, np.dtype(np.int8)):
         raise TypeError(f"{op}: a cache of {k_pages.dtype} for queries of {dt}")
-    out = empty((B, h, hd), _out_type(out_dtype, dt, op), "gpu")
+    stream = _stream(stream, k_scale, v_scale)
+    out = empty((B, h, hd), _out_type(out_dtype, dt, op), "gpu", stream)
     size = _C.lib().lq_paged_attention_workspace_size(B, h, hkv, hd, max_length)
     ws, _held = _scratch(size, stream)
     _C.call("lq_paged_attention", q.data_ptr(), FLOAT_TYPE_CODE[dt], ldq, B, h, hkv, hd, k_pages.data_ptr(),
@@ -212,7 +230,8 @@ def _prompt(op, q, ldq, k, ldk, v, ldv, dt, q_starts, k_starts, total_q, total_k
     k_starts = q_starts if k_starts is None else _ints(k_starts, op, "k_starts", q_starts.shape[0])
     if q_starts.shape[0] < 1:
         raise ValueError(f"{op}: starts hold one number more than there are sequences")
-    out = empty((total_q, h, hd), _out_type(out_dtype, dt, op), "gpu")
+    stream = _stream(stream)
+    out = empty((total_q, h, hd), _out_type(out_dtype, dt, op), "gpu", stream)
     _C.call("lq_prompt_attention", q, ldq, k, ldk, v, ldv, FLOAT_TYPE_CODE[dt], q_starts.data_ptr(), k_starts.data_ptr(),
             int(q_starts.shape[0]) - 1, total_q, total_k, h, hkv, hd, 1 if causal else 0, _scale(scale, hd, op),
             out.data_ptr(), FLOAT_TYPE_CODE[out.dtype], stream)
@@ -228,8 +247,9 @@ def token_logprobs(logits: Tensor, targets: Tensor, top: int = 0, stream=None):
     _ints(targets, op, "targets", rows)
     if not 0 <= top <= min(vocab, 64):
         raise ValueError(f"{op}: top must be within [0, {min(vocab, 64)}], got {top}")
-    lp, ent, lse = (empty((rows,), float32, "gpu") for _ in range(3))
-    top_lp, top_ids = empty((rows, top), float32, "gpu"), empty((rows, top), np.int32, "gpu")
+    stream = _stream(stream, logits)
+    lp, ent, lse = (empty((rows,), float32, "gpu", stream) for _ in range(3))
+    top_lp, top_ids = empty((rows, top), float32, "gpu", stream), empty((rows, top), np.int32, "gpu", stream)
     size = _C.lib().lq_token_logprobs_workspace_size(rows, vocab, top)
     ws, _held = _scratch(size, stream)
     _C.call("lq_token_logprobs", logits.data_ptr(), FLOAT_TYPE_CODE[dt], vocab, rows, vocab, targets.data_ptr(), top,
@@ -254,7 +274,8 @@ def token_logprobs_backward(logits: Tensor, targets: Tensor, lse: Tensor, g_logp
             _need(t, op, name, 1, (float32,))
             if t.shape[0] != rows:
                 raise ValueError(f"{op}: {name} must hold {rows} numbers, got {t.shape[0]}")
-    grad = empty((rows, vocab), dt, "gpu")
+    stream = _stream(stream, logits, lse, g_logprobs, entropy, g_entropy)
+    grad = empty((rows, vocab), dt, "gpu", stream)
     _C.call("lq_token_logprobs_backward", logits.data_ptr(), FLOAT_TYPE_CODE[dt], vocab, rows, vocab,
             targets.data_ptr(), lse.data_ptr(), _opt(entropy) if g_entropy is not None else None,
             g_logprobs.data_ptr(), _opt(g_entropy), grad.data_ptr(), vocab, stream)

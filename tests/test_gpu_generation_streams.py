@@ -1,0 +1,64 @@
+"""Serving ops on a stream of their own, with work pending elsewhere."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+N = 4096
+
+
+def _dev(a):
+    import lucid_amd as L
+
+    return L.tensor(np.ascontiguousarray(a), device="gpu")
+
+
+def _i32(a):
+    return _dev(np.asarray(a, np.int32))
+
+
+@pytest.fixture
+def stream(gpu):
+    from lucid_amd import _C
+
+    st = ctypes.c_void_p()
+    _C.call("lq_stream_create", ctypes.byref(st))
+    yield st
+    _C.call("lq_stream_synchronize", st)
+    _C.call("lq_stream_destroy", st)
+
+
+def test_a_result_on_a_stream_leaves_the_default_streams_pending_reads_alone(gpu, stream):
+    """x is dropped with products that read it still queued on the default stream; a result of x's size
+    made on another stream at that moment is not put where x was."""
+    from lucid_amd import _C
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(0)
+    a, b = (rng.integers(-127, 128, (N, N)).astype(np.int8) for _ in range(2))
+    tokens, h, hd = 1024, 64, 128  # fp16 rows of x's size
+    assert tokens * h * hd * 2 == a.nbytes
+    q, k = (_dev(rng.standard_normal((tokens, n, hd)).astype(np.float16)) for n in (h, 1))
+    starts = _i32([0, 5, tokens])
+    want = F.prompt_attention(q, k, k, starts).numpy()
+    gpu.synchronize()
+    _C.call("lq_empty_cache")
+    B, out = _dev(b), gpu.empty((N, N), np.int32, "gpu")
+    x = _dev(a)
+    gpu.synchronize()
+    at = x.data_ptr()
+    for _ in range(100):
+        _C.call("lq_gemm_w8a8", x.data_ptr(), N, B.data_ptr(), N, out.data_ptr(), N, N, N, N, None, 0, None, 0, None,
+                None, None, None, None, None, 0, 0, _C.OUT_I32, 0, None, 0, None)
+    del x
+    y = F.prompt_attention(q, k, k, starts, stream=stream)
+    assert y.data_ptr() != at
+    _C.call("lq_stream_synchronize", stream)
+    np.testing.assert_array_equal(y.numpy(), want)
+    rows = rng.choice(N, 16, replace=False)
+    np.testing.assert_array_equal(out.numpy()[rows], a[rows].astype(np.int64) @ b.astype(np.int64).T)

@@ -289,7 +289,11 @@ class PageTable:
     """Which pages each of ``seqs`` sequences holds, shared by the caches of a model's layers.
 
     ``table`` [seqs, per_seq] and ``lengths`` [seqs] are device int32 tensors that keep their
-    address, so captured graphs read the current state; the host keeps the free pages."""
+    address, so captured graphs read the current state; the host keeps the free pages.
+
+    Everything that reads or writes the caches of a table runs on one stream, and ``grow`` and
+    ``release`` are given that stream: they change the table and the lengths in place behind what is
+    queued there, and a released page's next owner writes it behind the last reader."""
 
     def __init__(self, seqs: int, pages: int, page: int = 64, max_length: int | None = None) -> None:
         if seqs < 1 or pages < 1 or page < 1:
@@ -311,14 +315,17 @@ class PageTable:
     def host_lengths(self) -> np.ndarray:
         return self._lengths.copy()
 
-    def rows(self, seqs) -> tuple[Tensor, Tensor]:
-        """Copies of some sequences' table rows and lengths."""
-        return (tensor(np.ascontiguousarray(self._table[seqs]), device="gpu"),
-                tensor(np.ascontiguousarray(self._lengths[seqs]), device="gpu"))
+    def rows(self, seqs, stream=None) -> tuple[Tensor, Tensor]:
+        """Copies of some sequences' table rows and lengths, for work on ``stream``."""
+        stream, copies = _stream(stream), []
+        for a in (np.ascontiguousarray(self._table[seqs]), np.ascontiguousarray(self._lengths[seqs])):
+            copies.append(empty(a.shape, a.dtype, "gpu", stream))
+            _C.call("lq_memcpy_h2d", copies[-1].data_ptr(), a.ctypes.data, a.nbytes, stream)
+        return copies[0], copies[1]
 
-    def grow(self, counts) -> None:
+    def grow(self, counts, stream=None) -> None:
         """``counts[s]`` more positions for every sequence: takes pages as needed and uploads the
-        table and the lengths.  Nothing changes when the free pages do not suffice."""
+        table and the lengths, on ``stream``.  Nothing changes when the free pages do not suffice."""
         counts = np.asarray(counts, np.int64)
         if counts.shape != (self.seqs,) or (counts < 0).any():
             raise ValueError(f"PageTable.grow: {self.seqs} counts of 0 or more expected")
@@ -335,24 +342,25 @@ class PageTable:
                 self._table[s, self._held[s]] = self._free.pop()
                 self._held[s] += 1
         self._lengths = new.astype(np.int32)
-        self._upload(more > 0)
+        self._upload(more > 0, stream)
 
-    def release(self, s: int) -> None:
-        """Sequence ``s`` ends: its pages are free again and its length is 0."""
+    def release(self, s: int, stream=None) -> None:
+        """Sequence ``s`` ends: its pages are free again and its length is 0, on ``stream``."""
         self._free.extend(int(p) for p in self._table[s, :self._held[s]][::-1])
         self._held[s] = 0
         self._lengths[s] = 0
-        self._upload(False)
+        self._upload(False, stream)
 
-    def _upload(self, table: bool) -> None:
+    def _upload(self, table: bool, stream) -> None:
+        stream = _stream(stream)
         if table:
-            _C.call("lq_memcpy_h2d", self.table.data_ptr(), self._table.ctypes.data, self._table.nbytes, None)
-        _C.call("lq_memcpy_h2d", self.lengths.data_ptr(), self._lengths.ctypes.data, self._lengths.nbytes, None)
+            _C.call("lq_memcpy_h2d", self.table.data_ptr(), self._table.ctypes.data, self._table.nbytes, stream)
+        _C.call("lq_memcpy_h2d", self.lengths.data_ptr(), self._lengths.ctypes.data, self._lengths.nbytes, stream)
 
 
 class PagedKVCache:
     """One layer's pages over a :class:`PageTable`: ``append`` what the projection made, then
-    ``attend`` with the step's queries.  ``dtype`` float16, bfloat16 or int8 (codes with one
+    ``attend`` with the step's queries, on the stream that the table is grown on.  ``dtype`` float16, bfloat16 or int8 (codes with one
     scale per row)."""
 
     def __init__(self, table: PageTable, kv_heads: int, head_dim: int, dtype=float16) -> None:

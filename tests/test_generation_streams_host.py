@@ -131,3 +131,19 @@ def test_values_behind_codes_are_there_before_another_stream_reads_them(lib):
     at = names.index("lq_dequantize_per_tensor")
     assert lib.calls[at + 1] == ("lq_stream_synchronize", (None,))
     assert "lq_token_logprobs" in names[at + 2:]
+
+
+def test_the_table_changes_on_the_stream_that_reads_it(lib):
+    """grow and release change the device's table and lengths behind the kernels that are queued there."""
+    pt = G.PageTable(3, 8, 4)
+    lib.calls.clear()
+    for stream in (S, None):
+        pt.grow([5, 0, 1], stream)
+        pt.release(0, stream)
+        uploads = [args for name, args in lib.calls if name == "lq_memcpy_h2d"]
+        assert [args[0] for args in uploads] == [t.data_ptr() for t in (pt.table, pt.lengths, pt.lengths)]
+        assert all(args[-1] is stream for args in uploads)
+        lib.calls.clear()
+    for t in pt.rows([2, 1], S):
+        assert S.value in lib.live[t.data_ptr()][1]
+    assert len(lib.calls) == 2 and all(args[-1] is S for _, args in lib.calls)

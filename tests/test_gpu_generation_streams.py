@@ -62,3 +62,43 @@ def test_a_result_on_a_stream_leaves_the_default_streams_pending_reads_alone(gpu
     np.testing.assert_array_equal(y.numpy(), want)
     rows = rng.choice(N, 16, replace=False)
     np.testing.assert_array_equal(out.numpy()[rows], a[rows].astype(np.int64) @ b.astype(np.int64).T)
+
+
+@pytest.mark.parametrize("longest", [900, 3000])
+def test_the_table_grows_behind_queued_attention(gpu, stream, longest):
+    """Steps queued one after the other without waiting: append, attend, grow, append, attend.  Every step's
+    attention is that of the lengths it was queued with."""
+    from lucid_amd import _C
+    from lucid_amd.nn.generation import PagedKVCache, PageTable
+
+    rng = np.random.default_rng(longest)
+    B, h, hkv, hd, steps = 24, 4, 2, 64, 6
+    first = [longest] + [int(n) for n in rng.integers(1, longest, B - 1)]
+    bound = longest + steps
+    kv = [[_dev(rng.standard_normal((sum(n), hkv, hd)).astype(np.float16)) for _ in range(2)]
+          for n in [first] + [[1] * B] * steps]
+    q = [_dev(rng.standard_normal((B, h, hd)).astype(np.float16)) for _ in range(steps)]
+    starts = _i32(np.concatenate([[0], np.cumsum(first)]))
+    one = _i32(np.arange(B + 1))
+
+    def serve(st, wait):
+        pt = PageTable(B, B * (bound // 16 + 1), 16)
+        cache = PagedKVCache(pt, hkv, hd)
+        _C.synchronize()
+        pt.grow(first, st)
+        cache.append(*kv[0], starts, stream=st)
+        outs = []
+        for i in range(steps):
+            pt.grow([1] * B, st)
+            cache.append(*kv[i + 1], one, stream=st)
+            outs.append(cache.attend(q[i], max_length=bound, stream=st))
+            if wait:
+                _C.synchronize()
+        pt.release(0, st)
+        pt.grow([40] + [0] * (B - 1), st)  # the released pages' next owner
+        cache.append(*kv[0], _i32([0, 40] + [40] * (B - 1)), stream=st)
+        _C.synchronize()
+        return [o.numpy() for o in outs]
+
+    for got, want in zip(serve(stream, False), serve(None, True)):
+        np.testing.assert_array_equal(got, want)

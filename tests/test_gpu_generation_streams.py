@@ -102,3 +102,83 @@ def test_the_table_grows_behind_queued_attention(gpu, stream, longest):
 
     for got, want in zip(serve(stream, False), serve(None, True)):
         np.testing.assert_array_equal(got, want)
+
+
+def test_calls_of_two_launches_on_a_stream_of_their_own(gpu, stream):
+    """Long sequences and long rows: the workspace is the call's own there, and the bits are the default
+    stream's, with eager calls of other sizes between."""
+    from lucid_amd import _C
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(4)
+    lens = [5000, 1, 0, 2300]
+    pages = 470
+    table = np.zeros((4, 320), np.int32)
+    ids, at = rng.permutation(pages), 0
+    for b, n in enumerate(lens):
+        table[b, :-(-n // 16)] = ids[at:at + -(-n // 16)]
+        at += -(-n // 16)
+    k, v = (_dev(rng.standard_normal((pages, 2, 16, 64)).astype(np.float16)) for _ in range(2))
+    codes = _dev(rng.integers(-127, 128, (pages, 2, 16, 64)).astype(np.int8))
+    scale = _dev((rng.random((pages, 2, 16)) / 100 + 1e-3).astype(np.float32))
+    q, dt, dl = _dev(rng.standard_normal((4, 8, 64)).astype(np.float16)), _i32(table), _i32(lens)
+    x = _dev((rng.standard_normal((5, 150001)) * 3).astype(np.float32))
+    t = _i32([3, -100, 7, 150000, 0])
+    _C.synchronize()
+
+    def ops(s):
+        out = [F.paged_attention(q, k, v, dt, dl, 5000, stream=s)]
+        assert _C.last_path() == "paged shared"
+        out.append(F.paged_attention(q, codes, codes, dt, dl, 5000, k_scale=scale, v_scale=scale, stream=s))
+        assert _C.last_path() == "paged shared"
+        out += F.token_logprobs(x, t, 7, stream=s)
+        assert _C.last_path() == "logprobs parts"
+        return out
+
+    want = [y.numpy() for y in ops(None)]
+    queued = []
+    for _ in range(3):
+        queued.append(ops(stream))
+        F.token_logprobs(x, t, 64)  # the thread's own workspace, meanwhile
+    _C.call("lq_stream_synchronize", stream)
+    for got in queued:
+        for y, z in zip(got, want):
+            np.testing.assert_array_equal(y.numpy(), z)
+
+
+def test_calls_of_two_launches_replayed_from_a_graph(gpu):
+    """Recorded once, replayed after the lengths, the table and the logits changed, with eager calls that use
+    the thread's own workspace and synchronizations between."""
+    import lucid_amd as L
+    from lucid_amd import _C
+    import lucid_amd.nn.functional as F
+    from lucid_amd.graphs import CapturedForward
+
+    rng = np.random.default_rng(5)
+    pages = 700
+    k, v = (_dev(rng.standard_normal((pages, 1, 16, 128)).astype(np.float16)) for _ in range(2))
+    t = _i32([3, -100, 7])
+    paths = []
+
+    def fn(q, table, lens, x):
+        a = F.paged_attention(q, k, v, table, lens, 4000, out_dtype=L.float32)
+        paths.append(_C.last_path())
+        b = F.token_logprobs(x, t, 6)
+        paths.append(_C.last_path())
+        return (a, *b)
+
+    def make():
+        lens = np.array([4000, *rng.integers(0, 4000, 1), rng.integers(1, 40)], np.int32)
+        return (rng.standard_normal((3, 4, 128)).astype(np.float16), rng.integers(0, pages, (3, 250)).astype(np.int32),
+                rng.permutation(lens), (rng.standard_normal((3, 90001)) * 3).astype(np.float32))
+
+    cap = CapturedForward(fn, *(_dev(a) for a in make()))
+    assert set(paths[::2]) == {"paged shared"} and set(paths[1::2]) == {"logprobs parts"}
+    for _ in range(6):
+        arrays = make()
+        cap.load(*arrays)
+        got = [y.numpy() for y in cap()]
+        want = [y.numpy() for y in fn(*(_dev(a) for a in arrays))]
+        L.synchronize()
+        for y, z in zip(got, want):
+            np.testing.assert_array_equal(y, z)

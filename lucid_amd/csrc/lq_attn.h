@@ -3,6 +3,7 @@
 #pragma once
 
 #include "lq_internal.h"
+#include "lq_place.h"
 
 namespace lq {
 
@@ -40,6 +41,13 @@ struct ElemI8 {
     static constexpr int code = LQ_I8;
     static __device__ __forceinline__ float load(T v) { return (float)v; }
 };
+
+// The grid of n workgroups, and a workgroup's place in it (past the end in the last row's rest).
+inline dim3 grid_of(int64_t n) {
+    const Workgroups w = workgroups(n);
+    return dim3(w.x, w.y);
+}
+__device__ __forceinline__ int64_t workgroup() { return workgroup_index(blockIdx.x, blockIdx.y); }
 
 inline bool is_float_type(int t) { return t == LQ_F32 || t == LQ_F16 || t == LQ_BF16; }
 inline bool is_half_type(int t) { return t == LQ_F16 || t == LQ_BF16; }

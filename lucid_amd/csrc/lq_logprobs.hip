@@ -157,8 +157,10 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
     __shared__ int who[NT];
     __shared__ uint64_t cand[LP_CAND];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x / (uint32_t)a.parts;
-    const int part = blockIdx.x - (uint32_t)r * (uint32_t)a.parts;
+    const uint32_t id = (uint32_t)workgroup();
+    const int64_t r = id / (uint32_t)a.parts;
+    if (r >= a.rows) return;
+    const int part = id - (uint32_t)r * (uint32_t)a.parts;
     // this workgroup's columns: whole chunks but for the last part's end
     const int64_t width = (a.vocab + (int64_t)a.parts * N - 1) / ((int64_t)a.parts * N) * N, c0 = part * width;
     const Split<E> row(static_cast<const typename E::T*>(a.x) + r * a.ldx + c0, min(width, a.vocab - c0));
@@ -242,11 +244,11 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
     }
     float lse = 0.0f;
     if (a.parts == 1) lse = row_results<E>(a, r, R, s, ed, tid == 0);
-    else if (tid == 0) a.sums[blockIdx.x] = PartSums{R, s, ed, 0.0f};
+    else if (tid == 0) a.sums[id] = PartSums{R, s, ed, 0.0f};
     if (a.top == 0) return;
 
     auto put = [&](int at, uint64_t key) {
-        if (a.parts > 1) a.keys[(int64_t)blockIdx.x * a.top + at] = key - (uint64_t)c0;  // the row's own index
+        if (a.parts > 1) a.keys[(int64_t)id * a.top + at] = key - (uint64_t)c0;  // the row's own index
         else row_choice<E>(a, r, at, (int)rank_index(key), lse);
     };
     if (s == s) {  // uniform: no NaN, no +inf in the row
@@ -448,7 +450,8 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogprobGradArgs a) {
 // Any alignment, element by element.
 template <class E>
 __global__ __launch_bounds__(256) void logprobs_grad_any_kernel(LogprobGradArgs a) {
-    const int64_t r = blockIdx.x;
+    const int64_t r = workgroup();
+    if (r >= a.rows) return;
     const typename E::T* x = static_cast<const typename E::T*>(a.x) + r * a.ldx;
     typename E::T* y = static_cast<typename E::T*>(a.grad) + r * a.ldg;
     const GradRow gr(a, r);
@@ -489,7 +492,7 @@ int lq_token_logprobs(const void* d_x, int type, int64_t ldx, int64_t rows, int6
     note_path(parts > 1 ? "logprobs parts" : "logprobs rows");
     with_float(type, [&](auto e) {
         using E = decltype(e);
-        const dim3 grid((unsigned)(rows * parts));
+        const dim3 grid = grid_of(rows * parts);
         const hipStream_t st = as_stream(stream);
         const int64_t chunks = vocab * (int64_t)sizeof(typename E::T) / 16;
         if (chunks <= 256) hipLaunchKernelGGL((logprobs_kernel<64, E>), grid, dim3(64), 0, st, a);
@@ -523,7 +526,7 @@ int lq_token_logprobs_backward(const void* d_x, int type, int64_t ldx, int64_t r
                             (unsigned)(rows < 65535 ? rows : 65535), (unsigned)((rows + 65534) / 65535));
             hipLaunchKernelGGL((logprobs_grad_kernel<E>), grid, dim3(256), 0, st, a);
         } else {
-            hipLaunchKernelGGL((logprobs_grad_any_kernel<E>), dim3((unsigned)rows), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((logprobs_grad_any_kernel<E>), grid_of(rows), dim3(256), 0, st, a);
         }
     });
     return launch_status("lq_token_logprobs_backward");

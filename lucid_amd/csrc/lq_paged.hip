@@ -43,7 +43,8 @@ __device__ __forceinline__ int64_t token_row(const AppendArgs& a, int64_t t) {
 template <class Src, class Dst>
 __global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
     const int64_t per = a.Hkv * a.hd;
-    const int64_t t = blockIdx.x;
+    const int64_t t = workgroup();
+    if (t >= a.tokens) return;
     const int64_t row = token_row(a, t);
     if (row < 0) return;
     for (int64_t e = threadIdx.x; e < 2 * per; e += blockDim.x) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ void load8(const typename Src::T* p, float (&x)[8]) {
 template <int TOK, class Src, class Dst>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     __shared__ int64_t rows[TOK];
-    const int64_t t0 = (int64_t)blockIdx.x * TOK;
+    const int64_t t0 = workgroup() * TOK;
     if (threadIdx.x < TOK) rows[threadIdx.x] = t0 + threadIdx.x < a.tokens ? token_row(a, t0 + threadIdx.x) : -1;
     __syncthreads();
     const uint32_t hd8 = (uint32_t)a.hd >> 3, per = (uint32_t)a.Hkv * hd8;
@@ -130,11 +131,12 @@ __device__ __forceinline__ int32_t magnitude(float x) { return __builtin_bit_cas
 // One wave per (token, head, k or v), element by element.
 template <class Src>
 __global__ __launch_bounds__(64) void append_i8_any_kernel(AppendArgs a) {
-    const int64_t t = blockIdx.x;
+    const int64_t n = workgroup(), t = n / (2 * a.Hkv);
+    if (t >= a.tokens) return;
     const int64_t row = token_row(a, t);
     if (row < 0) return;
-    const int h = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
+    const int64_t h = (n - t * 2 * a.Hkv) >> 1;
+    const bool is_v = n & 1;
     const typename Src::T* src = static_cast<const typename Src::T*>(is_v ? a.v : a.k) + t * a.ld + h * a.hd;
     const int64_t r = row + h * a.page;
     int32_t top = 0;
@@ -148,7 +150,8 @@ __global__ __launch_bounds__(64) void append_i8_any_kernel(AppendArgs a) {
 // LPR lanes per row of hd <= 8 LPR values, eight values a lane; one workgroup per token.
 template <int LPR, class Src>
 __global__ __launch_bounds__(256) void append_i8_kernel(AppendArgs a) {
-    const int64_t t = blockIdx.x;
+    const int64_t t = workgroup();
+    if (t >= a.tokens) return;
     const int64_t row = token_row(a, t);
     if (row < 0) return;
     const uint32_t d = (threadIdx.x % LPR) * 8;
@@ -252,17 +255,18 @@ struct Line {
         steps = (len + STEP - 1) / STEP;
         cost = unit ? (steps + unit - 1) / unit * unit : steps ? steps + START : 0;
     }
-    // Finds the part of workgroup blockIdx.x; `scan` holds NT numbers.
+    // Finds the part of this workgroup; `scan` holds NT numbers.
     __device__ __forceinline__ void init(const PagedArgs& a, int64_t* scan) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         heads = a.Hkv * a.qtiles;
         unit = 0;
         if (a.groups == 0) {
             lead = START;
-            const int i = blockIdx.x / heads;
-            sequence(a, i);
-            base = 0;
-            start = at = (int64_t)(blockIdx.x - i * heads) * cost;
+            const uint32_t n = (uint32_t)workgroup(), i = n / (uint32_t)heads;
+            start = at = stop = base = 0;
+            if (i >= (uint32_t)a.B) return;
+            sequence(a, (int)i);
+            start = at = (int64_t)(n - i * heads) * cost;
             stop = at + cost;
             return;
         }
@@ -361,13 +365,13 @@ struct Line {
 template <int WAVES, class Q>
 __device__ __forceinline__ void paged_empty(const PagedArgs& a) {
     const int64_t row = (int64_t)a.H * a.hd;
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    for (int64_t b = workgroup(); b < a.B; b += (int64_t)gridDim.x * gridDim.y) {
         bool over;
-        if (sequence_length(a, b, over) > 0) continue;
+        if (sequence_length(a, (int)b, over) > 0) continue;
         const float y = over ? __builtin_nanf("") : 0.0f;
         const int heads = a.Hkv * a.qtiles;
         if (a.groups)
-            for (int e = threadIdx.x; e < heads; e += 64 * WAVES) a.pieces[(int64_t)b * heads + e] = make_int2(0, 0);
+            for (int e = threadIdx.x; e < heads; e += 64 * WAVES) a.pieces[b * heads + e] = make_int2(0, 0);
         for (int64_t e = threadIdx.x; e < row; e += 64 * WAVES) {
             if (a.out_f32) static_cast<float*>(a.out)[b * row + e] = y;
             else static_cast<typename Q::T*>(a.out)[b * row + e] = Q::store(y);
@@ -899,21 +903,20 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
     const bool vec = hd % 8 == 0 && (ends & 15) == 0 && ld * elem_size(src_type) % 16 == 0 && Hkv * hd < (1 << 28);
     with_float(src_type, [&](auto s) {
         using S = decltype(s);
-        const dim3 one((unsigned)tokens);
+        const dim3 one = grid_of(tokens);
         if (cache_type == LQ_I8) {
             if (vec && hd <= 64) hipLaunchKernelGGL((append_i8_kernel<8, S>), one, dim3(256), 0, st, a);
             else if (vec && hd <= 128) hipLaunchKernelGGL((append_i8_kernel<16, S>), one, dim3(256), 0, st, a);
             else if (vec && hd <= 256) hipLaunchKernelGGL((append_i8_kernel<32, S>), one, dim3(256), 0, st, a);
             else
-                hipLaunchKernelGGL((append_i8_any_kernel<S>), dim3((unsigned)tokens, (unsigned)(2 * Hkv)), dim3(64), 0,
-                                   st, a);
+                hipLaunchKernelGGL((append_i8_any_kernel<S>), grid_of(tokens * 2 * Hkv), dim3(64), 0, st, a);
             return;
         }
         with_half(cache_type, [&](auto c) {
             using C = decltype(c);
             if (!vec) hipLaunchKernelGGL((append_any_kernel<S, C>), one, dim3(256), 0, st, a);
             else if (tokens <= 4 * 1024) hipLaunchKernelGGL((append_kernel<1, S, C>), one, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((append_kernel<4, S, C>), dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((append_kernel<4, S, C>), grid_of((tokens + 3) / 4), dim3(256), 0, st, a);
         });
     });
     return launch_status("lq_paged_kv_append");
@@ -960,7 +963,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
                       d_v_scale, pages, (int)page, d_table, table_stride, d_lengths, scale, d_out, out_type == LQ_F32,
                       aligned16(d_q) && ldq % 8 == 0, groups, reinterpret_cast<int2*>(ws), part_o,
                       alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
-    const dim3 grid((unsigned)(alone ? units : groups));
+    const dim3 grid = grid_of(alone ? units : groups);
     const hipStream_t st = as_stream(stream);
     // A few short sequences: as many waves each as the LDS holds tiles for, to hide more of the latency (8 sequences
     // of up to 640, 8 heads of 64: 9.9 us with four waves, 8.8 with eight); else two, two workgroups to a CU.

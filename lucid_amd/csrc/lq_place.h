@@ -13,6 +13,19 @@
 
 namespace lq {
 
+// Workgroups of a launch in two dimensions.  A launch takes fewer than 2^32 work items in x: rows of 2^22
+// workgroups (of 512 threads at most), the last row in part past the end, as many rows as it takes
+// (65535 at most, that is 2.7e11 workgroups: more than the memory has rows for).
+struct Workgroups {
+    uint32_t x, y;
+};
+constexpr int64_t WORKGROUPS_X = (int64_t)1 << 22;
+LQ_PLACE Workgroups workgroups(int64_t n) {
+    return n <= WORKGROUPS_X ? Workgroups{(uint32_t)n, 1}
+                             : Workgroups{(uint32_t)WORKGROUPS_X, (uint32_t)((n + WORKGROUPS_X - 1) / WORKGROUPS_X)};
+}
+LQ_PLACE int64_t workgroup_index(uint32_t x, uint32_t y) { return (int64_t)y * WORKGROUPS_X + x; }
+
 // The last of `seqs` (>= 1) sequences whose start is at or before t (the first one if none is).
 // Any contents of starts[0 .. seqs - 1] give a number in [0, seqs).
 LQ_PLACE int64_t sequence_of(const int32_t* starts, int64_t seqs, int64_t t) {

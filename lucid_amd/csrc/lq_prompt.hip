@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hh = lane >> 5;
     const uint32_t group = (uint32_t)(a.H / a.Hkv);
-    const uint32_t n = blockIdx.x / (uint32_t)a.H, hx = blockIdx.x - n * (uint32_t)a.H;
+    const uint32_t id = (uint32_t)workgroup(), n = id / (uint32_t)a.H, hx = id - n * (uint32_t)a.H;
     // consecutive workgroups (on consecutive XCDs) take different key heads: an XCD's L2 then
     // serves few of them
     const int hk = hx % (uint32_t)a.Hkv, h = hk * group + hx / (uint32_t)a.Hkv;
@@ -454,7 +454,7 @@ int lq_prompt_attention(const void* d_q, int64_t ldq, const void* d_k, int64_t l
         // 128: 87 us with 128 queries, 66 with 64; 34 of up to 3483 with 2 heads: 81 and 64; at twice as
         // many workgroups no difference).
         const bool many = blocks(128) >= 2 * 512;
-        const dim3 tiles((unsigned)blocks(many ? 128 : 64)), wg(64 * PT_WAVES);
+        const dim3 tiles = grid_of(blocks(many ? 128 : 64)), wg(64 * PT_WAVES);
         with_half(type, [&](auto e) {
             using E = decltype(e);
             auto go = [&](auto w, auto o) {

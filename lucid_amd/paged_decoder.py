@@ -82,12 +82,18 @@ class PagedDecoder:
                 raise ValueError(f"a prompt of {len(p)} tokens, {self.positions} positions")
         return out
 
+    def _sequences(self, keys) -> list[int]:
+        seqs = sorted(keys)
+        if seqs and (seqs[0] < 0 or seqs[-1] >= self.table.seqs):
+            raise ValueError(f"sequences {seqs}: this decoder serves 0 .. {self.table.seqs - 1}")
+        return seqs
+
     # ------------------------------------------------------------------ serving
 
     def prefill(self, prompts: dict[int, np.ndarray]) -> Tensor:
         """Prompts into the empty sequences they are keyed by; the logits ``[len(prompts),
         vocab]`` after each, in the order of the sequences."""
-        seqs = sorted(prompts)
+        seqs = self._sequences(prompts)
         toks = dict(zip(seqs, self._check([prompts[s] for s in seqs])))
         held = self.table.host_lengths()
         for s in seqs:
@@ -111,7 +117,7 @@ class PagedDecoder:
     def step(self, tokens: dict[int, int]) -> Tensor:
         """One token more for some of the sequences; the logits ``[len(tokens), vocab]``, in the
         order of the sequences."""
-        seqs = sorted(tokens)
+        seqs = self._sequences(tokens)
         held = self.table.host_lengths()
         if any(held[s] == 0 or held[s] >= self.positions for s in seqs):
             raise ValueError("a step needs sequences that hold something and have a position left")

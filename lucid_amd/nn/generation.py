@@ -344,6 +344,14 @@ class PageTable:
         self._lengths = new.astype(np.int32)
         self._upload(more > 0, stream)
 
+    def shrink(self, counts, stream=None) -> None:
+        """``counts[s]`` positions fewer at every sequence's end; its pages stay with it."""
+        new = self._lengths - np.asarray(counts, np.int64)
+        if new.shape != (self.seqs,) or (new < 0).any() or (new > self._lengths).any():
+            raise ValueError(f"PageTable.shrink: {self.seqs} counts of 0 to the lengths expected")
+        self._lengths = new.astype(np.int32)
+        self._upload(False, stream)
+
     def release(self, s: int, stream=None) -> None:
         """Sequence ``s`` ends: its pages are free again and its length is 0, on ``stream``."""
         self._free.extend(int(p) for p in self._table[s, :self._held[s]][::-1])

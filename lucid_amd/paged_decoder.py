@@ -110,9 +110,14 @@ class PagedDecoder:
             self.cache[i].append_qkv(qkv, HEADS, starts)
             return F.prompt_attention_qkv(qkv, HEADS, HEADS, starts, out_dtype=float32)
 
-        h = self._hidden(np.concatenate([toks[s] for s in seqs]),
-                         np.concatenate([np.arange(len(toks[s])) for s in seqs]), attend)
-        return self.qdec.head(self._rows(h, ends[seqs] - 1))
+        try:
+            h = self._hidden(np.concatenate([toks[s] for s in seqs]),
+                             np.concatenate([np.arange(len(toks[s])) for s in seqs]), attend)
+            return self.qdec.head(self._rows(h, ends[seqs] - 1))
+        except BaseException:  # their positions hold nothing
+            for s in seqs:
+                self.table.release(s)
+            raise
 
     def step(self, tokens: dict[int, int]) -> Tensor:
         """One token more for some of the sequences; the logits ``[len(tokens), vocab]``, in the
@@ -135,9 +140,13 @@ class PagedDecoder:
             return F.paged_attention(qkv, cache.k, cache.v, table, lengths, self.table.max_length, None, cache.k_scale,
                                      cache.v_scale, float32, None, HEADS)
 
-        if not whole:  # the stepping sequences' rows of the table
-            table, lengths = self.table.rows(seqs)
-        return self.qdec.head(self._hidden(np.array([tokens[s] for s in seqs]), held[seqs], attend))
+        try:
+            if not whole:  # the stepping sequences' rows of the table
+                table, lengths = self.table.rows(seqs)
+            return self.qdec.head(self._hidden(np.array([tokens[s] for s in seqs]), held[seqs], attend))
+        except BaseException:  # the last positions hold nothing
+            self.table.shrink(counts)
+            raise
 
     def generate(self, prompts: list, steps: int, top: int = 5):
         """Greedy continuations of up to ``seqs`` prompts: tokens ``[len(prompts), steps]``, their
@@ -145,18 +154,23 @@ class PagedDecoder:
         n = len(prompts)
         logits = self.prefill(dict(enumerate(prompts)))
         out, scores, others = [], [], []
-        for k in range(steps):
-            best = empty((n,), np.int32, "gpu")
-            _C.call("lq_argmax_f32", logits.data_ptr(), n, self.vocab, best.data_ptr(), None)
-            lp, _, _, _, ids = F.token_logprobs(logits, best, top)
-            out.append(best.numpy())
-            scores.append(lp.numpy())
-            others.append(ids.numpy())
-            if k + 1 < steps:
-                logits = self.step(dict(enumerate(out[-1].tolist())))
-        for s in range(n):
-            self.table.release(s)
+        try:
+            for k in range(steps):
+                for kept, new in zip((out, scores, others), self._choose(logits, n, top)):
+                    kept.append(new)
+                if k + 1 < steps:
+                    logits = self.step(dict(enumerate(out[-1].tolist())))
+        finally:
+            for s in range(n):
+                self.table.release(s)
         return np.stack(out, 1), np.stack(scores, 1), np.stack(others, 1)
+
+    def _choose(self, logits: Tensor, n: int, top: int):
+        """The most likely tokens after ``n`` sequences, their log probabilities, the alternatives' ids."""
+        best = empty((n,), np.int32, "gpu")
+        _C.call("lq_argmax_f32", logits.data_ptr(), n, self.vocab, best.data_ptr(), None)
+        lp, _, _, _, ids = F.token_logprobs(logits, best, top)
+        return best.numpy(), lp.numpy(), ids.numpy()
 
     # ------------------------------------------------------------------ scoring and tuning
 

@@ -32,3 +32,55 @@ def test_sequence_keys_outside_the_table_are_refused(key):
     with pytest.raises(ValueError, match="sequence"):
         pd.step({key: 5, 0: 1})
     assert (pd.table.host_lengths() == 2).all()
+
+
+def test_generate_gives_its_sequences_back_when_a_step_fails(monkeypatch):
+    """Pages used up on the way: the next call finds the sequences free, and those of others untouched."""
+    pd = _decoder()
+    pd.table.grow([0, 0, 3])  # somebody else's
+    monkeypatch.setattr(pd, "prefill", lambda prompts: pd.table.grow([len(prompts[0]), len(prompts[1]), 0]))
+    monkeypatch.setattr(pd, "_choose", lambda logits, n, top: (np.zeros(n, np.int32),) * 3, raising=False)
+
+    def step(tokens):
+        raise MemoryError("no pages")
+
+    monkeypatch.setattr(pd, "step", step)
+    with pytest.raises(MemoryError):
+        pd.generate([np.array([1, 2, 3]), np.array([4])], 3)
+    assert pd.table.host_lengths().tolist() == [0, 0, 3]
+    assert len(pd.table._free) == pd.table.pages - 1
+
+
+def test_a_failed_prefill_leaves_the_table_as_it_was(monkeypatch):
+    pd = _decoder()
+    pd.table.grow([0, 5, 0])
+
+    def hidden(*a):
+        raise MemoryError("no memory")
+
+    monkeypatch.setattr(pd, "_hidden", hidden)
+    monkeypatch.setattr("lucid_amd.paged_decoder._ints", lambda a: a)
+    with pytest.raises(MemoryError):
+        pd.prefill({0: np.array([1, 2]), 2: np.array([3])})
+    assert pd.table.host_lengths().tolist() == [0, 5, 0]
+    assert len(pd.table._free) == pd.table.pages - 2
+
+
+def test_a_failed_step_takes_its_positions_back(monkeypatch):
+    pd = _decoder()
+    pd.table.grow([4, 3, 2])
+
+    def hidden(*a):
+        raise MemoryError("no memory")
+
+    monkeypatch.setattr(pd, "_hidden", hidden)
+    monkeypatch.setattr("lucid_amd.paged_decoder._ints", lambda a: a)
+    with pytest.raises(MemoryError):
+        pd.step({0: 1, 1: 2, 2: 3})
+    assert pd.table.host_lengths().tolist() == [4, 3, 2]
+    pd.table.grow([1, 0, 0])  # the page it took serves the next try
+    assert len(pd.table._free) == pd.table.pages - 4
+    for counts in ([6, 0, 0], [-1, 0, 0], [1, 1]):
+        with pytest.raises(ValueError):
+            pd.table.shrink(counts)
+    assert pd.table.host_lengths().tolist() == [5, 3, 2]

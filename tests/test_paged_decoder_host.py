@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -18,6 +20,7 @@ def _decoder(seqs=3, pages=12, page=4, vocab=50, positions=32):
     table._upload = lambda *a: None
     pd = PagedDecoder.__new__(PagedDecoder)
     pd.table, pd.vocab, pd.positions = table, vocab, positions
+    pd.qdec = SimpleNamespace(head=lambda h: h)
     return pd
 
 

@@ -74,13 +74,16 @@ class PagedDecoder:
         return F.embedding(_ints(rows), x)
 
     def _check(self, prompts) -> list[np.ndarray]:
-        out = [np.asarray(p, np.int32).ravel() for p in prompts]
+        out = [np.asarray(p, np.int64).ravel() for p in prompts]
         for p in out:
-            if len(p) and (p.min() < 0 or p.max() >= self.vocab):
-                raise ValueError("prompt token ids out of the vocabulary")
+            self._known(p, "prompt")
             if len(p) > self.positions:
                 raise ValueError(f"a prompt of {len(p)} tokens, {self.positions} positions")
-        return out
+        return [p.astype(np.int32) for p in out]
+
+    def _known(self, ids: np.ndarray, what: str) -> None:
+        if len(ids) and (ids.min() < 0 or ids.max() >= self.vocab):
+            raise ValueError(f"{what} token ids out of the vocabulary")
 
     def _sequences(self, keys) -> list[int]:
         seqs = sorted(keys)
@@ -126,6 +129,8 @@ class PagedDecoder:
         held = self.table.host_lengths()
         if any(held[s] == 0 or held[s] >= self.positions for s in seqs):
             raise ValueError("a step needs sequences that hold something and have a position left")
+        ids = np.array([tokens[s] for s in seqs], np.int64)
+        self._known(ids, "step")
         counts = np.zeros(self.table.seqs, np.int64)
         counts[seqs] = 1
         self.table.grow(counts)
@@ -143,7 +148,7 @@ class PagedDecoder:
         try:
             if not whole:  # the stepping sequences' rows of the table
                 table, lengths = self.table.rows(seqs)
-            return self.qdec.head(self._hidden(np.array([tokens[s] for s in seqs]), held[seqs], attend))
+            return self.qdec.head(self._hidden(ids, held[seqs], attend))
         except BaseException:  # the last positions hold nothing
             self.table.shrink(counts)
             raise

@@ -87,3 +87,17 @@ def test_a_failed_step_takes_its_positions_back(monkeypatch):
         with pytest.raises(ValueError):
             pd.table.shrink(counts)
     assert pd.table.host_lengths().tolist() == [5, 3, 2]
+
+
+@pytest.mark.parametrize("token", [-1, 50, 1 << 31])
+def test_step_refuses_tokens_outside_the_vocabulary(token):
+    """The embedding would give a row of NaN, which every later step of that sequence would attend."""
+    pd = _decoder()
+    pd.table.grow([2, 2, 2])
+    with pytest.raises(ValueError, match="vocabulary"):
+        pd.step({1: token, 2: 3})
+    with pytest.raises(ValueError, match="vocabulary"):
+        pd.prefill({0: np.array([token])})
+    with pytest.raises(ValueError, match="vocabulary"):
+        pd.score([[token, 2]])
+    assert (pd.table.host_lengths() == 2).all()

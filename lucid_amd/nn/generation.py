@@ -196,7 +196,8 @@ def prompt_attention(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts
                      causal: bool = True, scale: float | None = None, out_dtype=None, stream=None) -> Tensor:
     """Attention over packed sequences: ``q`` [tokens, heads, head_dim], ``k`` / ``v`` [tokens,
     kv_heads, head_dim], ``q_starts`` / ``k_starts`` [seqs + 1] (the same for both unless given).
-    See ``lq_prompt_attention``."""
+    Rows of the result that belong to no sequence (before the first start, past the last) are not
+    written and hold whatever the memory held.  See ``lq_prompt_attention``."""
     op = "prompt_attention"
     dt = _need(q, op, "q", 3, (float16, bfloat16))
     _need(k, op, "k", 3, (dt,))
@@ -212,7 +213,7 @@ def prompt_attention(q: Tensor, k: Tensor, v: Tensor, q_starts: Tensor, k_starts
 def prompt_attention_qkv(qkv: Tensor, heads: int, kv_heads: int, starts: Tensor, causal: bool = True,
                          scale: float | None = None, out_dtype=None, stream=None) -> Tensor:
     """:func:`prompt_attention` of a fused projection's rows ``[tokens, heads + 2 kv_heads,
-    head_dim]``, read in place."""
+    head_dim]``, read in place.  Rows of no sequence are not written."""
     op = "prompt_attention_qkv"
     dt = _need(qkv, op, "qkv", 3, (float16, bfloat16))
     if kv_heads < 1 or heads < 1 or heads % kv_heads or qkv.shape[1] != heads + 2 * kv_heads:

@@ -230,8 +230,9 @@ __device__ __forceinline__ int sequence_length(const PagedArgs& a, int b, bool& 
 //   positions 4 g + i (and 16 + 4 g + i) of query l;
 //   O^T += V^T P^T: those weights are the B operand as they are; V comes from the wave's LDS, whose
 //   transposing read gives lane (l, g) dim l of the same positions.
-// A weight enters as two 16-bit terms (about 16 significant bits): the products are free beside the
-// loads.
+// A weight enters as 16-bit terms: two hold 22 bits of it in fp16 and 16 in bfloat16, which is more than a
+// 16-bit output keeps; a float32 output takes a third one in bfloat16 (24 bits).  The products are free
+// beside the loads.
 struct Piece {
     int b, h0, hk, heads, begin, end, len;
     bool over, whole;
@@ -430,9 +431,10 @@ struct Sums {
                 l += sc[T][i];
             }
     }
-    // O^T += V^T P^T, V at LDS `v_at` with rows of VROW bytes swizzled by swz
+    // O^T += V^T P^T, V at LDS `v_at` with rows of VROW bytes swizzled by swz; `all`: every bit of the weights
     template <int VROW, class F>
-    __device__ __forceinline__ void accumulate(const vf4 (&w)[2], uint32_t v_at, F swz) {
+    __device__ __forceinline__ void accumulate(const vf4 (&w)[2], uint32_t v_at, F swz, bool all) {
+        const bool third = P::code == LQ_BF16 && all;
         u4v ph, pl;
 #pragma unroll
         for (int T = 0; T < 2; ++T)
@@ -444,13 +446,27 @@ struct Sums {
                 pl[2 * T + i] = pack2(P{}, w[T][2 * i] - r[0], w[T][2 * i + 1] - r[1]);
             }
         const int lane = threadIdx.x & 63, vi = lane & 15, row = 4 * (lane >> 4) + (vi >> 2);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
+        auto values = [&](int d) __attribute__((always_inline)) {
             const uint32_t at = v_at + row * VROW + (((2 * d + ((vi & 3) >> 1)) ^ swz(row)) << 4) + 8 * (vi & 1);
             const u2v lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * VROW);
-            const u4v v = {lo[0], lo[1], hi[0], hi[1]};
+            return u4v{lo[0], lo[1], hi[0], hi[1]};
+        };
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const u4v v = values(d);
             o[d] = mfma_16x16x32(P{}, v, ph, o[d]);
             o[d] = mfma_16x16x32(P{}, v, pl, o[d]);
+        }
+        if (third) {  // apart, so that the loop above stays one block
+#pragma unroll
+            for (int T = 0; T < 2; ++T)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f2v r = unpack2(P{}, ph[2 * T + i]), e = unpack2(P{}, pl[2 * T + i]);
+                    ph[2 * T + i] = pack2(P{}, w[T][2 * i] - r[0] - e[0], w[T][2 * i + 1] - r[1] - e[1]);
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = mfma_16x16x32(P{}, values(d), ph, o[d]);
         }
     }
 };
@@ -645,7 +661,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
                             *reinterpret_cast<lds_u4v*>(vt + r * ROW + c * 16) = u4v{0, 0, 0, 0};
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 }
-                sums.template accumulate<ROW>(sc, vt, v_swz<HDP>);
+                sums.template accumulate<ROW>(sc, vt, v_swz<HDP>, a.out_f32 != 0);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
                 if (t + NST < tiles) issue(t + NST);
             }
@@ -776,7 +792,7 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sc[T][i] *= f[i];
                 }
-                sums.template accumulate<ROW>(sc, slot_at, v_swz<HDP>);
+                sums.template accumulate<ROW>(sc, slot_at, v_swz<HDP>, a.out_f32 != 0);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads, before the next tile's writes
             }
         }

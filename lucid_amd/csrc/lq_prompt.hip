@@ -157,7 +157,10 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
     constexpr int TILE = PT_K * HDP * 2;                        // bytes of a K (or V) tile
     constexpr int COPIES = PT_K * CPR / (64 * PT_WAVES);        // 16-byte copies of a lane per tile
     constexpr int KS = HDP / 16, DT = HDP / 32, KT = PT_K / 32 / SPLIT;
-    constexpr bool TWO = Out::code == LQ_F32;                   // weights as two terms
+    // A weight enters its product in 16 bits: once rounded for a 16-bit output (one more rounding of the size of
+    // the output's own; a second term would be half as many products again, and they bound the kernel);
+    // as two terms in fp16 (22 bits), three in bfloat16 (24 bits), for a float32 output.
+    constexpr int TERMS = Out::code != LQ_F32 ? 1 : E::code == LQ_F16 ? 2 : 3;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];
     __shared__ int odd_values[PT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
         const bool more = !MASKED || t + 1 < mine;
         if (more) scores(t + 1, next);
         const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<E>;
-        u4v p[2 * KT], pl[TWO ? 2 * KT : 1];
+        u4v p[TERMS][2 * KT];
         float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < KT; ++b)
@@ -301,11 +304,16 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i + 1], sl2, -base));
                 l += x;
                 sum += y;
-                const uint32_t w = pack2(E{}, x, y);
-                p[2 * b + (i >> 3)][(i & 7) >> 1] = w;
-                if constexpr (TWO) {
-                    const f2v r = unpack2(E{}, w);
-                    pl[2 * b + (i >> 3)][(i & 7) >> 1] = pack2(E{}, x - r[0], y - r[1]);
+                float u = x, v = y;  // what the terms so far leave
+#pragma unroll
+                for (int n = 0; n < TERMS; ++n) {
+                    const uint32_t w = pack2(E{}, u, v);
+                    p[n][2 * b + (i >> 3)][(i & 7) >> 1] = w;
+                    if (n + 1 < TERMS) {
+                        const f2v r = unpack2(E{}, w);
+                        u -= r[0];
+                        v -= r[1];
+                    }
                 }
             }
         l += sum;
@@ -320,8 +328,8 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const u4v v = value(d, ks);
-                o[d] = mfma_32x32x16(E{}, v, p[ks], o[d]);
-                if constexpr (TWO) o[d] = mfma_32x32x16(E{}, v, pl[ks], o[d]);
+#pragma unroll
+                for (int n = 0; n < TERMS; ++n) o[d] = mfma_32x32x16(E{}, v, p[n][ks], o[d]);
             }
         if (more) {
             if (MASKED && t + 1 >= open) mask(t + 1, next);
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
         for (int b = 0; b < KT; ++b) sa[b] = sb[b];
     }
     // An infinity or NaN among the values has met weights it must not meet: the 0 of a key that is not seen, the
-    // second term of a weight.  It left a sum that is not finite; such queries are computed again.
+    // second or third term of a weight.  It left a sum that is not finite; such queries are computed again.
     bool odd = false;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
             for (int i = 0; i < 16; i += 4) {
                 const int dim = 32 * d + 2 * i + 4 * hh;
                 if (dim < hd) {
-                    if constexpr (TWO) {
+                    if constexpr (Out::code == LQ_F32) {
                         *reinterpret_cast<vf4*>(orow + dim) = vf4{o[d][i] * r, o[d][i + 1] * r, o[d][i + 2] * r,
                                                                   o[d][i + 3] * r};
                     } else {

@@ -134,9 +134,14 @@ __device__ __forceinline__ void row_choice(const LogprobArgs& a, int64_t r, int 
     a.top_logprobs[r * a.top + at] = logprob_of(E::load(static_cast<const typename E::T*>(a.x)[r * a.ldx + j]), lse);
 }
 
-// One workgroup per row, one pass over it.  A thread keeps a reference for its exponentials (it
-// follows the largest value only when that has risen by more than 16, so that the sums are rarely
-// rescaled), the sums of e^d and of e^d d, and its largest value.
+// One workgroup per row, one pass over it.  A thread keeps a reference for its exponentials, the sums of e^d
+// and of e^d d, and its largest value.  The reference follows the largest value when that has risen by more
+// than 4, looked at once for four chunks: the sum of e^d d is rounded at the size that the largest value
+// has relative to the reference, and the final change of reference takes most of it away again (past a rise
+// of 16 only, the entropy of rows that one token rules was off by 100 half-steps of float32's 1, now by 4;
+// 8 rows of 32000 float32 logits take 7.6 us for 7.36, past a rise of 2 7.66).  Chunks are summed before
+// they are added: a sum that holds the row's largest value then loses the small ones by rounding only
+// where a whole group of them is below 2^-25 of it.
 //
 // The alternatives come from those largest values: of 64 groups of threads, the top-th largest group
 // maximum `cut` has at least `top` elements at or above it, and only threads whose own maximum
@@ -166,23 +171,36 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
     const Split<E> row(static_cast<const typename E::T*>(a.x) + r * a.ldx + c0, min(width, a.vocab - c0));
 
     float ref = -INFINITY, base = 0.0f, top = -INFINITY, s = 0.0f, ed = 0.0f;  // base: ref, 0 while it is -inf
-    auto add = [&](const Chunk<E>& c) __attribute__((always_inline)) {
+    auto largest = [](const Chunk<E>& c) __attribute__((always_inline)) {
         float m = c.v[0];
 #pragma unroll
         for (int e = 1; e < N; ++e) m = fmaxf(m, c.v[e]);
+        return m;
+    };
+    auto follow = [&](float m) __attribute__((always_inline)) {
         top = fmaxf(top, m);
-        if (m > ref + 16.0f) {
+        if (m > ref + 4.0f) {
             const float f = s > 0.0f ? __builtin_amdgcn_exp2f((base - m) * LOG2E) : 0.0f;
             ed = f > 0.0f ? f * __builtin_fmaf(s, base - m, ed) : 0.0f;
             s *= f;
             ref = base = m;
         }
+    };
+    auto sums = [&](const Chunk<E>& c, float& cs, float& ce) __attribute__((always_inline)) {
+        cs = ce = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const float d = c.v[e] - base, p = __builtin_amdgcn_exp2f(d * LOG2E);
-            s += p;
-            ed = __builtin_fmaf(p, fmaxf(d, -1000.0f), ed);  // p is 0 there: no 0 * inf
+            cs += p;
+            ce = __builtin_fmaf(p, fmaxf(d, -1000.0f), ce);  // p is 0 there: no 0 * inf
         }
+    };
+    auto add = [&](const Chunk<E>& c) __attribute__((always_inline)) {
+        follow(largest(c));
+        float cs, ce;
+        sums(c, cs, ce);
+        s += cs;
+        ed += ce;
     };
     // the single elements of both ends: one each of the first threads, on their way during the loop
     Chunk<E> ends;
@@ -195,8 +213,16 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs a) {
         u4v w[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) w[u] = row.load(q + u * NT);
+        Chunk<E> c[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) add(widen<E>(w[u]));
+        for (int u = 0; u < UNROLL; ++u) c[u] = widen<E>(w[u]);
+        static_assert(UNROLL == 4, "the sums below");
+        follow(fmaxf(fmaxf(largest(c[0]), largest(c[1])), fmaxf(largest(c[2]), largest(c[3]))));
+        float cs[UNROLL], ce[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) sums(c[u], cs[u], ce[u]);
+        s += (cs[0] + cs[1]) + (cs[2] + cs[3]);
+        ed += (ce[0] + ce[1]) + (ce[2] + ce[3]);
     }
     for (; q < row.chunks; q += NT) add(widen<E>(row.load(q)));
     if (tid < N) add(ends);

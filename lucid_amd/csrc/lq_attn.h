@@ -94,10 +94,19 @@ __device__ __forceinline__ f2v unpack2(ElemBF16, uint32_t w) {
 }
 // A weight that enters a product in 16 bits is 2^WEIGHT_SHIFT times its value relative to the
 // running maximum (which may lag by 2^RESCALE_AT): fp16 then resolves weights down to 2^-30 of
-// the largest and stays below 2^14; bfloat16 has float32's exponents and needs no shift.
+// the largest and stays below 2^14.  bfloat16 has float32's exponents, for its values too: the shift
+// down keeps the sums of a million values of 1e36, or of 4096 of the type's largest, finite.
 template <class E>
-constexpr float WEIGHT_SHIFT = E::code == LQ_F16 ? 6.0f : 0.0f;
+constexpr float WEIGHT_SHIFT = E::code == LQ_F16 ? 6.0f : -20.0f;
 constexpr float RESCALE_AT = 8.0f;
+// The reference of the weights for a largest score mx (log2 units).  In bfloat16 mx to 2^-13: the large shift is
+// then exact on it (below 2^11), so that sums with different references stay comparable, and the largest
+// weight, 2^-13 from a power of two at most, still rounds to it.
+template <class E>
+__device__ __forceinline__ float weight_reference(float mx) {
+    if constexpr (E::code == LQ_BF16) return fabsf(mx) < 2048.0f ? rintf(mx * 8192.0f) * (1.0f / 8192.0f) : mx;
+    return mx;
+}
 
 // The larger / the sum of the values that lanes l and l ^ 32 hold.
 __device__ __forceinline__ float half_max(float v) {

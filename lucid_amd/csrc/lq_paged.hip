@@ -413,7 +413,7 @@ struct Sums {
             }
         mx = quarter_max(mx) * sl2;
         if (__any(mx > m + RESCALE_AT)) {
-            const float mn = fmaxf(m, mx);
+            const float mn = fmaxf(m, weight_reference<P>(mx));
             const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
             l *= corr;

@@ -34,6 +34,7 @@ __device__ __forceinline__ void attend_row(const PromptArgs& a, int64_t t, int h
     const typename E::T* q = static_cast<const typename E::T*>(a.q) + t * a.ldq + (int64_t)h * hd;
     const typename E::T* k = static_cast<const typename E::T*>(a.k) + k0 * a.ldk + (int64_t)hk * hd;
     const typename E::T* v = static_cast<const typename E::T*>(a.v) + k0 * a.ldv + (int64_t)hk * hd;
+    const float fit = E::code == LQ_BF16 ? exp2f(WEIGHT_SHIFT<E>) : 1.0f;  // sums of the largest values stay finite
     float m = -INFINITY, l = 0.0f, acc[PARTS] = {};
     for (int64_t kb = 0; kb < len; kb += 64) {
         const int n = (int)min((int64_t)64, len - kb);
@@ -48,7 +49,7 @@ __device__ __forceinline__ void attend_row(const PromptArgs& a, int64_t t, int h
         for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
         mx = fmaxf(mx, m);
         const float base = mx == -INFINITY ? 0.0f : mx;
-        const float e = lane < n ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
+        const float e = lane < n ? __builtin_amdgcn_exp2f(s - base) * fit : 0.0f;
         const float corr = __builtin_amdgcn_exp2f(m - base);
         m = mx;
         l = l * corr + ln_wave_sum(e);
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) 
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
         mx = half_max(mx) * sl2;
         if (__any(mx > m + RESCALE_AT)) {
-            const float mn = fmaxf(m, mx);
+            const float mn = fmaxf(m, weight_reference<E>(mx));
             const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
             l *= corr;

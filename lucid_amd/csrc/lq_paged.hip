@@ -673,9 +673,10 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
 
 // int8 cache.  Codes are exact in 16 bits: they are loaded to registers (a tile ahead), widened there,
 // and V goes to the wave's LDS as bfloat16.  The key's scale multiplies the score, the value's scale
-// the weight, which is bfloat16 for its range.  The widening bounds it, one and a half vector
-// instructions a code: 131071 positions and a second sequence, 8 heads of 128, 81 us with the join (4.8
-// TB/s; 125 us with the compiler's own conversions).
+// the weight, which is bfloat16 for its range.  131071 positions and a second sequence, 8 heads of 128: 79
+// us with the join (4.9 TB/s).  No unit is full there: the vector unit is busy 44% of the time (one and a
+// half instructions a code; with the compiler's own conversions 125 us) and the matrix cores 9%, while the
+// waves, two to a SIMD with a tile ahead each, wait for loads half of theirs.
 template <int HDP, bool EXACT, class Q>
 __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) void paged_i8_kernel(PagedArgs a) {
     using P = ElemBF16;
@@ -878,8 +879,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 
 // Workgroups of a call over long sequences: as many as run at a time (two to a CU, one past 128 dims; three of
 // the int8 kernel up to 64: 69 sequences of up to 39768, 2 heads of 64, 59 -> 55 us).
-// Up to PG_ALONE positions each workgroup takes a sequence whole: the second launch would cost more
-// than it gives (8 sequences of 640: 9.1 us against 12.5).
+// Up to PG_ALONE positions each workgroup takes a sequence whole: the plan and the second launch would cost
+// more than they give.  Whole against shared, us a call, 16-bit rows of 64 / 128 dims, ragged lengths:
+//   sequences x key heads      8                    256                   1024
+//   longest 512     7.0-14.3 / 13.2-17.5   8.7-16.2 / 14.3-19.3   21.0-27.4 / 28.4-35.6
+//   longest 1024   10.4-15.1 / 20.4-17.7  12.8-17.4 / 22.8-21.7   35.6-34.8 / 48.2-45.7
+//   longest 2048   16.7-14.9 / 35.0-18.0  19.3-23.1 / 37.2-29.6   68.2-57.2 / 94.1-76.4
+// (at 1024 rows of 128 dims lose up to 15% by it; int8 rows are alike.)
 constexpr int PG_GROUPS = 512, PG_GROUPS_I8_64 = 768, PG_GROUPS_WIDE = 256, PG_ALONE = 1024;
 // bytes of the table of pieces, and the slots of a call (two to a workgroup)
 int64_t pieces_bytes(int64_t units) { return (units * (int64_t)sizeof(int2) + 15) / 16 * 16; }
@@ -982,7 +988,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
     const dim3 grid = grid_of(alone ? units : groups);
     const hipStream_t st = as_stream(stream);
     // A few short sequences: as many waves each as the LDS holds tiles for, to hide more of the latency (8 sequences
-    // of up to 640, 8 heads of 64: 9.9 us with four waves, 8.8 with eight); else two, two workgroups to a CU.
+    // of up to 640, 8 heads of 64: 9.4 us a call with four waves, 7.8 with eight); else two, two workgroups to a CU.
     const bool few = alone && units <= 256;
     note_path(!alone ? "paged shared" : few ? "paged whole few" : "paged whole");
     with_half(q_type, [&](auto q) {

@@ -147,10 +147,10 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int64_t n, Packe
 // The scores of the next tile are on the matrix cores while the vector unit makes this tile's weights (one
 // wave's exponentials beside its own products: 12288 tokens, 32 heads of 128 in bfloat16, 1192 -> 1135
 // us; an order of the two forced by scheduling hints 1155).
-// What bounds it: at that size 1090 TFLOP/s, where a library product of 16384^3 reaches 1326 on this
-// card; the card keeps 1.9 GHz under this load, at which the matrix cores are busy more than half of
-// the time, and the vector unit's work on the weights (exponential, sum, rounding) is only in
-// part beside them.  Short sequences add some 4 us of dependent loads to every workgroup.
+// What bounds it: at that size 1100 TFLOP/s, where a library product of 16384^3 reaches 1326 on this
+// card; the card keeps 1.6 to 1.9 GHz under this load, at which the matrix cores are busy 61% of the
+// time and the vector unit 54% (exponentials, sums and roundings of the weights, only in part beside
+// the products).  Short sequences add some 4 us of dependent loads to every workgroup.
 template <int HDP, int SPLIT, class E, class Out>
 __global__ __launch_bounds__(64 * PT_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 1) void prompt_tile_kernel(PromptArgs a) {
     constexpr int QB = 32 * PT_WAVES / SPLIT;

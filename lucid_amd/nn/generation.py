@@ -355,6 +355,8 @@ class PageTable:
 
     def release(self, s: int, stream=None) -> None:
         """Sequence ``s`` ends: its pages are free again and its length is 0, on ``stream``."""
+        if not 0 <= s < self.seqs:
+            raise ValueError(f"PageTable.release: sequence {s} of {self.seqs}")
         self._free.extend(int(p) for p in self._table[s, :self._held[s]][::-1])
         self._held[s] = 0
         self._lengths[s] = 0

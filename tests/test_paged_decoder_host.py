@@ -101,3 +101,13 @@ def test_step_refuses_tokens_outside_the_vocabulary(token):
     with pytest.raises(ValueError, match="vocabulary"):
         pd.score([[token, 2]])
     assert (pd.table.host_lengths() == 2).all()
+
+
+@pytest.mark.parametrize("s", [-1, 3])
+def test_release_refuses_sequences_outside_the_table(s):
+    """A negative number would end the last sequence."""
+    pd = _decoder()
+    pd.table.grow([2, 2, 2])
+    with pytest.raises(ValueError, match="sequence"):
+        pd.table.release(s)
+    assert (pd.table.host_lengths() == 2).all() and len(pd.table._free) == pd.table.pages - 3

@@ -102,3 +102,43 @@ def test_rows_no_vector_fits(gpu):
     assert _C.last_path() == "prompt rows"
     value = L.bf16_to_f32(_bf16(LARGEST)).astype(np.float64)
     _check(out.numpy().astype(np.float64), np.full((n, 1, hd), value), n, U)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 72])
+@pytest.mark.parametrize("n", [70, 1500])
+def test_infinite_values_in_pages(gpu, hd, n):
+    """An infinity among bfloat16 values gives an infinity in its dim (NaN where both signs meet), and nothing
+    elsewhere, whether a weight enters as two terms or three."""
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(n + hd)
+    pages = -(-n // 16)
+    k, v = (rng.standard_normal((pages, 1, 16, hd)) for _ in range(2))
+    v[1, 0, 3, 5], v[2, 0, 1, 6], v[3, 0, 0, 6], v[0, 0, 2, 9] = np.inf, np.inf, -np.inf, -np.inf
+    q = _dev(_bf16(rng.standard_normal((1, 3, hd))))
+    table, lens = _dev(np.arange(pages, dtype=np.int32)[None]), _dev(np.array([n], np.int32))
+    for dt in (L.float32, L.bfloat16):
+        got = _values(F.paged_attention(q, _dev(_bf16(k)), _dev(_bf16(v)), table, lens, n, out_dtype=dt))[0]
+        assert (got[:, 5] == np.inf).all() and np.isnan(got[:, 6]).all() and (got[:, 9] == -np.inf).all()
+        assert np.isfinite(np.delete(got, [5, 6, 9], 1)).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 72])
+@pytest.mark.parametrize("h", [2, 32])
+def test_infinite_values_in_prompts(gpu, hd, h):
+    """Queries before an infinity are finite, those from it on have it in its dim alone."""
+    import lucid_amd as L
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(hd)
+    lens = [200] + [3] * 60
+    n = sum(lens)
+    q, k, v = (rng.standard_normal((n, m, hd)) for m in (h, 1, 1))
+    v[90, 0, 7] = -np.inf
+    st = _dev(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    for dt in (L.float32, L.bfloat16):
+        got = _values(F.prompt_attention(_dev(_bf16(q)), _dev(_bf16(k)), _dev(_bf16(v)), st, out_dtype=dt))
+        assert (got[90:200, :, 7] == -np.inf).all()
+        got[90:200, :, 7] = 0
+        assert np.isfinite(got).all()

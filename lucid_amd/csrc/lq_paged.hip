@@ -558,7 +558,7 @@ constexpr int PG_IDS = WAVES > 4 ? 128 : 512;
 // fp16 / bfloat16 cache.  K and V tiles are copied to the wave's LDS 16 bytes a lane, NST tiles deep: the
 // copies of a row are one contiguous access, they need no registers, and a wave waits only for
 // its oldest tile.  The byte offsets of PG_IDS positions at a time are looked up before their copies.
-// Bound by HBM: 64 sequences of 256 to 8191 positions, 8 heads of 128, 108 us with the join (5.5 TB/s); of
+// Bound by HBM: 64 sequences of 256 to 8191 positions, 8 heads of 128, 110 us with the join (5.4 TB/s); of
 // 8192 each 336 us (6.4 TB/s).  Rows loaded to registers, 64 bytes of each at a time: 130 us, the
 // first.
 template <int HDP, int WAVES, int NST, bool EXACT, class Q>

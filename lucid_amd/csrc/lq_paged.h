@@ -386,8 +386,9 @@ __device__ __forceinline__ float paged_sum_again(const PagedArgs& a, const Piece
 }
 
 // The waves' sums meet: wave w's lie at LDS lds + w * SLOT (16 queries of OROW floats each), and the
-// workgroup writes the output or its part of it.
-template <int WAVES, int SLOT, int DT, class Q, class P>
+// workgroup writes the output or its part of it.  AGAIN: the pages hold values of type Q, infinities among
+// them; pages of codes are not read that way.
+template <bool AGAIN, int WAVES, int SLOT, int DT, class Q, class P>
 __device__ __forceinline__ void paged_finish(const PagedArgs& a, const Piece& w, uint8_t* lds, float (*ml)[2][16],
                                              Sums<DT, P>& s, bool bad) {
     constexpr int OROW = 16 * DT + 4;
@@ -416,7 +417,7 @@ __device__ __forceinline__ void paged_finish(const PagedArgs& a, const Piece& w,
             L = __builtin_fmaf(f, ml[v][1][r], L);
             x = __builtin_fmaf(f, reinterpret_cast<const float*>(lds + v * SLOT)[r * OROW + d], x);
         }
-        if constexpr (std::is_same_v<Q, P>)  // the int8 cache's values are finite codes
+        if constexpr (AGAIN)
             if (!(fabsf(x) < INFINITY) && L == L) x = paged_sum_again<Q>(a, w, r, d, M);
         if (w.whole) {
             const int64_t at = ((int64_t)w.b * a.H + w.h0 + r) * hd + d;

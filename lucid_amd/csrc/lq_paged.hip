@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
                 if (t + NST < tiles) issue(t + NST);
             }
         }
-        paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
+        paged_finish<true, WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
     paged_empty<WAVES, Q>(a);
 }
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads, before the next tile's writes
             }
         }
-        paged_finish<WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
+        paged_finish<false, WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
     paged_empty<WAVES, Q>(a);
 }

@@ -62,7 +62,8 @@ enum {
     LQ_I64 = 8,   /* int64 (indices and offsets) */
     LQ_I8_QPAIR = 9, /* table lookups only: int8 rows whose d_scale holds interleaved float32
                       * {scale, zero point} pairs per row (d_zero_point unused) */
-    LQ_BF16 = 10     /* bfloat16 (the upper 16 bits of a float32) */
+    LQ_BF16 = 10,    /* bfloat16 (the upper 16 bits of a float32) */
+    LQ_U4 = 11       /* paged caches only: 4-bit codes, two to a byte, with bfloat16 scales and biases */
 };
 
 /* ---- runtime -------------------------------------------------------------- */
@@ -735,6 +736,22 @@ int lq_layer_norm_f32(const float* d_x, int64_t ldx, float* d_y, int64_t ldy, in
 int lq_add_layer_norm_f32(float* d_x, int64_t ldx, const float* d_res, int64_t ldres, float* d_y, int64_t ldy,
                           int64_t rows, int64_t D, const float* d_gamma, const float* d_beta, float eps,
                           void* stream);
+/* Root-mean-square norm of rows, with the addition of a residual: h = x + res, rounded to `type`
+ * (LQ_F32, LQ_F16 or LQ_BF16) and stored to d_sum (d_res NULL: h = x and d_sum is not written; d_sum NULL:
+ * the sum is not stored; d_sum may be d_x or d_res, with its stride), then y = h / sqrt(mean(h^2) + eps) * gamma, where
+ * the mean, the root and the products are float32 whatever the types, and hold for rows whose squares
+ * would overflow.  gamma [D] of gamma_type (a float type; NULL: ones); rows ldx / ldres / ldsum / ldy elements
+ * apart; y of y_type (any of the three), rounded once, and apart from the inputs; eps > 0.
+ * lq_rms_norm_quantize writes y in 8 bits, a scale to a row (the a_scale of lq_gemm_w8a8 with a_scale_stride 1):
+ * scale = max|y| / 127, code = rne(y * (127 / max|y|)); a row whose magnitudes are below 127 / FLT_MAX is
+ * zeros with scale 0, one that holds NaN or an infinity has a scale that is not finite.
+ * No reference counterpart (its decoders normalize with nn.LayerNorm, in float). */
+int lq_rms_norm(const void* d_x, int type, int64_t ldx, const void* d_res, int64_t ldres, void* d_sum, int64_t ldsum,
+                const void* d_gamma, int gamma_type, float eps, int64_t rows, int64_t D, void* d_y, int y_type,
+                int64_t ldy, void* stream);
+int lq_rms_norm_quantize(const void* d_x, int type, int64_t ldx, const void* d_res, int64_t ldres, void* d_sum,
+                         int64_t ldsum, const void* d_gamma, int gamma_type, float eps, int64_t rows, int64_t D,
+                         int8_t* d_codes, int64_t ldc, float* d_scales, void* stream);
 /* y = 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) (F.gelu, approximate="tanh"), evaluated as
  * x / (1 + exp(-2 sqrt(2/pi) (x + 0.044715 x^3))) with the hardware exp2 and reciprocal (the same
  * function, within a few float32 ulps). */
@@ -798,6 +815,10 @@ int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_
  * row in [pages][Hkv][page]: value = code * scale); d_table [seqs][table_stride] of page numbers;
  * position p of sequence s is slot p % page of page d_table[s][p / page].  d_lengths [seqs]: the
  * positions each sequence holds, the new tokens among them.
+ * cache_type LQ_U4 holds 4 bits a value (hd a multiple of 32, at most 256): pages [pages][Hkv][page][hd / 2] bytes, dim
+ * d in the low half of byte d / 2 where d is even; d_k_scale [pages][Hkv][page][2][hd / 32] bfloat16, a scale for
+ * each 32 dims of a key, then a bias for each (keys have strong channels); d_v_scale [pages][Hkv][page][2] bfloat16, a
+ * scale and a bias for the whole row of a value; value = code * scale + bias.
  *
  * Appends packed new tokens: token t's keys at d_k + t * ld (elements of src_type LQ_F32, LQ_F16
  * or LQ_BF16; [Hkv][hd] contiguous), its values at d_v + t * ld.  Sequence s owns tokens
@@ -805,15 +826,35 @@ int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_
  * the one new token of sequence s (tokens == seqs).  A float cache gets each value rounded once
  * to nearest even.  An int8 cache gets scale = max|x| / 127 and code = rne(x * (127 / max|x|)) per
  * row of hd; a row with an infinity or NaN gets a scale that is not finite and is attended as
- * NaN, one whose magnitudes are below 127 / FLT_MAX as zeros.  A token is left out when its
+ * NaN, one whose magnitudes are below 127 / FLT_MAX as zeros.  4 bits: bias = the bfloat16 at or below
+ * the least x of a group, scale = the one at or above (max x - bias) / 15, code = rne((x - bias) * (1 / scale)) within
+ * 0 .. 15; a group with an infinity or NaN, or whose width passes float32, has a scale and a bias of NaN; one whose
+ * scale has no float32 reciprocal has the scale 0.  A token is left out when its
  * position is negative (a sequence of length 0), lies past the table, or its page number is
  * outside [0, pages).  Two tokens of one call must not share a place. */
 int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t ld, int64_t tokens,
                        const int32_t* d_starts, int64_t seqs, int64_t Hkv, int64_t hd, const int32_t* d_table,
                        int64_t table_stride, const int32_t* d_lengths, void* d_k_pages, void* d_v_pages,
-                       int cache_type, float* d_k_scale, float* d_v_scale, int64_t pages, int64_t page, void* stream);
+                       int cache_type, void* d_k_scale, void* d_v_scale, int64_t pages, int64_t page, void* stream);
+/* lq_paged_kv_append of keys that are rotated by their position on the way, with the queries: token t's
+ * queries at d_q + t * ldq ([H][hd] contiguous), its keys and values at d_k, d_v + t * ldkv, all of src_type.  d_angles
+ * [positions][rot] float32: for each position the cosines, then the sines, of rot / 2 angles.  Pair i of a head is
+ * its dims (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved != 0; (a, b) becomes (a c - b s, b c + a s) in
+ * float32; dims from rot (even, 0 .. hd) on stay.  The rotated queries are rounded to q_type (LQ_F16 or LQ_BF16) in
+ * d_q_out (rows ldqo apart), the rotated keys likewise in d_k_out (NULL: not wanted) and to the cache (of q_type,
+ * LQ_I8 or LQ_U4), the values to the cache.  d_q_out may be d_q, and d_k_out d_k, where types and strides are equal.
+ * H may be 0 (then no queries).  A token of a sequence whose position lies outside [0, positions)
+ * gets NaN for its rotated rows and is not appended; rows of tokens that belong to no sequence are not
+ * written.  Else the rules of lq_paged_kv_append; hd at most 256. */
+int lq_paged_kv_append_rotary(const void* d_q, int64_t ldq, const void* d_k, const void* d_v, int64_t ldkv,
+                              int src_type, int64_t tokens, const int32_t* d_starts, int64_t seqs, int64_t H,
+                              int64_t Hkv, int64_t hd, const float* d_angles, int64_t positions, int64_t rot,
+                              int interleaved, const int32_t* d_table, int64_t table_stride, const int32_t* d_lengths,
+                              void* d_q_out, int64_t ldqo, void* d_k_out, int64_t ldko, int q_type, void* d_k_pages,
+                              void* d_v_pages, int cache_type, void* d_k_scale, void* d_v_scale, int64_t pages,
+                              int64_t page, void* stream);
 /* Attention of one new token per sequence: q [B][H][hd] (rows ldq apart, q_type LQ_F16 or LQ_BF16)
- * against positions 0 .. d_lengths[b] - 1 of the cache (of q_type or LQ_I8); query head h reads
+ * against positions 0 .. d_lengths[b] - 1 of the cache (of q_type, LQ_I8 or LQ_U4); query head h reads
  * key head h / (H / Hkv); softmax(scale q.k) v with float32 scores, statistics and sums; out
  * [B][H][hd] contiguous, of q_type or LQ_F32.  A sequence of length <= 0 has the output 0, one
  * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
@@ -823,8 +864,8 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
  * workgroup takes a whole sequence), no contents kept from call to call. */
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
-                       const void* d_k_pages, const void* d_v_pages, int cache_type, const float* d_k_scale,
-                       const float* d_v_scale, int64_t pages, int64_t page, const int32_t* d_table,
+                       const void* d_k_pages, const void* d_v_pages, int cache_type, const void* d_k_scale,
+                       const void* d_v_scale, int64_t pages, int64_t page, const int32_t* d_table,
                        int64_t table_stride, const int32_t* d_lengths, int64_t max_length, float scale, void* d_out,
                        int out_type, void* d_workspace, size_t workspace_bytes, void* stream);
 /* Attention over packed sequences of different lengths: sequence s has queries d_q_starts[s] ..
@@ -862,6 +903,26 @@ int lq_token_logprobs_backward(const void* d_x, int type, int64_t ldx, int64_t r
                                const int32_t* d_targets, const float* d_lse, const float* d_entropy,
                                const float* d_g_logprobs, const float* d_g_entropy, void* d_grad, int64_t ldg,
                                void* stream);
+/* Verification of drafted tokens: which of them a target model keeps, and the token after them, so that
+ * the tokens are distributed as if the target had drawn each.  Sequence s owns rows d_starts[s] .. d_starts[s + 1] - 1
+ * of the logits [rows][vocab] (ld elements apart, LQ_F32, LQ_F16 or LQ_BF16) and of the other row arrays; each row's
+ * draft d_drafts[r] is the token proposed after its context, the sequence's last row has none (its draft is not
+ * read).  p = e^(x - lse) from the logits and d_lse of lq_token_logprobs, q likewise from d_draft_logits (rows ldd
+ * apart, the same type) and d_draft_lse; both NULL: each draft was certain, q(draft) = 1.  In order, draft r is
+ * kept while accept_u[r] q(draft) < p(draft); a draft outside [0, vocab) is not.  The token after the kept ones
+ * comes from the first row whose draft was not kept, with the weights max(p_j - q_j, 0) (certain drafts: p without the
+ * draft; where no weight is left: p), or from the last row with the weights p: the first j where the sum of the weights
+ * up to j passes sample_u[s] times their sum.  Weights and sums are 64-bit.  Random numbers are in [0, 1).
+ * Out: d_accepted[s], how many drafts were kept; d_tokens[rows]: a sequence's kept drafts, its new token (-1
+ * where its row allows no token or holds NaN), then -1.  A sequence without rows has accepted 0; rows of no
+ * sequence are not written.  Starts never decrease and stay within `rows` (rows past it are neither read nor
+ * written).  Workspace: lq_verify_drafts_workspace_size bytes, 16-byte aligned, no contents kept from
+ * call to call. */
+size_t lq_verify_drafts_workspace_size(int64_t seqs, int64_t vocab);
+int lq_verify_drafts(const void* d_logits, int type, int64_t ld, const float* d_lse, const void* d_draft_logits,
+                     int64_t ldd, const float* d_draft_lse, const int32_t* d_drafts, const int32_t* d_starts,
+                     int64_t seqs, int64_t rows, int64_t vocab, const float* d_accept_u, const float* d_sample_u,
+                     int32_t* d_tokens, int32_t* d_accepted, void* d_workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

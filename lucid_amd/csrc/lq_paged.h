@@ -8,7 +8,6 @@
 #include "lq_place.h"
 
 namespace lq {
-namespace {
 
 // ------------------------------------------------------------------------------ append
 
@@ -21,7 +20,7 @@ struct AppendArgs {
     int64_t table_stride;
     const int32_t* lengths;
     void *kp, *vp;
-    float *ks, *vs;
+    void *ks, *vs;  // float32 of int8 rows, bfloat16 of 4-bit ones
     int64_t pages, page;
 };
 
@@ -80,7 +79,7 @@ struct PagedArgs {
     int64_t ldq;
     int B, H, Hkv, hd, group, qtiles;
     const void *k, *v;
-    const float *ks, *vs;
+    const void *ks, *vs;  // float32 of int8 rows, bfloat16 of 4-bit ones
     int64_t pages;
     int page;
     const int32_t* table;
@@ -133,9 +132,9 @@ struct Piece {
 };
 
 // The line of steps as a workgroup walks it.
-template <int WAVES>
+template <int WAVES, int TILE = PG_K>
 struct Line {
-    static constexpr int STEP = WAVES * PG_K, NT = 64 * WAVES, START = 256 / STEP;
+    static constexpr int STEP = WAVES * TILE, NT = 64 * WAVES, START = 256 / STEP;
     int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
     int64_t base;                    // first step of sequence b
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
@@ -445,5 +444,4 @@ __device__ __forceinline__ int v_swz(int r) {
     return HDP == 64 ? 2 * ((r >> 1) & 3) : HDP % 128 == 0 ? 2 * (r & 7) : 2 * (r & 3);
 }
 
-}  // namespace
 }  // namespace lq

@@ -9,7 +9,8 @@
 #include <hip/hip_fp16.h>
 
 #include "lq_dma.h"
-#include "lq_paged.h"
+#include "lq_paged_u4.h"
+#include "lq_u4.h"
 
 namespace lq {
 namespace {
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(64) void append_i8_any_kernel(AppendArgs a) {
     const RowScale rs(wave_max(top));
     int8_t* dst = static_cast<int8_t*>(is_v ? a.vp : a.kp) + r * a.hd;
     for (int64_t d = threadIdx.x; d < a.hd; d += 64) dst[d] = (int8_t)rs.code(Src::load(src[d]));
-    if (threadIdx.x == 0) (is_v ? a.vs : a.ks)[r] = rs.scale;
+    if (threadIdx.x == 0) static_cast<float*>(is_v ? a.vs : a.ks)[r] = rs.scale;
 }
 
 // LPR lanes per row of hd <= 8 LPR values, eight values a lane; one workgroup per token.
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(256) void append_i8_kernel(AppendArgs a) {
         for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(rs.code(x[j]) & 0xff) << (8 * (j & 3));
         const int64_t r = row + (int64_t)h * a.page;
         *reinterpret_cast<u2v*>(static_cast<int8_t*>(is_v ? a.vp : a.kp) + r * a.hd + d) = u2v{w[0], w[1]};
-        if (d == 0) (is_v ? a.vs : a.ks)[r] = rs.scale;
+        if (d == 0) static_cast<float*>(is_v ? a.vs : a.ks)[r] = rs.scale;
     }
 }
 
@@ -284,8 +285,8 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 
                 const int64_t row = ok ? ((int64_t)id[T] * a.Hkv + w.hk) * a.page + (uint32_t)key % (uint32_t)a.page : 0;
                 const int8_t* kp = static_cast<const int8_t*>(a.k) + row * hd;
                 const int8_t* vp = static_cast<const int8_t*>(a.v) + row * hd;
-                ksc[T] = a.ks[row];
-                vsc[T] = a.vs[row];
+                ksc[T] = static_cast<const float*>(a.ks)[row];
+                vsc[T] = static_cast<const float*>(a.vs)[row];
                 auto load = [&](const int8_t* p, int d) {
                     if constexpr (EXACT) return *reinterpret_cast<const u4v*>(p + d);
                     const u2v lo = *reinterpret_cast<const u2v*>(p + (d < hd ? d : 0));
@@ -470,11 +471,15 @@ extern "C" {
 int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t ld, int64_t tokens,
                        const int32_t* d_starts, int64_t seqs, int64_t Hkv, int64_t hd, const int32_t* d_table,
                        int64_t table_stride, const int32_t* d_lengths, void* d_k_pages, void* d_v_pages,
-                       int cache_type, float* d_k_scale, float* d_v_scale, int64_t pages, int64_t page,
+                       int cache_type, void* d_k_scale, void* d_v_scale, int64_t pages, int64_t page,
                        void* stream) {
     LQ_REQUIRE(is_float_type(src_type), "lq_paged_kv_append: source must be float32, fp16 or bfloat16");
-    LQ_REQUIRE(is_half_type(cache_type) || cache_type == LQ_I8,
-               "lq_paged_kv_append: cache must be fp16, bfloat16 or int8");
+    LQ_REQUIRE(is_half_type(cache_type) || cache_type == LQ_I8 || cache_type == LQ_U4,
+               "lq_paged_kv_append: cache must be fp16, bfloat16, int8 or 4 bits");
+    if (cache_type == LQ_U4)  // the append with rotation, of nothing
+        return paged_append_rotary("lq_paged_kv_append", nullptr, 0, d_k, d_v, ld, src_type, tokens, d_starts, seqs, 0,
+                                   Hkv, hd, nullptr, 0, 0, 0, d_table, table_stride, d_lengths, nullptr, 0, nullptr, 0,
+                                   LQ_F16, d_k_pages, d_v_pages, cache_type, d_k_scale, d_v_scale, pages, page, stream);
     LQ_REQUIRE(tokens >= 0 && seqs >= 0 && Hkv > 0 && hd > 0 && Hkv <= 65535 && hd <= 65535 && ld >= Hkv * hd &&
                    table_stride >= 0 && pages >= 0 && page > 0 && tokens <= 0x7fffffff && seqs <= 0x7fffffff &&
                    table_stride <= 0x7fffffff && pages <= 0x7fffffff && page <= 0x7fffffff,
@@ -518,12 +523,13 @@ size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int6
 }
 
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,
-                       const void* d_k_pages, const void* d_v_pages, int cache_type, const float* d_k_scale,
-                       const float* d_v_scale, int64_t pages, int64_t page, const int32_t* d_table,
+                       const void* d_k_pages, const void* d_v_pages, int cache_type, const void* d_k_scale,
+                       const void* d_v_scale, int64_t pages, int64_t page, const int32_t* d_table,
                        int64_t table_stride, const int32_t* d_lengths, int64_t max_length, float scale, void* d_out,
                        int out_type, void* d_workspace, size_t workspace_bytes, void* stream) {
     LQ_REQUIRE(is_half_type(q_type), "lq_paged_attention: q must be fp16 or bfloat16");
-    LQ_REQUIRE(cache_type == q_type || cache_type == LQ_I8, "lq_paged_attention: the cache must be of q's type or int8");
+    LQ_REQUIRE(cache_type == q_type || cache_type == LQ_I8 || cache_type == LQ_U4,
+               "lq_paged_attention: the cache must be of q's type, int8 or 4 bits");
     LQ_REQUIRE(out_type == q_type || out_type == LQ_F32, "lq_paged_attention: out must be of q's type or float32");
     LQ_REQUIRE(B >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && hd > 0 && ldq >= H * hd && pages >= 0 && page > 0 &&
                    table_stride >= 0 && max_length >= 0 && B <= 65535 && H <= 65535 && table_stride <= 0x7fffffff &&
@@ -531,12 +537,16 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
                "lq_paged_attention: bad shape");
     if (hd % 8 != 0 || hd > ATTN_MAX_HD)
         return set_error(LQ_ERR_UNSUPPORTED, "lq_paged_attention: head dim must be a multiple of 8, 256 at most");
+    if (cache_type == LQ_U4 && hd % U4_GROUP != 0)
+        return set_error(LQ_ERR_UNSUPPORTED, "lq_paged_attention: head dims of a 4-bit cache are multiples of 32");
     LQ_REQUIRE(scale > 0.0f && scale < INFINITY, "lq_paged_attention: scale must be positive and finite");
     if (B == 0) return LQ_OK;
     LQ_REQUIRE(d_q && d_lengths && d_out && (d_table || table_stride == 0) && ((d_k_pages && d_v_pages) || pages == 0),
                "lq_paged_attention: NULL pointer");
-    LQ_REQUIRE(cache_type != LQ_I8 || pages == 0 || (d_k_scale && d_v_scale),
-               "lq_paged_attention: an int8 cache needs scales");
+    LQ_REQUIRE(cache_type == q_type || pages == 0 || (d_k_scale && d_v_scale),
+               "lq_paged_attention: a cache of codes needs scales");
+    LQ_REQUIRE(cache_type != LQ_U4 || (aligned16(d_k_scale) && aligned16(d_v_scale)),
+               "lq_paged_attention: the scales of a 4-bit cache must be 16-byte aligned");
     LQ_REQUIRE(aligned16(d_k_pages) && aligned16(d_v_pages), "lq_paged_attention: pages must be 16-byte aligned");
     const bool alone = max_length <= PG_ALONE;
     LQ_REQUIRE(alone || (d_workspace && aligned16(d_workspace) &&
@@ -554,6 +564,11 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
                       alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
     const dim3 grid = grid_of(alone ? units : groups);
     const hipStream_t st = as_stream(stream);
+    if (cache_type == LQ_U4) {
+        note_path("paged u4");
+        paged_u4_launch(a, q_type, grid, st);
+        return launch_status("lq_paged_attention");
+    }
     // A few short sequences: as many waves each as the LDS holds tiles for, to hide more of the latency (8 sequences
     // of up to 640, 8 heads of 64: 9.4 us a call with four waves, 7.8 with eight); else two, two workgroups to a CU.
     const bool few = alone && units <= 256;

@@ -15,10 +15,17 @@ from lucid_amd.nn.generation import (  # noqa: F401  (part of this module's surf
     paged_attention,
     paged_kv_append,
     paged_kv_append_qkv,
+    paged_kv_append_rotary,
+    paged_kv_append_rotary_qkv,
     prompt_attention,
     prompt_attention_qkv,
+    rms_norm,
+    rms_norm_quantize,
+    rotary_angles,
+    rotary_qkv,
     token_logprobs,
     token_logprobs_backward,
+    verify_drafts,
 )
 from lucid_amd.quantization._device import on_device, require_gpu
 

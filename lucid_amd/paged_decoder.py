@@ -5,9 +5,14 @@
 through its modules: prompts of any lengths enter packed (``F.prompt_attention_qkv``), their
 keys and values go to pages (``F.paged_kv_append_qkv``), every step attends them
 (``F.paged_attention``), ended sequences give their pages back, and ``F.token_logprobs`` gives
-the tokens' scores and alternatives.  :meth:`PagedDecoder.tune` is the training direction: the
-gradient of weighted token scores and entropies in the head's logits
-(``F.token_logprobs_backward``) and in its bias.
+the tokens' scores and alternatives.  :meth:`PagedDecoder.speculate` takes several drafted tokens per
+sequence in one pass and keeps those that the model's distribution allows (``F.verify_drafts``).
+:meth:`PagedDecoder.tune` is the training direction: the gradient of weighted token scores and entropies in
+the head's logits (``F.token_logprobs_backward``) and in its bias.
+
+:class:`RotaryDecoder` serves the same layers as a decoder with root-mean-square norms, whose 8-bit rows
+feed the products (``F.rms_norm_quantize``), and with queries and keys rotated by their positions
+(``F.paged_kv_append_rotary_qkv``), by default over 4-bit pages.
 
 ``python3 -m lucid_amd.paged_decoder [steps]`` serves eight prompts and prints what it took.
 """
@@ -21,6 +26,7 @@ from lucid_amd import _C
 from lucid_amd._tensor import Tensor, empty, float16, float32, tensor
 from lucid_amd.bench_configs import D_MODEL, HEADS
 from lucid_amd.nn.generation import PagedKVCache, PageTable
+from lucid_amd.quantization._gemm import gemm_w8a8
 
 
 def _ints(a) -> Tensor:
@@ -30,7 +36,7 @@ def _ints(a) -> Tensor:
 class PagedDecoder:
     """``qdec`` (``quantize_dynamic`` of the decoder) and its embeddings ``glue``, serving up to
     ``seqs`` sequences at a time from ``pages`` pages of ``page`` positions per layer;
-    ``cache_dtype`` float16 or int8.  One stream: everything runs on the default one."""
+    ``cache_dtype`` float16, int8 or "uint4".  One stream: everything runs on the default one."""
 
     def __init__(self, qdec, glue: dict, seqs: int, pages: int, page: int = 16, cache_dtype=float16) -> None:
         self.qdec = qdec
@@ -67,6 +73,13 @@ class PagedDecoder:
             _C.call("lq_gelu_tanh_f32", up.data_ptr(), up.data_ptr(), up.numel(), None)
             res = layer.down(up)
         return self._norm(x, res)
+
+    def _append(self, i: int, qkv: Tensor, starts: Tensor) -> None:
+        """The keys and values of layer i's rows into its pages."""
+        self.cache[i].append_qkv(qkv, HEADS, starts)
+
+    def _place(self, qkv: Tensor, lengths: Tensor, starts: Tensor) -> None:
+        """Rows that enter no cache, before their attention."""
 
     @staticmethod
     def _rows(x: Tensor, rows: np.ndarray) -> Tensor:
@@ -110,7 +123,7 @@ class PagedDecoder:
         starts = _ints(np.concatenate([[0], ends]))
 
         def attend(i, qkv):
-            self.cache[i].append_qkv(qkv, HEADS, starts)
+            self._append(i, qkv, starts)
             return F.prompt_attention_qkv(qkv, HEADS, HEADS, starts, out_dtype=float32)
 
         try:
@@ -139,7 +152,7 @@ class PagedDecoder:
 
         def attend(i, qkv):
             cache = self.cache[i]
-            cache.append_qkv(qkv, HEADS, starts)
+            self._append(i, qkv, starts)
             if whole:
                 return cache.attend(qkv, out_dtype=float32, heads=HEADS)
             return F.paged_attention(qkv, cache.k, cache.v, table, lengths, self.table.max_length, None, cache.k_scale,
@@ -152,6 +165,61 @@ class PagedDecoder:
         except BaseException:  # the last positions hold nothing
             self.table.shrink(counts)
             raise
+
+    def speculate(self, tokens: dict[int, list], accept_u, sample_u, draft_logits: Tensor | None = None,
+                  draft_lse: Tensor | None = None) -> dict[int, np.ndarray]:
+        """A step of several tokens: ``tokens[s]`` is the token after sequence s and the drafts that follow it.  All
+        of them run in one pass; the drafts that the model's distribution allows are kept and one token more is
+        drawn.  Returns the kept drafts and the new token of each sequence, which then holds its first token and
+        the kept drafts.  In the order of the sequences, ``accept_u`` has a uniform random number for every token
+        and ``sample_u`` one for every sequence; ``draft_logits`` [tokens, vocab] and ``draft_lse`` are the drafting
+        model's, row for row (a row predicts the token after it; a sequence's last row is not read); without
+        them each draft was certain."""
+        seqs = self._sequences(tokens)
+        toks = [np.asarray(tokens[s], np.int64).ravel() for s in seqs]
+        held = self.table.host_lengths()
+        for s, t in zip(seqs, toks):
+            self._known(t, "speculate")
+            if not len(t) or held[s] == 0 or held[s] + len(t) > self.positions:
+                raise ValueError(f"sequence {s} holds {held[s]} positions of {self.positions}; {len(t)} tokens")
+        each = [len(t) for t in toks]
+        rows = sum(each)
+        accept_u, sample_u = (np.ascontiguousarray(u, np.float32).ravel() for u in (accept_u, sample_u))
+        if len(accept_u) != rows or len(sample_u) != len(seqs):
+            raise ValueError(f"{len(accept_u)} and {len(sample_u)} random numbers for {rows} tokens of {len(seqs)} sequences")
+        if not rows:
+            return {}
+        counts = np.zeros(self.table.seqs, np.int64)
+        counts[seqs] = each
+        self.table.grow(counts)
+        try:
+            starts = _ints(np.concatenate([[0], np.cumsum(counts)]))
+            positions = np.concatenate([held[s] + np.arange(n) for s, n in zip(seqs, each)])
+            # a token attends as a sequence of its own that ends with it
+            table, _ = self.table.rows(np.repeat(seqs, each))
+            lengths = _ints(positions + 1)
+
+            def attend(i, qkv):
+                cache = self.cache[i]
+                self._append(i, qkv, starts)
+                return F.paged_attention(qkv, cache.k, cache.v, table, lengths, int(positions.max()) + 1, None,
+                                         cache.k_scale, cache.v_scale, float32, None, HEADS)
+
+            logits = self.qdec.head(self._hidden(np.concatenate(toks), positions, attend))
+            drafts = _ints(np.concatenate([np.append(t[1:], -100) for t in toks]))
+            _, _, lse, _, _ = F.token_logprobs(logits, drafts)
+            out, kept = F.verify_drafts(logits, lse, drafts, _ints(np.cumsum([0] + each)),
+                                        tensor(accept_u, device="gpu"), tensor(sample_u, device="gpu"), draft_logits,
+                                        draft_lse)
+            out, kept = out.numpy(), kept.numpy()
+        except BaseException:  # the new positions hold nothing
+            self.table.shrink(counts)
+            raise
+        drop = np.zeros(self.table.seqs, np.int64)
+        drop[seqs] = np.array(each) - 1 - kept
+        self.table.shrink(drop)
+        ends = np.cumsum([0] + each)
+        return {s: out[ends[j]:ends[j] + kept[j] + 1] for j, s in enumerate(seqs)}
 
     def generate(self, prompts: list, steps: int, top: int = 5):
         """Greedy continuations of up to ``seqs`` prompts: tokens ``[len(prompts), steps]``, their
@@ -181,9 +249,13 @@ class PagedDecoder:
 
     def _score_rows(self, prompts):
         toks = self._check(prompts)
-        starts = _ints(np.cumsum([0] + [len(t) for t in toks]))
-        h = self._hidden(np.concatenate(toks), np.concatenate([np.arange(len(t)) for t in toks]),
-                         lambda i, qkv: F.prompt_attention_qkv(qkv, HEADS, HEADS, starts, out_dtype=float32))
+        starts, lengths = _ints(np.cumsum([0] + [len(t) for t in toks])), _ints([len(t) for t in toks])
+
+        def attend(i, qkv):
+            self._place(qkv, lengths, starts)
+            return F.prompt_attention_qkv(qkv, HEADS, HEADS, starts, out_dtype=float32)
+
+        h = self._hidden(np.concatenate(toks), np.concatenate([np.arange(len(t)) for t in toks]), attend)
         # a row predicts the token after it; the last row of a prompt predicts none
         targets = np.concatenate([np.append(t[1:], -100) if len(t) else t for t in toks])
         return self.qdec.head(h), _ints(targets)
@@ -206,6 +278,45 @@ class PagedDecoder:
         grad = F.token_logprobs_backward(logits, targets, lse, g, ent, ge)
         value = float((weights * lp.numpy()).sum(dtype=np.float64) + entropy_weight * ent.numpy().sum(dtype=np.float64))
         return value, grad, grad.numpy().sum(0, dtype=np.float64)
+
+
+class RotaryDecoder(PagedDecoder):
+    """The layers of ``qdec`` as a decoder with root-mean-square norms and rotated queries and keys, over the token
+    embeddings ``tok`` [vocab, d] alone, for up to ``positions`` positions.  The rows of a norm enter the qkv and up
+    products in 8 bits with a scale each."""
+
+    def __init__(self, qdec, tok: np.ndarray, seqs: int, pages: int, page: int = 16, cache_dtype="uint4",
+                 positions: int = 4096, base: float = 10000.0) -> None:
+        self.qdec, self.tok = qdec, tensor(np.ascontiguousarray(tok), device="gpu")
+        self.vocab, self.positions, self.head_dim = tok.shape[0], positions, D_MODEL // HEADS
+        self.angles = F.rotary_angles(positions, self.head_dim, base)
+        self.table = PageTable(seqs, pages, page, positions)
+        self.cache = [PagedKVCache(self.table, HEADS, self.head_dim, cache_dtype) for _ in qdec.layers]
+
+    @staticmethod
+    def _product(layer, x: Tensor, res: Tensor | None, out_kind: int) -> tuple[Tensor, Tensor]:
+        """The layer's product with the norm of ``x + res``, and that sum."""
+        codes, scales, *total = F.rms_norm_quantize(x, residual=res)
+        layer._device_buffers()
+        y = gemm_w8a8(codes, _C.I8, scales, None, layer._operands(), layer.bias, out_kind)
+        return y, total[0] if total else x
+
+    def _hidden(self, ids: np.ndarray, positions: np.ndarray, attend) -> Tensor:
+        rows, res = len(ids), None
+        x = F.embedding(_ints(ids), self.tok)
+        for i, layer in enumerate(self.qdec.layers):
+            qkv, x = self._product(layer.qkv, x, res, _C.OUT_F16)
+            res = layer.out(attend(i, qkv.reshape(rows, 3 * HEADS, self.head_dim)).reshape(rows, D_MODEL))
+            up, x = self._product(layer.up, x, res, _C.OUT_F32)
+            _C.call("lq_gelu_tanh_f32", up.data_ptr(), up.data_ptr(), up.numel(), None)
+            res = layer.down(up)
+        return F.rms_norm(x, residual=res)[0]
+
+    def _append(self, i: int, qkv: Tensor, starts: Tensor) -> None:
+        self.cache[i].append_rotary_qkv(qkv, HEADS, self.angles, starts)
+
+    def _place(self, qkv: Tensor, lengths: Tensor, starts: Tensor) -> None:
+        F.rotary_qkv(qkv, HEADS, HEADS, self.angles, lengths, starts)
 
 
 def _main(argv: list[str]) -> None:

@@ -81,4 +81,9 @@ __device__ __forceinline__ void lds_copy16(const void* src, uint32_t lds_addr) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
 }
 
+// Four bytes per lane, likewise, at lds_addr + 4 * lane.
+__device__ __forceinline__ void lds_copy4(const void* src, uint32_t lds_addr) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
+}
+
 }  // namespace lq

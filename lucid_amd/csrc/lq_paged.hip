@@ -564,11 +564,6 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
                       alone ? nullptr : part_o + (int64_t)2 * groups * 16 * hd};
     const dim3 grid = grid_of(alone ? units : groups);
     const hipStream_t st = as_stream(stream);
-    if (cache_type == LQ_U4) {
-        note_path("paged u4");
-        paged_u4_launch(a, q_type, grid, st);
-        return launch_status("lq_paged_attention");
-    }
     // A few short sequences: as many waves each as the LDS holds tiles for, to hide more of the latency (8 sequences
     // of up to 640, 8 heads of 64: 9.4 us a call with four waves, 7.8 with eight); else two, two workgroups to a CU.
     const bool few = alone && units <= 256;
@@ -591,7 +586,9 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
         const std::integral_constant<int, 128> w128{};
         const std::integral_constant<int, 192> w192{};
         const std::integral_constant<int, 256> w256{};
-        if (cache_type == LQ_I8) {
+        if (cache_type == LQ_U4) {
+            paged_u4_launch(a, q_type, grid, st);
+        } else if (cache_type == LQ_I8) {
             if (hd == 64) i8(w64, std::true_type{});
             else if (hd == 128) i8(w128, std::true_type{});
             else if (hd < 64) i8(w64, std::false_type{});

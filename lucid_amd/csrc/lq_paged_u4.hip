@@ -20,16 +20,27 @@ constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_WAVES = 4;
 constexpr int U4_NST = 2;     // tiles on their way
 
-// Four registers of eight 16-bit values 16 + c for the codes c of a word; pair p holds codes p and p + 4.  A code
-// under the exponent of 16 is one shift and one and-or for two of them.
-__device__ __forceinline__ u4v widen8(ElemBF16, uint32_t w) {
-    constexpr uint32_t M = 0x00780078u, B = 0x41804180u;
-    return u4v{((w << 3) & M) | B, ((w >> 1) & M) | B, ((w >> 5) & M) | B, ((w >> 9) & M) | B};
-}
-__device__ __forceinline__ u4v widen8(ElemF16, uint32_t w) {
-    constexpr uint32_t M = 0x03c003c0u, B = 0x4c004c00u;
-    return u4v{((w << 6) & M) | B, ((w << 2) & M) | B, ((w >> 2) & M) | B, ((w >> 6) & M) | B};
-}
+// Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
+// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes; where two pairs
+// share a shift, 256 + c for even p (a score of a 16-bit output has room for what that adds to its rounding).
+// An and-or takes no literal, so masks and exponents are kept in registers whose values the compiler does not see.
+template <bool SHARE>
+struct Widen8 {
+    static constexpr float EVEN = SHARE ? 256.0f : 16.0f, ODD = 16.0f;  // what is added to a code
+    uint32_t m0, e0, m1, e1;
+    __device__ __forceinline__ Widen8()
+        : m0(SHARE ? 0x003c003cu : 0x03c003c0u), e0(SHARE ? 0x5c005c00u : 0x4c004c00u), m1(0x03c003c0u), e1(0x4c004c00u) {
+        asm("" : "+v"(m0), "+v"(e0));
+        if (SHARE) asm("" : "+v"(m1), "+v"(e1));
+    }
+    __device__ __forceinline__ u4v operator()(uint32_t w) const {
+        if constexpr (SHARE) {
+            const uint32_t lo = w << 2, hi = w >> 6;
+            return u4v{(lo & m0) | e0, (lo & m1) | e1, (hi & m0) | e0, (hi & m1) | e1};
+        }
+        return u4v{((w << 6) & m0) | e0, ((w << 2) & m0) | e0, ((w >> 2) & m0) | e0, ((w >> 6) & m0) | e0};
+    }
+};
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
@@ -66,55 +77,63 @@ struct Place {
 // (l, g) holds the scores and weights of query l at positions 16 g + 4 T + i: row r of the first product's
 // operand T is position 16 (r / 4) + 4 T + r % 4, and the transposing read brings a lane the codes of its dim at just
 // these 16 positions.
+// Both products are fp16.  Queries of bfloat16 enter times a power of two (their largest value between 2^13 and 2^14:
+// fp16 then holds every bit of values down to 2^-27 of it), which goes into the scores' factor.  A weight enters with its
+// value's scale over the largest power of two among the scales so far, once rounded for a 16-bit output (what
+// one more rounding of the output would cost), as two terms (22 bits) for a float32 one; sums and maximum
+// stay float32.
+// A code c enters as 16 + c or 256 + c.  What that adds to a score is taken off where the biases come in: one
+// instruction more multiplies the row's scales and biases, bfloat16 as they are stored, by minus the queries' sums times
+// what was added and by their sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of
+// that, and 7.5 scales more from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
-// its oldest tile alone.
-template <int G, class Q>
+// the older of two tiles alone.
+// ALL: for a float32 output.
+template <int G, bool ALL, class Q>
 __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel(PagedArgs a) {
-    using P = ElemBF16;
-    constexpr int HD = 32 * G, DT = 2 * G, WAVES = U4_WAVES, NST = U4_NST;
-    constexpr int ROW = 16 * G, CODES = U4_TILE * ROW, KMETA = U4_TILE * 4 * G, VMETA = U4_TILE * 4;
-    constexpr int TILE = 2 * CODES + KMETA + VMETA;
-    constexpr bool WIDE = G % 4 == 0;                 // the scales of keys 16 bytes a lane
-    constexpr int KCOPIES = WIDE ? G / 4 : G, COPIES = 2 * G + KCOPIES + 2;
-    constexpr int IDS = NST * TILE, ROWS = IDS + NST * 256, VBIAS = ROWS + 512, SLOT = VBIAS + 256;
+    using P = ElemF16;
+    using B = ElemBF16;
+    constexpr int HD = 32 * G, DT = 2 * G, WAVES = U4_WAVES, OPS = G <= 4 ? 1 : 2;
+    constexpr int NST = U4_NST, ROW = 16 * G, CODES = U4_TILE * ROW, KMETA = U4_TILE * 4 * G, VMETA = U4_TILE * 4;
+    constexpr int KM = 2 * CODES, VM = KM + KMETA, TILE = VM + VMETA;
+    constexpr int VBIAS = NST * TILE, IDS = VBIAS + VMETA, ROWS = IDS + NST * 256, SLOT = ROWS + 512;
+    constexpr bool WIDE = G % 4 == 0;  // the scales of keys 16 bytes a lane
+    constexpr int KM_COPIES = WIDE ? G / 4 : G, COPIES = 2 * G + KM_COPIES + 2;
     static_assert((NST - 1) * COPIES < 64, "the counter's range");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOT];
     __shared__ float ml[WAVES][2][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // scalar, and what follows from it
     Line<WAVES, U4_TILE> line;
     line.init(a, reinterpret_cast<int64_t*>(lds));
+    const Widen8<!ALL> key_codes;
+    const Widen8<false> value_codes;
     constexpr int STEP = WAVES * U4_TILE;
     const int page = a.page, cols = STEP / page, slots = STEP - cols * page;
     const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
-    const float sl2 = a.scale * LOG2E;
     const char *kp = static_cast<const char*>(a.k), *vp = static_cast<const char*>(a.v);
     const char *kmp = static_cast<const char*>(a.ks), *vmp = static_cast<const char*>(a.vs);
-    auto swz = [](int r) { return (G & (G - 1)) == 0 ? ((r >> 2) ^ (r >> 4)) & (G - 1) : 0; };
+    // chunk c of row r lies at place c ^ swz(r): the 16 rows of a read spread over the banks
+    constexpr bool POW2 = (G & (G - 1)) == 0;
+    auto swz = [](int r) { return POW2 ? ((r >> 2) ^ (r >> 4)) & 3 & (G - 1) : 0; };
+    // where this lane reads: its row of operand T = 0 (T is 4 rows further, its swizzle T ^ that of row 0), and its row
+    // of values
+    const int kr = 16 * (l16 >> 2) + (l16 & 3), vr = 16 * g + l16;
+    uint32_t kat[POW2 ? G : 1], vat[POW2 ? G : 1];
+#pragma unroll
+    for (int x = 0; x < (POW2 ? G : 1); ++x) {
+        kat[x] = kr * ROW + ((POW2 ? x ^ ((l16 >> 2) & (G - 1)) : 0) << 4) + 4 * g;
+        vat[x] = CODES + vr * ROW + ((POW2 ? x ^ swz(vr) : 0) << 4);
+    }
+    auto key_at = [&](int T, int s) { return (POW2 ? kat[(s ^ T) & (G - 1)] : kat[0] + 16 * s) + 4 * T * ROW; };
+    auto value_at = [&](int d) { return (POW2 ? vat[(d >> 1) & (G - 1)] : vat[0] + 16 * (d >> 1)) + 8 * (d & 1); };
     for (Piece w; line.next(a, w);) {
         __syncthreads();  // the plan's numbers are read: their LDS may be filled
-        // queries in the order of the codes' pairs, and the sums of each group
-        u4v qf[G];
-        vf4 start[G];
-        u4v qsum = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < G; ++s) {
-            const u4v q = paged_query(a, w, l16, 32 * s + 8 * g, HD);
-            float sum = 0.0f;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const f2v u = unpack2(Q{}, q[p]);
-                sum += u[0] + u[1];
-            }
-#pragma unroll
-            for (int p = 0; p < 4; ++p)  // halves of words p / 2 and p / 2 + 2
-                qf[s][p] = __builtin_amdgcn_perm(q[2 + (p >> 1)], q[p >> 1], p & 1 ? 0x07060302u : 0x05040100u);
-            sum = quarter_sum(sum);
-            start[s] = vf4{-16.0f * sum, -16.0f * sum, -16.0f * sum, -16.0f * sum};
-            // 24 bits of the sum as three bfloat16 terms, lane group g the g-th: the biases' products in one instruction
-            const float t0 = bf16_bits_to_f32(f32_to_bf16_bits(sum)), t1 = bf16_bits_to_f32(f32_to_bf16_bits(sum - t0));
-            const float term = g == 0 ? t0 : g == 1 ? t1 : g == 2 ? sum - t0 - t1 : 0.0f;
-            qsum[s >> 1] |= (uint32_t)f32_to_bf16_bits(term) << (16 * (s & 1));
-        }
+        // the same in all lanes, but found in vector registers
+        w.b = __builtin_amdgcn_readfirstlane(w.b);
+        w.hk = __builtin_amdgcn_readfirstlane(w.hk);
+        w.begin = __builtin_amdgcn_readfirstlane(w.begin);
+        w.end = __builtin_amdgcn_readfirstlane(w.end);
         const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
         const int first = w.begin + wave * U4_TILE;
         const int tiles = a.pages > 0 && first < w.end ? (w.end - first + STEP - 1) / STEP : 0;
@@ -123,15 +142,21 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.0f, vbias = 0.0f;
-        // this lane's position in the tile that is issued next, and in the one whose page numbers are fetched next
+        int top = 0;  // the largest exponent among the values' scales, as stored
+        // this lane's position in the tile that is issued next, and in the one whose page number is fetched next
         int key = first + lane;
         Place at, ahead;
         at.start((uint32_t)key, (uint32_t)page);
         ahead = at;
         const int last = (int)((uint32_t)(w.end - 1) / (uint32_t)page);  // the last column with a position
+        auto fetch_id = [&](int t) __attribute__((always_inline)) {
+            lds_copy4(table + min(ahead.col, last), slot + IDS + (t % NST) * 256);
+            ahead.advance(cols, slots, page);
+        };
+        // tile t, whose page numbers have come
         auto issue = [&](int t) __attribute__((always_inline)) {
-            const uint32_t to = slot + (t % NST) * TILE, ids = slot + IDS + (t % NST) * 256;
-            const int id = (int)*reinterpret_cast<lds_u32*>(ids + 4 * lane);
+            const uint32_t to = slot + (t % NST) * TILE;
+            const int id = (int)*reinterpret_cast<lds_u32*>(slot + IDS + (t % NST) * 256 + 4 * lane);
             const bool ok = id >= 0 && id < a.pages;
             bad |= key < w.end && !ok;
             // row 0 stands in past the end and for a bad page: its scores and values are dropped
@@ -145,96 +170,164 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
                 lds_copy16(kp + off, to + i * 1024);
                 lds_copy16(vp + off, to + CODES + i * 1024);
             }
-            if constexpr (WIDE) {
 #pragma unroll
-                for (int i = 0; i < KCOPIES; ++i) {
-                    const int r = (64 * i + lane) / KCOPIES, c = (64 * i + lane) % KCOPIES;
-                    const int64_t off = *reinterpret_cast<lds_i64*>(slot + ROWS + 8 * r) * (4 * G) + 16 * c;
-                    lds_copy16(kmp + off, to + 2 * CODES + i * 1024);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < KCOPIES; ++i) {
-                    const int r = (64 * i + lane) / G, c = (64 * i + lane) % G;
-                    const int64_t off = *reinterpret_cast<lds_i64*>(slot + ROWS + 8 * r) * (4 * G) + 4 * c;
-                    lds_copy4(kmp + off, to + 2 * CODES + i * 256);
-                }
+            for (int i = 0; i < KM_COPIES; ++i) {
+                const int r = (64 * i + lane) / KM_COPIES, c = (64 * i + lane) % KM_COPIES;
+                const char* from = kmp + *reinterpret_cast<lds_i64*>(slot + ROWS + 8 * r) * (4 * G);
+                if constexpr (WIDE) lds_copy16(from + 16 * c, to + KM + i * 1024);
+                else lds_copy4(from + 4 * c, to + KM + i * 256);
             }
-            lds_copy4(vmp + row * 4, to + 2 * CODES + KMETA);
-            lds_copy4(table + min(ahead.col, last), ids);  // the tile NST later: this tile's numbers are read
+            lds_copy4(vmp + row * 4, to + VM);
+            fetch_id(t + NST);
             key += STEP;
             at.advance(cols, slots, page);
-            ahead.advance(cols, slots, page);
         };
+        // the first page numbers and the queries are on their way together, then the first tiles while the queries are
+        // laid out
         if (tiles > 0) {
-            // page numbers of the first tiles
 #pragma unroll
-            for (int t = 0; t < NST; ++t) {
-                lds_copy4(table + min(ahead.col, last), slot + IDS + t * 256);
-                ahead.advance(cols, slots, page);
-            }
-            wait_vmcnt<0>();
-            asm volatile("" ::: "memory");
+            for (int t = 0; t < NST; ++t) fetch_id(t);
+        }
+        u4v q[G];
+#pragma unroll
+        for (int s = 0; s < G; ++s) q[s] = paged_query(a, w, l16, 32 * s + 8 * g, HD);
+#pragma unroll
+        for (int s = 0; s < G; ++s) asm volatile("" : "+v"(q[s]));  // loaded here
+        wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+        if (tiles > 0) {
 #pragma unroll
             for (int t = 0; t < NST; ++t)
                 if (t < tiles) issue(t);
         }
+        // queries in the order of the codes' pairs, and the sums of each group
+        float sl2 = a.scale * LOG2E;
+        if constexpr (Q::code == LQ_BF16) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < G; ++s)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) top = max(top, max(q[s][p] & 0x7fffu, (q[s][p] >> 16) & 0x7fffu));
+            const int e = max((int)(__float_as_uint(quarter_max(__uint_as_float(top << 16))) >> 23) - 127, -100);
+            sl2 = ldexpf(sl2, e - 13);
+#pragma unroll
+            for (int s = 0; s < G; ++s)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const f2v u = unpack2(B{}, q[s][p]);
+                    q[s][p] = pack2(P{}, ldexpf(u[0], 13 - e), ldexpf(u[1], 13 - e));
+                }
+        }
+        u4v qf[G], qsum[OPS];
+#pragma unroll
+        for (int i = 0; i < OPS; ++i) qsum[i] = u4v{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+            float even = 0.0f, odd = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const f2v u = unpack2(P{}, q[s][p]);
+                even += u[0];
+                odd += u[1];
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p)  // halves of words p / 2 and p / 2 + 2
+                qf[s][p] = __builtin_amdgcn_perm(q[s][2 + (p >> 1)], q[s][p >> 1], p & 1 ? 0x07060302u : 0x05040100u);
+            even = quarter_sum(even);
+            odd = quarter_sum(odd);
+            // lane group g holds the g-th of three terms of the sum, and of what the codes' offsets add, negative
+            auto term = [&](float x) {
+                const float t0 = unpack2(B{}, pack2(B{}, x, 0.0f))[0], r1 = x - t0;
+                const float t1 = unpack2(B{}, pack2(B{}, r1, 0.0f))[0];
+                return g == 0 ? t0 : g == 1 ? t1 : g == 2 ? r1 - t1 : 0.0f;
+            };
+            const uint32_t both = pack2(B{}, term(even + odd), term(-(Widen8<!ALL>::EVEN * even + Widen8<!ALL>::ODD * odd)));
+            const int at = G <= 4 ? G + s : 8 + s;
+            qsum[0][(s >> 1) & 3] |= s & 1 ? both & 0xffff0000u : both >> 16;      // with the scales
+            qsum[at >> 3][(at >> 1) & 3] |= at & 1 ? both << 16 : both & 0xffffu;  // with the biases
+        }
         for (int t = 0; t < tiles; ++t) {
-            if (tiles - 1 - t == 0) wait_vmcnt<0>();
+            if (t + 1 == tiles) wait_vmcnt<0>();
             else wait_vmcnt<COPIES>();
             static_assert(NST == 2, "the waits above");
             asm volatile("" ::: "memory");
-            const uint32_t kt = slot + (t % NST) * TILE, vt = kt + CODES, km = vt + CODES, vm = km + KMETA;
+            const uint32_t tile = slot + (t % NST) * TILE, meta_at = tile + KM + kr * 4 * G, four_at = tile + 64 * g;
             const int left = w.end - (first + t * STEP);  // positions of this tile that exist
-            // biases of the rows this lane feeds to the matrix cores; the scales as float32, [group][position]
-            u4v kb[4];
-#pragma unroll
-            for (int T = 0; T < 4; ++T) {
-                const uint32_t r = 16 * (l16 >> 2) + 4 * T + (l16 & 3), from = km + r * 4 * G + 2 * G;
-                kb[T] = u4v{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < G; s += 2) {
-                    if constexpr (G % 2 == 0) kb[T][s >> 1] = *reinterpret_cast<lds_u32*>(from + 2 * s);
-                    else
-                        kb[T][s >> 1] = *reinterpret_cast<lds_u16*>(from + 2 * s) |
-                                        (s + 1 < G ? (uint32_t)*reinterpret_cast<lds_u16*>(from + 2 * s + 2) << 16 : 0u);
-                }
-            }
-            float ks[G];
-#pragma unroll
-            for (int s = 0; s < G; ++s)
-                ks[s] = bf16_bits_to_f32(*reinterpret_cast<lds_u16*>(km + lane * 4 * G + 2 * s));
-            const uint32_t vw = *reinterpret_cast<lds_u32*>(vm + 4 * lane);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-            for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(km + 256 * s + 4 * lane) = ks[s];
-            // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are
-            *reinterpret_cast<lds_f32*>(vm + 4 * lane) = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
-            *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) = lane < left ? bf16_bits_to_f32((uint16_t)(vw >> 16)) : 0.0f;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            // scales and biases of the rows this lane feeds to the matrix cores, in their place or in two operands
             vf4 sc[4];
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
-                const int r = 16 * (l16 >> 2) + 4 * T + (l16 & 3);
-                sc[T] = mfma_16x16x32(P{}, kb[T], qsum, vf4{0.f, 0.f, 0.f, 0.f});
+                const uint32_t from = meta_at + 4 * T * 4 * G;
+                sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (G <= 4) {
+                    u4v f = {0, 0, 0, 0};
+                    if constexpr (G == 4) f = *reinterpret_cast<lds_u4v*>(from);
+                    else
+#pragma unroll
+                        for (int i = 0; i < G; ++i) f[i] = *reinterpret_cast<lds_u32*>(from + 4 * i);
+                    sc[T] = mfma_16x16x32(B{}, f, qsum[0], sc[T]);
+                } else {
+#pragma unroll
+                    for (int op = 0; op < 2; ++op) {
+                        u4v f = {0, 0, 0, 0};
+#pragma unroll
+                        for (int s = 0; s < G; ++s)
+                            f[s >> 1] |= (uint32_t)*reinterpret_cast<lds_u16*>(from + 2 * (op * G + s)) << (16 * (s & 1));
+                        sc[T] = mfma_16x16x32(B{}, f, qsum[OPS - 1 ? op : 0], sc[T]);
+                    }
+                }
+            }
+            // the scales and the values' biases as float32, [group][position], over the bytes that every lane has read;
+            // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are 0
+            float ks[G];
+#pragma unroll
+            for (int s = 0; s < G; ++s)
+                ks[s] = bf16_bits_to_f32(*reinterpret_cast<lds_u16*>(tile + KM + lane * 4 * G + 2 * s));
+            const uint32_t vw = *reinterpret_cast<lds_u32*>(tile + VM + 4 * lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
+            const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
+            const int high = __builtin_amdgcn_readfirstlane(wave_max((int)(__float_as_uint(vs) >> 23)));
+            if (high > top) {
+                const float f = __builtin_amdgcn_ldexpf(1.0f, top - high);
+                top = high;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ones[i] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][i] *= f;
+            }
+            *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = __builtin_amdgcn_ldexpf(vs, 127 - top);
+            *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) =
+                lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16))) : 0.0f;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
 #pragma unroll
                 for (int s = 0; s < G; ++s) {
-                    const uint32_t c = *reinterpret_cast<lds_u32*>(kt + r * ROW + ((s ^ swz(r)) << 4) + 4 * g);
-                    const vf4 x = mfma_16x16x32(Q{}, widen8(Q{}, c), qf[s], start[s]);
-                    const vf4 f = *reinterpret_cast<lds_vf4*>(km + 256 * s + 4 * (16 * g + 4 * T));
+                    const uint32_t c = *reinterpret_cast<lds_u32*>(tile + key_at(T, s));
+                    const vf4 x = mfma_16x16x32(P{}, key_codes(c), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
+                    const vf4 f = *reinterpret_cast<lds_vf4*>(four_at + KM + 256 * s + 16 * T);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sc[T][i] = __builtin_fmaf(f[i], x[i], sc[T][i]);
                 }
+            if (left < U4_TILE) {
+#pragma unroll
+                for (int T = 0; T < 4; ++T)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (16 * g + 4 * T + i >= left) sc[T][i] = -INFINITY;
+                        asm volatile("" : "+v"(sc[T][i]));  // in the branch: not sixteen selects for every tile
+                    }
             }
             // weights relative to the running maximum, as the other caches' kernels form them
             float mx = -INFINITY;
 #pragma unroll
             for (int T = 0; T < 4; ++T)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (left < U4_TILE && 16 * g + 4 * T + i >= left) sc[T][i] = -INFINITY;
-                    mx = fmaxf(mx, sc[T][i]);
-                }
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[T][i]);
             mx = quarter_max(mx) * sl2;
             if (__any(mx > m + RESCALE_AT)) {
                 const float mn = fmaxf(m, weight_reference<P>(mx));
@@ -252,8 +345,8 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
             const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<P>;
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
-                const vf4 f = *reinterpret_cast<lds_vf4*>(vm + 4 * (16 * g + 4 * T));
-                const vf4 b = *reinterpret_cast<lds_vf4*>(slot + VBIAS + 4 * (16 * g + 4 * T));
+                const vf4 f = *reinterpret_cast<lds_vf4*>(four_at + VM + 16 * T);
+                const vf4 b = *reinterpret_cast<lds_vf4*>(slot + VBIAS + 64 * g + 16 * T);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -base));
@@ -270,59 +363,40 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
                 for (int p = 0; p < 4; ++p) {
                     const float x = sc[2 * j][p], y = sc[2 * j + 1][p];
                     hi[j][p] = pack2(P{}, x, y);
-                    const f2v u = unpack2(P{}, hi[j][p]);
-                    lo[j][p] = pack2(P{}, x - u[0], y - u[1]);
+                    if constexpr (ALL) {
+                        const f2v u = unpack2(P{}, hi[j][p]);
+                        lo[j][p] = pack2(P{}, x - u[0], y - u[1]);
+                    }
                 }
-            const u4v sixteen = {0x41804180u, 0x41804180u, 0x41804180u, 0x41804180u};
-            const int vr = 16 * g + l16;
-            auto codes = [&](int d) __attribute__((always_inline)) {
-                return lds_read_tr4(vt + vr * ROW + (((d >> 1) ^ swz(vr)) << 4) + 8 * (d & 1));
-            };
+            const u4v offset = {0x4de04de0u, 0x4de04de0u, 0x4de04de0u, 0x4de04de0u};  // 23.5
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                ones = mfma_16x16x32(P{}, sixteen, hi[j], ones);
-                ones = mfma_16x16x32(P{}, sixteen, lo[j], ones);
+                ones = mfma_16x16x32(P{}, offset, hi[j], ones);
+                if constexpr (ALL) ones = mfma_16x16x32(P{}, offset, lo[j], ones);
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const v2i c = codes(d);
+                const v2i c = lds_read_tr4(tile + value_at(d));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const u4v v = widen8(P{}, (uint32_t)c[j]);
+                    const u4v v = value_codes((uint32_t)c[j]);
                     o[d] = mfma_16x16x32(P{}, v, hi[j], o[d]);
-                    o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
-                }
-            }
-            if (a.out_f32) {  // every bit of the weights
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        const f2v u = unpack2(P{}, hi[j][p]), e = unpack2(P{}, lo[j][p]);
-                        hi[j][p] = pack2(P{}, sc[2 * j][p] - u[0] - e[0], sc[2 * j + 1][p] - u[1] - e[1]);
-                    }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) ones = mfma_16x16x32(P{}, sixteen, hi[j], ones);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const v2i c = codes(d);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) o[d] = mfma_16x16x32(P{}, widen8(P{}, (uint32_t)c[j]), hi[j], o[d]);
+                    if constexpr (ALL) o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
             if (t + NST < tiles) issue(t + NST);
         }
         wait_vmcnt<0>();  // page numbers fetched ahead
-        // what all dims of a query share: the sum of its values' biases, less the 16 of every code
-        const float extra = quarter_sum(vbias) - ones[0];
+        // what all dims of a query share: the sum of its values' middles
+        const float extra = quarter_sum(vbias);
         Sums<DT, P> sums;
         sums.m = m;
         sums.l = l;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums.o[d][i] = o[d][i] + extra;
+            for (int i = 0; i < 4; ++i) sums.o[d][i] = __builtin_amdgcn_ldexpf(o[d][i] - ones[0], top - 127) + extra;
         paged_finish<false, WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
     paged_empty<WAVES, Q>(a);
@@ -334,7 +408,9 @@ void paged_u4_launch(const PagedArgs& a, int q_type, dim3 grid, hipStream_t st) 
     with_half(q_type, [&](auto q) {
         using Q = decltype(q);
         auto go = [&](auto groups) {
-            hipLaunchKernelGGL((paged_u4_kernel<decltype(groups)::value, Q>), grid, dim3(64 * U4_WAVES), 0, st, a);
+            constexpr int G = decltype(groups)::value;
+            if (a.out_f32) hipLaunchKernelGGL((paged_u4_kernel<G, true, Q>), grid, dim3(64 * U4_WAVES), 0, st, a);
+            else hipLaunchKernelGGL((paged_u4_kernel<G, false, Q>), grid, dim3(64 * U4_WAVES), 0, st, a);
         };
         switch (a.hd / U4_GROUP) {
         case 1: go(std::integral_constant<int, 1>{}); break;

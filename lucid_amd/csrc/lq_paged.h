@@ -134,7 +134,9 @@ struct Piece {
 // The line of steps as a workgroup walks it.
 template <int WAVES, int TILE = PG_K>
 struct Line {
-    static constexpr int STEP = WAVES * TILE, NT = 64 * WAVES, START = 256 / STEP;
+    static constexpr int STEP = WAVES * TILE, NT = 64 * WAVES;
+    static constexpr int PART = STEP < 256 ? 256 / STEP : 1, PART2 = STEP < 512 ? 512 / STEP : 1;  // 256, 512 positions
+    static constexpr int START = PART;
     int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
     int64_t base;                    // first step of sequence b
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
@@ -169,8 +171,8 @@ struct Line {
         int64_t n256 = 0, n512 = 0;
         for (int i = first; i < last; ++i) {
             sequence(a, i);
-            n256 += (int64_t)heads * ((steps + 256 / STEP - 1) / (256 / STEP));
-            n512 += (int64_t)heads * ((steps + 512 / STEP - 1) / (512 / STEP));
+            n256 += (int64_t)heads * ((steps + PART - 1) / PART);
+            n512 += (int64_t)heads * ((steps + PART2 - 1) / PART2);
         }
         int small = wave_add((int)min(n256, (int64_t)1 << 20)), large = wave_add((int)min(n512, (int64_t)1 << 20));
         if (lane == 0) scan[wave] = (int64_t)small << 32 | large;
@@ -180,7 +182,7 @@ struct Line {
             small += (int)(scan[w] >> 32);
             large += (int)scan[w];
         }
-        unit = small <= a.groups ? 256 / STEP : large <= a.groups ? 512 / STEP : 0;
+        unit = small <= a.groups ? PART : large <= a.groups ? PART2 : 0;
         lead = unit ? 0 : START;
         int64_t mine = 0;
         for (int i = first; i < last; ++i) {

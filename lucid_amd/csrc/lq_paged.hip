@@ -587,7 +587,7 @@ int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int6
         const std::integral_constant<int, 192> w192{};
         const std::integral_constant<int, 256> w256{};
         if (cache_type == LQ_U4) {
-            paged_u4_launch(a, q_type, grid, st);
+            paged_u4_launch(a, q_type, few, grid, st);
         } else if (cache_type == LQ_I8) {
             if (hd == 64) i8(w64, std::true_type{});
             else if (hd == 128) i8(w128, std::true_type{});

@@ -13,7 +13,7 @@ int paged_append_rotary(const char* name, const void* q, int64_t ldq, const void
                         void* k_out, int64_t ldko, int q_type, void* k_pages, void* v_pages, int cache_type,
                         void* k_scale, void* v_scale, int64_t pages, int64_t page, void* stream);
 
-// The kernel of attention over 4-bit pages (lq_paged_u4.hip).
-void paged_u4_launch(const PagedArgs& a, int q_type, dim3 grid, hipStream_t st);
+// The kernel of attention over 4-bit pages (lq_paged_u4.hip); few: a few short sequences, one workgroup each.
+void paged_u4_launch(const PagedArgs& a, int q_type, bool few, dim3 grid, hipStream_t st);
 
 }  // namespace lq

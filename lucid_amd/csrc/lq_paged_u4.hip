@@ -17,7 +17,6 @@ namespace lq {
 namespace {
 
 constexpr int U4_TILE = 64;   // positions of a wave's tile
-constexpr int U4_WAVES = 4;
 constexpr int U4_NST = 2;     // tiles on their way
 
 // Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
@@ -89,11 +88,11 @@ struct Place {
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
 // ALL: for a float32 output.
-template <int G, bool ALL, class Q>
-__global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel(PagedArgs a) {
+template <int G, int WAVES, bool ALL, class Q>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged_u4_kernel(PagedArgs a) {
     using P = ElemF16;
     using B = ElemBF16;
-    constexpr int HD = 32 * G, DT = 2 * G, WAVES = U4_WAVES, OPS = G <= 4 ? 1 : 2;
+    constexpr int HD = 32 * G, DT = 2 * G, OPS = G <= 4 ? 1 : 2;
     constexpr int NST = U4_NST, ROW = 16 * G, CODES = U4_TILE * ROW, KMETA = U4_TILE * 4 * G, VMETA = U4_TILE * 4;
     constexpr int KM = 2 * CODES, VM = KM + KMETA, TILE = VM + VMETA;
     constexpr int VBIAS = NST * TILE, IDS = VBIAS + VMETA, ROWS = IDS + NST * 256, SLOT = ROWS + 512;
@@ -253,38 +252,40 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
             asm volatile("" ::: "memory");
             const uint32_t tile = slot + (t % NST) * TILE, meta_at = tile + KM + kr * 4 * G, four_at = tile + 64 * g;
             const int left = w.end - (first + t * STEP);  // positions of this tile that exist
-            // scales and biases of the rows this lane feeds to the matrix cores, in their place or in two operands
-            vf4 sc[4];
+            // Reads come in batches ahead of their use, and each operand T's products beside the sums of the one
+            // before: left to itself the compiler waits for every read and every product in turn.  A wave's LDS
+            // operations keep their order, so a write needs no wait before the read that follows.
+            u4v meta[4][OPS];  // scales and biases of the rows this lane feeds, in one operand or in two
+            uint32_t code[4][G];
+            float ks[G];
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
                 const uint32_t from = meta_at + 4 * T * 4 * G;
-                sc[T] = vf4{0.f, 0.f, 0.f, 0.f};
-                if constexpr (G <= 4) {
-                    u4v f = {0, 0, 0, 0};
-                    if constexpr (G == 4) f = *reinterpret_cast<lds_u4v*>(from);
-                    else
 #pragma unroll
-                        for (int i = 0; i < G; ++i) f[i] = *reinterpret_cast<lds_u32*>(from + 4 * i);
-                    sc[T] = mfma_16x16x32(B{}, f, qsum[0], sc[T]);
+                for (int i = 0; i < OPS; ++i) meta[T][i] = u4v{0, 0, 0, 0};
+                if constexpr (G == 4) {
+                    meta[T][0] = *reinterpret_cast<lds_u4v*>(from);
+                } else if constexpr (G < 4) {
+#pragma unroll
+                    for (int i = 0; i < G; ++i) meta[T][0][i] = *reinterpret_cast<lds_u32*>(from + 4 * i);
                 } else {
 #pragma unroll
-                    for (int op = 0; op < 2; ++op) {
-                        u4v f = {0, 0, 0, 0};
-#pragma unroll
-                        for (int s = 0; s < G; ++s)
-                            f[s >> 1] |= (uint32_t)*reinterpret_cast<lds_u16*>(from + 2 * (op * G + s)) << (16 * (s & 1));
-                        sc[T] = mfma_16x16x32(B{}, f, qsum[OPS - 1 ? op : 0], sc[T]);
-                    }
+                    for (int i = 0; i < 2 * G; ++i)
+                        meta[T][i / G][(i % G) >> 1] |= (uint32_t)*reinterpret_cast<lds_u16*>(from + 2 * i)
+                                                        << (16 * ((i % G) & 1));
                 }
             }
-            // the scales and the values' biases as float32, [group][position], over the bytes that every lane has read;
-            // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are 0
-            float ks[G];
 #pragma unroll
             for (int s = 0; s < G; ++s)
                 ks[s] = bf16_bits_to_f32(*reinterpret_cast<lds_u16*>(tile + KM + lane * 4 * G + 2 * s));
             const uint32_t vw = *reinterpret_cast<lds_u32*>(tile + VM + 4 * lane);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int s = 0; s < G; ++s) code[T][s] = *reinterpret_cast<lds_u32*>(tile + key_at(T, s));
+            asm volatile("" ::: "memory");
+            // the scales and the values' biases as float32, [group][position], over the bytes that every lane has read;
+            // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are 0
 #pragma unroll
             for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
             const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
@@ -302,17 +303,43 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
             *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = __builtin_amdgcn_ldexpf(vs, 127 - top);
             *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) =
                 lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16))) : 0.0f;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("" ::: "memory");
+            vf4 sc[4], x[2][G], f[2][G];
+            auto factors = [&](int T) __attribute__((always_inline)) {
 #pragma unroll
-            for (int T = 0; T < 4; ++T)
+                for (int s = 0; s < G; ++s) f[T & 1][s] = *reinterpret_cast<lds_vf4*>(four_at + KM + 256 * s + 16 * T);
+            };
+            factors(0);
 #pragma unroll
-                for (int s = 0; s < G; ++s) {
-                    const uint32_t c = *reinterpret_cast<lds_u32*>(tile + key_at(T, s));
-                    const vf4 x = mfma_16x16x32(P{}, key_codes(c), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
-                    const vf4 f = *reinterpret_cast<lds_vf4*>(four_at + KM + 256 * s + 16 * T);
+            for (int T = 0; T < 5; ++T) {
+                if (T < 4) {
+                    sc[T] = mfma_16x16x32(B{}, meta[T][0], qsum[0], vf4{0.f, 0.f, 0.f, 0.f});
+                    if constexpr (OPS == 2) sc[T] = mfma_16x16x32(B{}, meta[T][1], qsum[1], sc[T]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[T][i] = __builtin_fmaf(f[i], x[i], sc[T][i]);
+                    for (int s = 0; s < G; ++s)
+                        x[T & 1][s] = mfma_16x16x32(P{}, key_codes(code[T][s]), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
                 }
+                if (T > 0) {
+#pragma unroll
+                    for (int s = 0; s < G; ++s)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[T - 1][i] = __builtin_fmaf(f[(T - 1) & 1][s][i], x[(T - 1) & 1][s][i], sc[T - 1][i]);
+                }
+                if (T + 1 < 4) factors(T + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // what the values need, read beside the weights
+            v2i vcode[DT];
+            vf4 vf[4], vb[4];
+#pragma unroll
+            for (int T = 0; T < 4; ++T) {
+                vf[T] = *reinterpret_cast<lds_vf4*>(four_at + VM + 16 * T);
+                vb[T] = *reinterpret_cast<lds_vf4*>(slot + VBIAS + 64 * g + 16 * T);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vcode[d] = lds_read_tr4(tile + value_at(d));
+            __builtin_amdgcn_sched_barrier(0);
             if (left < U4_TILE) {
 #pragma unroll
                 for (int T = 0; T < 4; ++T)
@@ -345,14 +372,12 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
             const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<P>;
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
-                const vf4 f = *reinterpret_cast<lds_vf4*>(four_at + VM + 16 * T);
-                const vf4 b = *reinterpret_cast<lds_vf4*>(slot + VBIAS + 64 * g + 16 * T);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -base));
                     l += e;
-                    vbias = __builtin_fmaf(e, b[i], vbias);
-                    sc[T][i] = e * f[i];
+                    vbias = __builtin_fmaf(e, vb[T][i], vbias);
+                    sc[T][i] = e * vf[T][i];
                 }
             }
             // O^T += C^T P^T: word j of a transposed read holds positions 8 j .. of this lane's 16, pairs four apart
@@ -375,15 +400,13 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
                 if constexpr (ALL) ones = mfma_16x16x32(P{}, offset, lo[j], ones);
             }
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const v2i c = lds_read_tr4(tile + value_at(d));
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const u4v v = value_codes((uint32_t)c[j]);
+                for (int d = 0; d < DT; ++d) {
+                    const u4v v = value_codes((uint32_t)vcode[d][j]);
                     o[d] = mfma_16x16x32(P{}, v, hi[j], o[d]);
                     if constexpr (ALL) o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
                 }
-            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
             if (t + NST < tiles) issue(t + NST);
         }
@@ -404,13 +427,20 @@ __global__ __launch_bounds__(64 * U4_WAVES, G <= 4 ? 2 : 1) void paged_u4_kernel
 
 }  // namespace
 
-void paged_u4_launch(const PagedArgs& a, int q_type, dim3 grid, hipStream_t st) {
+void paged_u4_launch(const PagedArgs& a, int q_type, bool few, dim3 grid, hipStream_t st) {
     with_half(q_type, [&](auto q) {
         using Q = decltype(q);
+        auto launch = [&](auto groups, auto waves) {
+            constexpr int G = decltype(groups)::value, W = decltype(waves)::value;
+            if (a.out_f32) hipLaunchKernelGGL((paged_u4_kernel<G, W, true, Q>), grid, dim3(64 * W), 0, st, a);
+            else hipLaunchKernelGGL((paged_u4_kernel<G, W, false, Q>), grid, dim3(64 * W), 0, st, a);
+        };
+        // a few short sequences: eight waves each where the LDS holds their tiles, to hide more of the latency
         auto go = [&](auto groups) {
-            constexpr int G = decltype(groups)::value;
-            if (a.out_f32) hipLaunchKernelGGL((paged_u4_kernel<G, true, Q>), grid, dim3(64 * U4_WAVES), 0, st, a);
-            else hipLaunchKernelGGL((paged_u4_kernel<G, false, Q>), grid, dim3(64 * U4_WAVES), 0, st, a);
+            if constexpr (decltype(groups)::value < 4) {
+                if (few) return launch(groups, std::integral_constant<int, 8>{});
+            }
+            launch(groups, std::integral_constant<int, 4>{});
         };
         switch (a.hd / U4_GROUP) {
         case 1: go(std::integral_constant<int, 1>{}); break;

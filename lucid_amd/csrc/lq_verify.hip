@@ -31,29 +31,39 @@ struct VerifyArgs {
     double2* sums;  // [seqs][runs]: of the weights max(p - q, 0) and of p
 };
 
-// Threads of a workgroup; tokens of a run, which one wave sums (sixteen to a lane) and one workgroup searches.
+// Threads of a workgroup; tokens of a run, which one wave sums and one searches (sixteen to a lane).
 constexpr int VF_T = 256, VF_RUN = 1024;
 
-// e^t for t <= 709, within a few 2^-52: t = k log 2 + r, |r| <= log(2) / 2, Taylor's sum to r^12 (the next term is
-// 2^-52), the high and low part of log 2 taken off in turn.  NaN for NaN.
-__device__ __forceinline__ double exp64(double t) {
-    const double k = __builtin_rint(t * 1.4426950408889634);
-    const double r = __builtin_fma(k, -2.3190468138462996e-17, __builtin_fma(k, -0.6931471805599453, t));
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return t < -746.0 ? 0.0 : ldexp(p, (int)k);
-}
+// e^t within a few 2^-53: t = n log(2) / 64 + r, the high and low part of log(2) / 64 taken off in turn; 2^(n % 64 / 64)
+// from a table in LDS, Taylor's sum of e^r to r^5 (|r| < 0.0055: the next term is 2^-54), 2^(n / 64) as an
+// exponent.  0 below -745 and for NaN.  Coefficients are held in scalar registers whose values the compiler does not see:
+// it would move each into place again for every exponential.
+struct Exp64 {
+    double by, lo, hi, c[4];
+    const double* table;
+    // `t`: 64 numbers of LDS, filled here by the workgroup's first wave; a barrier where there are others
+    __device__ __forceinline__ explicit Exp64(double* t)
+        : by(92.332482616893657), lo(-3.6235106466348430e-19), hi(-0.010830424696249145),
+          c{0.5, 1.0 / 6.0, 1.0 / 24.0, 1.0 / 120.0}, table(t) {
+        asm("" : "+s"(by), "+s"(lo), "+s"(hi));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("" : "+s"(c[i]));
+        if (threadIdx.x < 64) t[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+    }
+    __device__ __forceinline__ double operator()(double t) const {
+        constexpr double SHIFT = 6755399441055744.0;  // 1.5 * 2^52: a sum with it is rounded to whole numbers
+        t = fmax(t, -800.0);
+        const double n = __builtin_fma(t, by, SHIFT), k = n - SHIFT;
+        const double r = __builtin_fma(k, lo, __builtin_fma(k, hi, t));
+        double p = __builtin_fma(c[3], r, c[2]);
+        p = __builtin_fma(p, r, c[1]);
+        p = __builtin_fma(p, r, c[0]);
+        p = __builtin_fma(p, r, 1.0) * r;
+        const int whole = (int)(uint32_t)__builtin_bit_cast(uint64_t, n);
+        const double y = table[whole & 63];
+        return __builtin_amdgcn_ldexp(__builtin_fma(y, p, y), whole >> 6);
+    }
+};
 
 // Eight values from any address (rows of odd lengths).
 template <class E>
@@ -84,13 +94,13 @@ __device__ __forceinline__ void sequence_rows(const VerifyArgs& a, int64_t s, in
 }
 
 template <class E>
-__device__ __forceinline__ double probability(const void* x, int64_t ld, const float* lse, int64_t row, int64_t j) {
-    return exp64((double)E::load(static_cast<const typename E::T*>(x)[row * ld + j]) - (double)lse[row]);
+__device__ __forceinline__ double log_probability(const void* x, int64_t ld, const float* lse, int64_t row, int64_t j) {
+    return (double)E::load(static_cast<const typename E::T*>(x)[row * ld + j]) - (double)lse[row];
 }
 
 // How many of a sequence's drafts are kept; every thread of a wave calls it, 64 drafts at a time.
 template <class E>
-__device__ __forceinline__ int64_t kept(const VerifyArgs& a, int64_t first, int64_t drafts) {
+__device__ __forceinline__ int64_t kept(const Exp64& e, const VerifyArgs& a, int64_t first, int64_t drafts) {
     const int lane = threadIdx.x & 63;
     for (int64_t i = 0; i < drafts; i += 64) {
         bool fails = false;
@@ -99,8 +109,9 @@ __device__ __forceinline__ int64_t kept(const VerifyArgs& a, int64_t first, int6
             const int32_t t = a.drafts[r];
             fails = true;
             if (t >= 0 && t < a.vocab) {
-                const double q = a.d ? probability<E>(a.d, a.ldd, a.dlse, r, t) : 1.0;
-                fails = !((double)a.accept[r] * q < probability<E>(a.x, a.ld, a.lse, r, t));
+                const double q = a.d ? log_probability<E>(a.d, a.ldd, a.dlse, r, t) : 0.0;
+                const double p = log_probability<E>(a.x, a.ld, a.lse, r, t);
+                fails = !(q == q && (double)a.accept[r] * e(q) < e(p));
             }
         }
         const uint64_t m = __ballot(fails);
@@ -112,13 +123,14 @@ __device__ __forceinline__ int64_t kept(const VerifyArgs& a, int64_t first, int6
 // The weights of eight tokens from j on in a row: of what is left of p, and p.  Past the vocabulary both are 0.
 template <class E>
 struct Weights {
+    const Exp64& exp;
     const typename E::T *x, *d;
     double lse, dlse;
     int vocab;
     bool rejected;
     int32_t draft;
-    __device__ __forceinline__ Weights(const VerifyArgs& a, int64_t row, bool rejected)
-        : x(static_cast<const typename E::T*>(a.x) + row * a.ld),
+    __device__ __forceinline__ Weights(const Exp64& exp, const VerifyArgs& a, int64_t row, bool rejected)
+        : exp(exp), x(static_cast<const typename E::T*>(a.x) + row * a.ld),
           d(rejected && a.d ? static_cast<const typename E::T*>(a.d) + row * a.ldd : nullptr), lse((double)a.lse[row]),
           dlse(rejected && a.d ? (double)a.dlse[row] : 0.0), vocab(a.vocab), rejected(rejected),
           draft(rejected ? a.drafts[row] : -1) {}
@@ -140,18 +152,15 @@ struct Weights {
                     if (d) v[i] = E::load(d[j + i]);
                 }
         }
+        double p[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const double p = j + i < vocab ? exp64((double)u[i] - lse) : 0.0;
-            double r = 0.0;
-            if (rejected) {
-                if (!d) r = j + i == draft ? 0.0 : p;
-                else {
-                    const double e = p - exp64((double)v[i] - dlse);
-                    r = e > 0.0 ? e : 0.0;
-                }
-            }
-            w[i] = make_double2(r, p);
+        for (int i = 0; i < N; ++i) p[i] = exp((double)u[i] - lse);  // -inf past the vocabulary: 0
+        if (d) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = make_double2(fmax(p[i] - exp((double)v[i] - dlse), 0.0), p[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = make_double2(rejected && j + i != draft ? p[i] : 0.0, p[i]);
         }
     }
 };
@@ -165,16 +174,19 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // One wave per run.  verify_b64 (64 rows of 100003, twice): FIGURE
 template <class E>
 __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
+    __shared__ double table[64];
+    const Exp64 e(table);
+    __syncthreads();
     const int64_t groups = (a.runs + VF_T / 64 - 1) / (VF_T / 64), n = workgroup(), s = n / groups;
     if (s >= a.seqs) return;
     const int lane = threadIdx.x & 63;
     const int run = __builtin_amdgcn_readfirstlane((int)(n - s * groups) * (VF_T / 64) + (threadIdx.x >> 6));
     int64_t first, rows;
     sequence_rows(a, s, first, rows);
-    const int64_t keep = rows > 0 ? kept<E>(a, first, rows - 1) : 0;
+    const int64_t keep = rows > 0 ? kept<E>(e, a, first, rows - 1) : 0;
     if (run == 0 && lane == 0) a.accepted[s] = (int32_t)keep;
     if (rows == 0 || run >= a.runs) return;
-    const Weights<E> w(a, first + keep, keep < rows - 1);
+    const Weights<E> w(e, a, first + keep, keep < rows - 1);
     double2 sum = make_double2(0.0, 0.0);
 #pragma unroll
     for (int i = 0; i < VF_RUN; i += 512) {
@@ -191,111 +203,98 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
     if (lane == 0) a.sums[s * a.runs + run] = sum;
 }
 
-// The inclusive sums over the workgroup's threads of one number each, and the sum of all.
-__device__ __forceinline__ double block_scan(double mine, double* scan, double& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double upto = mine;
+// The sum of the lanes up to this one, and of all.
+__device__ __forceinline__ double wave_scan64(double v, double& total) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += o;
+        const double o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
     }
-    __syncthreads();
-    if (lane == 63) scan[wave] = upto;
-    __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-#pragma unroll
-    for (int w = 0; w < VF_T / 64; ++w) {
-        if (w < wave) before += scan[w];
-        total += scan[w];
-    }
-    return before + upto;
+    total = __shfl(v, 63, 64);
+    return v;
 }
 
-// The smallest of the threads' candidates, or where none has one (n) the largest of `last`.
-__device__ __forceinline__ int first_of(int found, int n, int last, int* best) {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        best[0] = n;
-        best[1] = -1;
-    }
-    __syncthreads();
-    if (found < n) atomicMin(&best[0], found);
-    if (last >= 0) atomicMax(&best[1], last);
-    __syncthreads();
-    return best[0] < n ? best[0] : best[1];
-}
-
-// A workgroup per sequence.  Where rounding leaves no sum above the border, the last token with a weight is taken.
+// A wave per sequence, without a barrier: the run that holds the border, then the token in it.  Where rounding leaves
+// no sum above the border, the last token with a weight is taken.
 template <class E>
-__global__ __launch_bounds__(VF_T) void verify_token_kernel(VerifyArgs a) {
-    __shared__ double scan[VF_T / 64], before;
-    __shared__ int best[2];
+__global__ __launch_bounds__(64) void verify_token_kernel(VerifyArgs a) {
+    __shared__ double table[64];
+    const Exp64 e(table);
+    __syncthreads();
     const int64_t s = workgroup();
     if (s >= a.seqs) return;
-    const int tid = threadIdx.x;
+    const int lane = threadIdx.x;
     int64_t first, rows;
     sequence_rows(a, s, first, rows);
     if (rows == 0) return;
-    const int64_t keep = a.accepted[s];
-    const Weights<E> w(a, first + keep, keep < rows - 1);
     const double u = (double)a.sample[s];
+    const int64_t keep = a.accepted[s];
     const double2* sums = a.sums + s * a.runs;
-    // runs lo .. hi - 1 are this thread's
-    const int per = (a.runs + VF_T - 1) / VF_T, lo = min(tid * per, a.runs), hi = min(lo + per, a.runs);
+    // runs lo .. hi - 1 are this lane's
+    const int per = (a.runs + 63) / 64, lo = min(lane * per, a.runs), hi = min(lo + per, a.runs);
     double2 mine = make_double2(0.0, 0.0), total;
+#pragma unroll 4
     for (int i = lo; i < hi; ++i) {
         const double2 v = sums[i];
         mine.x += v.x;
         mine.y += v.y;
     }
-    const double upto_x = block_scan(mine.x, scan, total.x), upto_y = block_scan(mine.y, scan, total.y);
+    const Weights<E> w(e, a, first + keep, keep < rows - 1);
+    const double upto_x = wave_scan64(mine.x, total.x), upto_y = wave_scan64(mine.y, total.y);
     const bool rest = total.x > 0.0;
     const double all = rest ? total.x : total.y, at = u * all;
     int token = -1;
     if (all > 0.0 && all < INFINITY) {
-        double run = rest ? upto_x - mine.x : upto_y - mine.y, at_found = 0.0;
-        int found = a.runs, last = -1;
+        double upto = rest ? upto_x - mine.x : upto_y - mine.y, before = 0.0;
+        int found = -1, last = -1;
+#pragma unroll 4
         for (int i = lo; i < hi; ++i) {
             const double v = rest ? sums[i].x : sums[i].y;
             if (v > 0.0) {
                 last = i;
-                if (found == a.runs && run + v > at) {
+                if (found < 0 && upto + v > at) {
                     found = i;
-                    at_found = run;
+                    before = upto;
                 }
             }
-            run += v;
+            upto += v;
         }
-        const int part = first_of(found, a.runs, last, best);
-        if (found == part) before = at_found;
-        else if (last == part) before = -1.0;  // no border: every weight passes it, and the last one is taken
-        __syncthreads();
-        if (part >= 0) {
-            const bool none = before < 0.0;
-            const int j0 = part * VF_RUN;
-            constexpr int EACH = VF_RUN / VF_T;
-            double2 v[EACH];
-            w(j0 + EACH * tid, v);
-            double sum = 0.0, all_of_it;
+        uint64_t m = __ballot(found >= 0);
+        const bool border = m != 0;
+        if (!border) m = __ballot(last >= 0);  // one has, as the total is positive
+        const int owner = border ? __builtin_ctzll(m) : 63 - __builtin_clzll(m);
+        const int run = __shfl(border ? found : last, owner, 64);
+        before = __shfl(before, owner, 64);
+        constexpr int EACH = VF_RUN / 64;
+        double v[EACH], sum = 0.0, all_of_it;
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) sum += rest ? v[i].x : v[i].y;
-            double upto = block_scan(sum, scan, all_of_it) - sum + (none ? 0.0 : before);
-            int pick = VF_RUN, tail = -1;
+        for (int i = 0; i < EACH; i += 8) {
+            double2 x[8];
+            w(run * VF_RUN + EACH * lane + i, x);
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                const double x = rest ? v[i].x : v[i].y;
-                if (x > 0.0) {
-                    tail = EACH * tid + i;
-                    if (!none && pick == VF_RUN && upto + x > at) pick = tail;
-                }
-                upto += x;
+            for (int k = 0; k < 8; ++k) {
+                v[i + k] = rest ? x[k].x : x[k].y;
+                sum += v[i + k];
             }
-            token = j0 + first_of(pick, VF_RUN, tail, best);
         }
+        upto = wave_scan64(sum, all_of_it) - sum + before;
+        found = last = -1;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (v[i] > 0.0) {
+                last = EACH * lane + i;
+                if (found < 0 && border && upto + v[i] > at) found = last;
+            }
+            upto += v[i];
+        }
+        m = __ballot(found >= 0);
+        const bool there = m != 0;
+        if (!there) m = __ballot(last >= 0);
+        // a run is taken for its positive sum, so that some lane of it has a weight
+        if (m) token = run * VF_RUN + __shfl(there ? found : last, there ? __builtin_ctzll(m) : 63 - __builtin_clzll(m), 64);
     }
-    for (int64_t i = tid; i < rows; i += VF_T)
+    for (int64_t i = lane; i < rows; i += 64)
         a.tokens[first + i] = i < keep ? a.drafts[first + i] : i == keep ? token : -1;
 }
 
@@ -334,7 +333,7 @@ int lq_verify_drafts(const void* d_logits, int type, int64_t ld, const float* d_
     with_float(type, [&](auto e) {
         using E = decltype(e);
         hipLaunchKernelGGL((verify_sums_kernel<E>), grid_of(seqs * ((runs + VF_T / 64 - 1) / (VF_T / 64))), dim3(VF_T), 0, st, a);
-        hipLaunchKernelGGL((verify_token_kernel<E>), grid_of(seqs), dim3(VF_T), 0, st, a);
+        hipLaunchKernelGGL((verify_token_kernel<E>), grid_of(seqs), dim3(64), 0, st, a);
     });
     return launch_status("lq_verify_drafts");
 }

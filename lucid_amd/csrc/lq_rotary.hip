@@ -123,17 +123,68 @@ __global__ __launch_bounds__(64) void rotary_any_kernel(RotaryArgs r) {
     for (int d = rot + lane; d < hd; d += 64) y[d] = Out::store(k.turned ? Src::load(x[d]) : nan);
 }
 
-// A workgroup per token, lpr lanes (8, 16 or 32) to a row of hd <= 8 lpr values, eight values a lane.  A lane keeps its
-// place in the row for every head, so the angles of its dims are loaded once.
-template <class Src, class Out, class Cache>
-__global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
-    const int64_t t = workgroup();
+// Eight source values as they lie in memory.
+template <class Src>
+struct Raw8 {
+    static constexpr int N = Src::code == LQ_F32 ? 8 : 4;
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const typename Src::T* p) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u4v v = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(p) + i / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i + j] = v[j];
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+        if constexpr (Src::code == LQ_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f2v u = unpack2(Src{}, w[j]);
+                x[2 * j] = u[0];
+                x[2 * j + 1] = u[1];
+            }
+        }
+    }
+    __device__ __forceinline__ Raw8 of_lane_xor(int m) const {
+        Raw8 r;
+#pragma unroll
+        for (int j = 0; j < N; ++j) r.w[j] = (uint32_t)__shfl_xor((int)w[j], m, 64);
+        return r;
+    }
+};
+
+// A workgroup takes AHEAD rows of a token a lane, lpr lanes (8, 16 or 32) to a row of hd <= 8 lpr values, eight values
+// a lane.  A lane keeps its place in the row for every head, so the angles of its dims are loaded once.  The values are on
+// their way before the token's place is looked up (a search, two numbers, a page number and the angles, each
+// after the other).  swap: the lane whose place holds the partners differs by this bit; 0: the partners are loaded.
+// Rows of a call from which a lane takes four: the loads of one hide nothing of the places' latency.
+constexpr int RT_T = 64;
+constexpr int64_t RT_ROWS = 1 << 16;
+template <int AHEAD, class Src, class Out, class Cache>
+__global__ __launch_bounds__(RT_T) void rotary_kernel(RotaryArgs r, int lpr, int swap, uint32_t groups) {
+    const int64_t n = workgroup(), t = n / groups;
     if (t >= r.a.tokens) return;
-    Token k;
-    if (!find_token(r, t, k)) return;
     const int hd = (int)r.a.hd, half = r.rot / 2, Hkv = (int)r.a.Hkv, heads = r.H + 2 * Hkv;
     const int d = (threadIdx.x & (lpr - 1)) * 8;
     const int other = r.interleaved || d >= r.rot ? d : d < half ? d + half : d - half;  // the partners' dims
+    auto kind_of = [&](int e) { return e < r.H ? ROW_Q : e < r.H + Hkv ? ROW_K : ROW_V; };
+    auto head_of = [&](int e) { return e < r.H ? e : e < r.H + Hkv ? e - r.H : e - r.H - Hkv; };
+    // rows e0 + i * round; those past the last are nobody's, but take part in the exchanges
+    const int round = blockDim.x / lpr, e0 = (int)(n - t * groups) * AHEAD * round + threadIdx.x / lpr;
+    Raw8<Src> raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int e = e0 + i * round;
+#pragma unroll
+        for (int j = 0; j < Raw8<Src>::N; ++j) raw[i].w[j] = 0;
+        if (e < heads && d < hd) raw[i].load(source_row<Src>(r, t, kind_of(e), head_of(e)) + d);
+    }
+    Token k;
+    if (!find_token(r, t, k)) return;
     float c[8], s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -163,28 +214,25 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
             }
         }
     }
-    // every lane of a wave takes the same number of rounds: the exchanges below need them all
-    const int per = 64 / lpr, rounded = (heads + per - 1) / per * per, round = blockDim.x / lpr;
-    for (int e = threadIdx.x / lpr; e < rounded; e += round) {
-        const int kind = e < r.H ? ROW_Q : e < r.H + Hkv ? ROW_K : ROW_V;
-        const int h = kind == ROW_Q ? e : kind == ROW_K ? e - r.H : e - r.H - Hkv;
+    auto row_of = [&](int e, const Raw8<Src>& in) __attribute__((always_inline)) {
+        const int kind = kind_of(e), h = head_of(e);
         const bool mine = e < heads && d < hd;
-        float x[8] = {};
-        if (mine) {
-            const typename Src::T* src = source_row<Src>(r, t, kind, h);
-            load8<Src>(src + d, x);
-            if (kind != ROW_V && d < r.rot) {
-                float y[8];
-                if (r.interleaved) {
+        float x[8], y[8];
+        in.unpack(x);
+        if (r.interleaved) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
-                } else {
-                    load8<Src>(src + other, y);
-                }
-                // a c - b s, and b c + a s: the sign is in s
+            for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+        } else if (swap) {
+            in.of_lane_xor(swap).unpack(y);
+        } else if (mine && kind != ROW_V) {
+            Raw8<Src> p;
+            p.load(source_row<Src>(r, t, kind, h) + other);
+            p.unpack(y);
+        }
+        // a c - b s, and b c + a s: the sign is in s
+        if (kind != ROW_V && d < r.rot) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = x[j] * c[j] + y[j] * s[j];
-            }
+            for (int j = 0; j < 8; ++j) x[j] = x[j] * c[j] + y[j] * s[j];
         }
         if (mine && kind != ROW_V) {
             void* out = kind == ROW_Q ? r.qo : r.ko;
@@ -195,7 +243,7 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     o[j] = pack2(Out{}, k.turned ? x[2 * j] : nan, k.turned ? x[2 * j + 1] : nan);
-                *reinterpret_cast<u4v*>(static_cast<typename Out::T*>(out) + at) = o;
+                __builtin_nontemporal_store(o, reinterpret_cast<u4v*>(static_cast<typename Out::T*>(out) + at));
             }
         }
         const bool keep = mine && kind != ROW_Q && k.row >= 0;
@@ -203,11 +251,13 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
         void* pages = kind == ROW_K ? r.a.kp : r.a.vp;
         if constexpr (std::is_same_v<Cache, ElemI8>) {
             int32_t top = 0;
+            if (mine) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[j]));
+                for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[j]));
+            }
             for (int off = lpr / 2; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
             const RowScale rs(top);
-            if (!keep) continue;
+            if (!keep) return;
             u2v w = {0, 0};
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(rs.code(x[j]) & 0xff) << (8 * (j & 3));
@@ -230,7 +280,7 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
                     hi = fmaxf(hi, oh);
                 }
             }
-            if (!keep) continue;
+            if (!keep) return;
             const Group4 q(lo, hi);
             uint32_t w = 0;
 #pragma unroll
@@ -244,13 +294,15 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotaryArgs r, int lpr) {
                 meta[groups] = f32_to_bf16_bits(q.bias);
             }
         } else {
-            if (!keep) continue;
+            if (!keep) return;
             u4v o;
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] = pack2(Cache{}, x[2 * j], x[2 * j + 1]);
             *reinterpret_cast<u4v*>(static_cast<typename Cache::T*>(pages) + row * hd + d) = o;
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) row_of(e0 + i * round, raw[i]);
 }
 
 }  // namespace
@@ -303,23 +355,27 @@ int paged_append_rotary(const char* name, const void* q, int64_t ldq, const void
     const bool vec = hd % 8 == 0 && rot % (interleaved ? 8 : 16) == 0 && (ends & 15) == 0 && (strides & 15) == 0;
     const int64_t heads = H + 2 * Hkv;
     const int lpr = hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
+    const int64_t apart = rot / 16;  // lanes between partners: an exchange where that is a power of two
+    const int swap = !interleaved && rot > 0 && (apart & (apart - 1)) == 0 ? (int)apart : 0;
     note_path(vec ? "rotary" : "rotary single");
     with_float(src_type, [&](auto s) {
         using S = decltype(s);
         with_half(q_type, [&](auto o) {
             using O = decltype(o);
-            auto go = [&](auto vk, auto ak) {
-                if (vec) {
-                    const int64_t threads = heads * lpr;
-                    const unsigned block = threads >= 512 ? 512 : (unsigned)((threads + 63) / 64 * 64);
-                    hipLaunchKernelGGL(vk, grid_of(tokens), dim3(block), 0, st, r, lpr);
-                } else {
+            auto go = [&](auto one, auto four, auto ak) {
+                if (!vec) {
                     hipLaunchKernelGGL(ak, grid_of(tokens * heads), dim3(64), 0, st, r);
+                    return;
                 }
+                const bool few = tokens * heads < RT_ROWS;
+                const int64_t each = RT_T / lpr * (few ? 1 : 4), groups = (heads + each - 1) / each;
+                const dim3 grid = grid_of(tokens * groups);
+                if (few) hipLaunchKernelGGL(one, grid, dim3(RT_T), 0, st, r, lpr, swap, (uint32_t)groups);
+                else hipLaunchKernelGGL(four, grid, dim3(RT_T), 0, st, r, lpr, swap, (uint32_t)groups);
             };
-            if (cache_type == LQ_I8) go(rotary_kernel<S, O, ElemI8>, rotary_any_kernel<S, O, ElemI8>);
-            else if (cache_type == LQ_U4) go(rotary_kernel<S, O, void>, rotary_any_kernel<S, O, void>);
-            else go(rotary_kernel<S, O, O>, rotary_any_kernel<S, O, O>);
+            if (cache_type == LQ_I8) go(rotary_kernel<1, S, O, ElemI8>, rotary_kernel<4, S, O, ElemI8>, rotary_any_kernel<S, O, ElemI8>);
+            else if (cache_type == LQ_U4) go(rotary_kernel<1, S, O, void>, rotary_kernel<4, S, O, void>, rotary_any_kernel<S, O, void>);
+            else go(rotary_kernel<1, S, O, O>, rotary_kernel<4, S, O, O>, rotary_any_kernel<S, O, O>);
         });
     });
     return launch_status(name);

@@ -81,6 +81,15 @@ __device__ __forceinline__ void lds_copy16(const void* src, uint32_t lds_addr) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");
 }
 
+// The same from a scalar base and a lane's 32-bit offset.  The wait covers a base that a vector instruction made
+// (v_readfirstlane, v_readlane), as in lds_dma16_fresh, and M0.
+__device__ __forceinline__ void lds_copy16_from(const void* base, uint32_t off, uint32_t lds_addr) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+}
+__device__ __forceinline__ void lds_copy4_from(const void* base, uint32_t off, uint32_t lds_addr) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1 nt" : : "v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+}
+
 // Four bytes per lane, likewise, at lds_addr + 4 * lane.
 __device__ __forceinline__ void lds_copy4(const void* src, uint32_t lds_addr) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off nt" : : "v"(src), "{m0}"(lds_addr) : "memory");

@@ -88,7 +88,8 @@ struct Place {
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
 // ALL: for a float32 output.
-template <int G, int WAVES, bool ALL, class Q>
+// ALIGNED: pages of whole tiles: a tile lies in one page, its addresses are a scalar and a constant of the lane.
+template <int G, int WAVES, bool ALL, bool ALIGNED, class Q>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged_u4_kernel(PagedArgs a) {
     using P = ElemF16;
     using B = ElemBF16;
@@ -126,6 +127,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
     }
     auto key_at = [&](int T, int s) { return (POW2 ? kat[(s ^ T) & (G - 1)] : kat[0] + 16 * s) + 4 * T * ROW; };
     auto value_at = [&](int d) { return (POW2 ? vat[(d >> 1) & (G - 1)] : vat[0] + 16 * (d >> 1)) + 8 * (d & 1); };
+    uint32_t tile_off[G];  // of the chunk that this lane copies, in a tile of consecutive rows
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        const int r = (64 * i + lane) / G, c = ((64 * i + lane) % G) ^ swz(r);
+        tile_off[i] = r * ROW + 16 * c;
+    }
     for (Piece w; line.next(a, w);) {
         __syncthreads();  // the plan's numbers are read: their LDS may be filled
         // the same in all lanes, but found in vector registers
@@ -145,20 +152,42 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         // this lane's position in the tile that is issued next, and in the one whose page number is fetched next
         int key = first + lane;
         Place at, ahead;
-        at.start((uint32_t)key, (uint32_t)page);
+        at.start((uint32_t)(ALIGNED ? first : key), (uint32_t)page);
         ahead = at;
         const int last = (int)((uint32_t)(w.end - 1) / (uint32_t)page);  // the last column with a position
         auto fetch_id = [&](int t) __attribute__((always_inline)) {
             lds_copy4(table + min(ahead.col, last), slot + IDS + (t % NST) * 256);
             ahead.advance(cols, slots, page);
         };
-        // tile t, whose page numbers have come
+        // tile t, whose page numbers have come; row 0 stands in past the end and for a bad page: its scores and values
+        // are dropped
         auto issue = [&](int t) __attribute__((always_inline)) {
             const uint32_t to = slot + (t % NST) * TILE;
             const int id = (int)*reinterpret_cast<lds_u32*>(slot + IDS + (t % NST) * 256 + 4 * lane);
+            if constexpr (ALIGNED) {
+                const int one = __builtin_amdgcn_readfirstlane(id);
+                const bool ok = one >= 0 && one < a.pages;
+                bad |= !ok;
+                const int64_t row =
+                    ok ? ((int64_t)one * a.Hkv + w.hk) * page + __builtin_amdgcn_readfirstlane(at.slot) : 0;
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    lds_copy16_from(kp + row * ROW, tile_off[i], to + i * 1024);
+                    lds_copy16_from(vp + row * ROW, tile_off[i], to + CODES + i * 1024);
+                }
+#pragma unroll
+                for (int i = 0; i < KM_COPIES; ++i) {
+                    if constexpr (WIDE)
+                        lds_copy16_from(kmp + row * (4 * G) + i * 1024, 16 * lane, to + KM + i * 1024);
+                    else lds_copy4_from(kmp + row * (4 * G) + i * 256, 4 * lane, to + KM + i * 256);
+                }
+                lds_copy4_from(vmp + row * 4, 4 * lane, to + VM);
+                fetch_id(t + NST);
+                at.advance(cols, slots, page);
+                return;
+            }
             const bool ok = id >= 0 && id < a.pages;
             bad |= key < w.end && !ok;
-            // row 0 stands in past the end and for a bad page: its scores and values are dropped
             const int64_t row = key < w.end && ok ? ((int64_t)id * a.Hkv + w.hk) * page + at.slot : 0;
             *reinterpret_cast<lds_i64*>(slot + ROWS + 8 * lane) = row;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -432,8 +461,15 @@ void paged_u4_launch(const PagedArgs& a, int q_type, bool few, dim3 grid, hipStr
         using Q = decltype(q);
         auto launch = [&](auto groups, auto waves) {
             constexpr int G = decltype(groups)::value, W = decltype(waves)::value;
-            if (a.out_f32) hipLaunchKernelGGL((paged_u4_kernel<G, W, true, Q>), grid, dim3(64 * W), 0, st, a);
-            else hipLaunchKernelGGL((paged_u4_kernel<G, W, false, Q>), grid, dim3(64 * W), 0, st, a);
+            auto all = [&](auto every) {
+                constexpr bool ALL = decltype(every)::value;
+                if (a.page % U4_TILE == 0)
+                    hipLaunchKernelGGL((paged_u4_kernel<G, W, ALL, true, Q>), grid, dim3(64 * W), 0, st, a);
+                else
+                    hipLaunchKernelGGL((paged_u4_kernel<G, W, ALL, false, Q>), grid, dim3(64 * W), 0, st, a);
+            };
+            if (a.out_f32) all(std::true_type{});
+            else all(std::false_type{});
         };
         // a few short sequences: eight waves each where the LDS holds their tiles, to hide more of the latency
         auto go = [&](auto groups) {

@@ -131,12 +131,38 @@ struct Piece {
     int64_t slot;
 };
 
+// n / d of numbers that are seldom past 32 bits: the longer division is a few hundred instructions.
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+    return (n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
+// What lane `i` of the wave holds, the same in all.
+__device__ __forceinline__ int64_t of_lane(int64_t v, int i) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, i), hi = __builtin_amdgcn_readlane((int)(v >> 32), i);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+// The sum over this lane and those below it.
+template <int FROM, int ROWS>
+__device__ __forceinline__ int64_t add_moved(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, FROM, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), FROM, ROWS, 0xF, false);
+    return v + (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_upto(int64_t v) {
+    v = add_moved<0x111, 0xF>(v);  // row_shr: 1, 2, 4, 8
+    v = add_moved<0x112, 0xF>(v);
+    v = add_moved<0x114, 0xF>(v);
+    v = add_moved<0x118, 0xF>(v);
+    v = add_moved<0x142, 0xA>(v);    // lane 15 of the row before, into rows 1 and 3
+    return add_moved<0x143, 0xC>(v);  // lane 31, into rows 2 and 3
+}
+
 // The line of steps as a workgroup walks it.
 template <int WAVES, int TILE = PG_K>
 struct Line {
     static constexpr int STEP = WAVES * TILE, NT = 64 * WAVES;
     static constexpr int PART = STEP < 256 ? 256 / STEP : 1, PART2 = STEP < 512 ? 512 / STEP : 1;  // 256, 512 positions
     static constexpr int START = PART;
+    static_assert((PART & (PART - 1)) == 0 && (PART2 & (PART2 - 1)) == 0, "masks");
     int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
     int64_t base;                    // first step of sequence b
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
@@ -148,9 +174,10 @@ struct Line {
         b = i;
         len = sequence_length(a, i, over);
         steps = (len + STEP - 1) / STEP;
-        cost = unit ? (steps + unit - 1) / unit * unit : steps ? steps + START : 0;
+        places();
     }
-    // Finds the part of this workgroup; `scan` holds NT numbers.
+    __device__ __forceinline__ void places() { cost = unit ? (steps + unit - 1) & -unit : steps ? steps + START : 0; }
+    // Finds the part of this workgroup; `scan` holds WAVES + 1 numbers.
     __device__ __forceinline__ void init(const PagedArgs& a, int64_t* scan) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         heads = a.Hkv * a.qtiles;
@@ -165,6 +192,7 @@ struct Line {
             stop = at + cost;
             return;
         }
+        if (a.B <= 64) return init_alone(a);
         const int per = (a.B + NT - 1) / NT, first = min(tid * per, a.B), last = min(first + per, a.B);
         // parts of 256 or 512 positions, if the workgroups suffice: none then has two pieces (a thread counts no
         // further than 2^20 parts, more than there are workgroups)
@@ -189,34 +217,56 @@ struct Line {
             sequence(a, i);
             mine += (int64_t)heads * cost;
         }
-        int64_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += o;
+        const int64_t upto = wave_upto(mine);
+        __syncthreads();
+        if (lane == 63) scan[wave] = upto;
+        __syncthreads();
+        int64_t before = upto - mine, total = 0;
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) before += scan[w];
+            total += scan[w];
+        }
+        total = of_lane(total, 0);
+        part_of(a, total);
+        if (at >= stop) return;
+        __syncthreads();
+        if (at >= before && at < before + mine) {  // one thread's sequences
+            scan[0] = before;
+            scan[1] = first;
         }
         __syncthreads();
-        scan[tid] = upto;
-        __syncthreads();
-        int64_t before = upto - mine;
-        for (int w = 0; w < wave; ++w) before += scan[64 * w + 63];
-        int64_t total = 0;
-        for (int w = 0; w < WAVES; ++w) total += scan[64 * w + 63];
-        __syncthreads();
-        scan[tid] = before;
-        share = unit ? unit : (total + a.groups - 1) / a.groups;
-        __syncthreads();
+        base = of_lane(scan[0], 0);
+        sequence(a, (int)of_lane(scan[1], 0));
+        advance(a);
+    }
+    // The same for up to 64 sequences, one a lane: each wave for itself, without a barrier, each length loaded once.  A
+    // workgroup has its part after 2400 cycles; with the scan over the workgroup, a search in LDS and 64-bit
+    // divisions it had it after 6500 (32 sequences of up to 2047 positions of 4 bits: 16.1 us, 17.4 with those).
+    __device__ __forceinline__ void init_alone(const PagedArgs& a) {
+        const int lane = threadIdx.x & 63;
+        sequence(a, min(lane, a.B - 1));
+        if (lane >= a.B) steps = 0;
+        auto parts = [&](int of) {
+            return wave_add((int)min((int64_t)heads * ((steps + of - 1) / of), (int64_t)1 << 20));
+        };
+        unit = parts(PART) <= a.groups ? PART : parts(PART2) <= a.groups ? PART2 : 0;
+        lead = unit ? 0 : START;
+        places();
+        const int64_t mine = (int64_t)heads * cost, upto = wave_upto(mine);
+        part_of(a, of_lane(upto, 63));
+        if (at >= stop) return;
+        const int from = __builtin_ctzll(__ballot(at >= upto - mine && at < upto));
+        base = of_lane(upto - mine, from);
+        b = from;
+        len = __builtin_amdgcn_readlane(len, from);
+        steps = __builtin_amdgcn_readlane(steps, from);
+        cost = __builtin_amdgcn_readlane(cost, from);
+        over = __builtin_amdgcn_readlane((int)over, from);
+    }
+    __device__ __forceinline__ void part_of(const PagedArgs& a, int64_t total) {
+        share = unit ? unit : quotient(total + a.groups - 1, a.groups);
         start = at = min((int64_t)blockIdx.x * share, total);
         stop = min(at + share, total);
-        if (at >= stop) return;
-        int lo = 0, hi = NT;  // the last thread whose sequences begin at or before `at`
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (scan[mid] <= at) lo = mid; else hi = mid;
-        }
-        base = scan[lo];
-        sequence(a, lo * per);
-        advance(a);
     }
     __device__ __forceinline__ void advance(const PagedArgs& a) {
         while (at >= base + (int64_t)heads * cost) {
@@ -228,7 +278,7 @@ struct Line {
     __device__ __forceinline__ bool next(const PagedArgs& a, Piece& p) {
         while (at < stop) {
             advance(a);
-            const int hq = (int)((at - base) / cost), x0 = (int)(at - base - (int64_t)hq * cost);
+            const int hq = (int)quotient(at - base, cost), x0 = (int)(at - base - (int64_t)hq * cost);
             const int x1 = (int)min((int64_t)cost, x0 + (stop - at));
             const int s0 = max(x0 - lead, 0), s1 = min(x1 - lead, steps);
             const bool first = at == start;
@@ -247,7 +297,7 @@ struct Line {
             p.slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
             if (a.groups && s0 == 0 && threadIdx.x == 0) {  // for the join
                 const int64_t end = base + (int64_t)hq * cost + lead + steps - 1;  // its last step
-                const int more = p.whole ? 0 : (int)(end / share) - (int)blockIdx.x;
+                const int more = p.whole ? 0 : (int)quotient(end, share) - (int)blockIdx.x;
                 a.pieces[(int64_t)b * heads + hq] = make_int2((int)p.slot, more + 1);
             }
             return true;

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_copy_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * SLOT];
     __shared__ int64_t offsets[WAVES][PG_IDS<WAVES>];
     __shared__ float ml[WAVES][2][16];
-    __shared__ int64_t scan[64 * WAVES];
+    __shared__ int64_t scan[WAVES + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(64 * PG_I8_WAVES, HDP <= 64 ? 3 : HDP <= 128 ? 2 : 
     constexpr int SLOT = (TILE > OTILE ? TILE : OTILE) + 256;  // + 64 scales
     __shared__ __attribute__((aligned(16))) uint8_t lds[WAVES * SLOT];
     __shared__ float ml[WAVES][2][16];
-    __shared__ int64_t scan[64 * WAVES];
+    __shared__ int64_t scan[WAVES + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
     const int hd = EXACT ? HDP : a.hd;
     Line<WAVES> line;

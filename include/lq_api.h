@@ -818,7 +818,7 @@ int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_
  * cache_type LQ_U4 holds 4 bits a value (hd a multiple of 32, at most 256): pages [pages][Hkv][page][hd / 2] bytes, dim
  * d in the low half of byte d / 2 where d is even; d_k_scale [pages][Hkv][page][2][hd / 32] bfloat16, a scale for
  * each 32 dims of a key, then a bias for each (keys have strong channels); d_v_scale [pages][Hkv][page][2] bfloat16, a
- * scale and a bias for the whole row of a value; value = code * scale + bias.
+ * scale and a bias for the whole row of a value; value = code * scale + bias (scales of either sign).
  *
  * Appends packed new tokens: token t's keys at d_k + t * ld (elements of src_type LQ_F32, LQ_F16
  * or LQ_BF16; [Hkv][hd] contiguous), its values at d_v + t * ld.  Sequence s owns tokens
@@ -844,7 +844,7 @@ int lq_paged_kv_append(const void* d_k, const void* d_v, int src_type, int64_t l
  * d_q_out (rows ldqo apart), the rotated keys likewise in d_k_out (NULL: not wanted) and to the cache (of q_type,
  * LQ_I8 or LQ_U4), the values to the cache.  d_q_out may be d_q, and d_k_out d_k, where types and strides are equal.
  * H may be 0 (then no queries).  A token of a sequence whose position lies outside [0, positions)
- * gets NaN for its rotated rows and is not appended; rows of tokens that belong to no sequence are not
+ * gets NaN for its rotated rows and is not appended (rot 0: no position is outside, and d_angles is not read); rows of tokens that belong to no sequence are not
  * written.  Else the rules of lq_paged_kv_append; hd at most 256. */
 int lq_paged_kv_append_rotary(const void* d_q, int64_t ldq, const void* d_k, const void* d_v, int64_t ldkv,
                               int src_type, int64_t tokens, const int32_t* d_starts, int64_t seqs, int64_t H,
@@ -860,7 +860,9 @@ int lq_paged_kv_append_rotary(const void* d_q, int64_t ldq, const void* d_k, con
  * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
  * lengths: the split over the positions is planned from it, and lengths past it are still
  * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and
- * finite; pages 16-byte aligned.  Workspace: lq_paged_attention_workspace_size bytes (0 where one
+ * finite; pages (and the scales of LQ_U4) 16-byte aligned.  Over LQ_U4 a weight meets its value's scale in 16-bit
+ * terms relative to the sequence's largest scale: what lies 2^-31 below the largest weight times that scale is
+ * lost.  Workspace: lq_paged_attention_workspace_size bytes (0 where one
  * workgroup takes a whole sequence), no contents kept from call to call. */
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
             for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
             const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
-            const int high = __builtin_amdgcn_readfirstlane(wave_max((int)(__float_as_uint(vs) >> 23)));
+            const int high = __builtin_amdgcn_readfirstlane(wave_max((int)(__float_as_uint(vs) >> 23 & 255)));
             if (high > top) {
                 const float f = __builtin_amdgcn_ldexpf(1.0f, top - high);
                 top = high;

@@ -64,11 +64,11 @@ class Cache4:
         w /= w.sum()
         out = w @ values4(vc, vs, vb)
         Q = np.abs(q).reshape(-1, 32).sum(1)
-        K = scale * 1.4427 * (((2 * offset + 15) * ks.astype(np.float64) + np.abs(kb)) @ Q).max()
+        K = scale * 1.4427 * (((2 * offset + 15) * np.abs(ks).astype(np.float64) + np.abs(kb)) @ Q).max()
         rel = 2 * ((hd + 16) * U * K + 16 * U) + 2 * w_eps + (n + 64) * U
-        size = w @ (31 * vs[:, 0].astype(np.float64) + np.abs(vb[:, 0]))
+        size = w @ (31 * np.abs(vs[:, 0]).astype(np.float64) + np.abs(vb[:, 0]))
         tiny = 2.0 ** -25 if out_eps == HALF["float16"] else 1e-38
-        size = rel * size + n * 2.0 ** -31 * w.max() * 31 * vs.max()
+        size = rel * size + n * 2.0 ** -31 * w.max() * 31 * np.abs(vs).max()
         return out, size * (1 + out_eps) + out_eps * np.abs(out) + tiny
 
 
@@ -141,6 +141,28 @@ def test_sizes_far_from_one(gpu, dtype, out, size):
     scale = 0.125 / size
     got = values(F.paged_attention(dev(qh), max_length=1400, scale=scale, out_dtype=types()["float32"], **cache.tensors()))
     _check(cache, q, got, 2, scale, dtype, "float32")
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("bound", [200, 2000])
+def test_scales_of_either_sign(gpu, dtype, out, bound):
+    """Pages that a caller filled: code * scale + bias holds for a negative scale too."""
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(bound)
+    cache = Cache4(rng, [bound, 70], 2, 16, 64)
+    for b, n in enumerate(cache.lens):
+        page_no, slot = cache.p.at(b, np.arange(n))
+        for c in "kv":
+            _, scale, bias = cache.rows[b][c]
+            turned = rng.random(scale.shape) < (0.5 if b else 1.0)
+            bias[turned] += rounded(15 * scale[turned], "bfloat16")[0]
+            bias[:] = rounded(bias, "bfloat16")[0]
+            scale[turned] *= -1
+            cache.meta[c][page_no, :, slot] = np.stack([scale, bias], -2)
+    q, qh = rounded(rng.standard_normal((2, 4, 64)), dtype)
+    got = values(F.paged_attention(dev(qh), max_length=bound, out_dtype=types()[out], **cache.tensors()))
+    _check(cache, q, got, 2, 0.125, dtype, out)
 
 
 @pytest.mark.parametrize("n,bound", [(100, 100), (3000, 3000)])

@@ -5,7 +5,8 @@
 //   codes: scale = max|y| / 127, code = rne(y * 127 / max|y|).
 //
 // A row stays in registers: x and the residual are read once, the sum and the output written once, and
-// nothing else moves.
+// nothing else moves.  Bound by HBM: 4097 rows of 4096 in bfloat16 with a residual, 8-bit rows out, 23 us (5.1 TB/s read
+// and written), 16384 rows of 8192 151 us (6.2); 8 rows of 512 take the 3 us of any launch.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 
@@ -268,8 +269,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_kernel(RmsArgs a) {
 // Rows that registers do not hold: read again on each pass, from the stored sum where there is one (each thread
 // reads the places that it wrote).
 template <class E>
-__global__ __launch_bounds__(1024) void rms_wide_kernel(RmsArgs a) {
-    constexpr int TPR = 1024;
+__global__ __launch_bounds__(512) void rms_wide_kernel(RmsArgs a) {
+    constexpr int TPR = 512;
     __shared__ float red[TPR / 64];
     const int64_t row = workgroup();
     if (row >= a.rows) return;
@@ -314,7 +315,16 @@ __global__ __launch_bounds__(1024) void rms_wide_kernel(RmsArgs a) {
     for (int d = tid; d < D; d += TPR) q[d] = (int8_t)rs.code(out(d));
 }
 
-constexpr int RMS_MAX = 16384;  // values of a row in registers
+// Values of a row in registers.  Threads to a row, kernel us, bfloat16, few rows / many (8-bit rows from 4096 dims):
+//   dims    rows         threads (chunks of eight each)
+//    512    8 / 4096     64 (1): 2.9 / 5.0     256 (1): 3.2 / 7.6
+//   1024    8 / 8192     64 (2): 3.3 / 13.4    256 (1): 3.3 / 16.6
+//   2048    8 / 4096     64 (4): 4.6 / 13.1    256 (1): 3.4 / 14.4
+//   4096    8 / 4097     64 (8): 6.9 / 26.5    256 (2): 4.0 / 23.1    512 (1): 3.5 / 24.0
+//   8192    - / 4096    256 (4): 42.6          512 (2): 41.0         1024 (1): 51.6
+//  16384    8 / 2048    256 (8): 7.6 / 48.0    512 (4): 5.5 / 44.7   1024 (2): 4.6 / 43.0
+// (not 1024: a launch of 2^22 such workgroups and more would pass 2^32 threads)
+constexpr int RMS_MAX = 16384;
 
 int rms_launch(const RmsArgs& a, int type, hipStream_t st, const char* name) {
     const uintptr_t ends = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.res) |
@@ -334,18 +344,18 @@ int rms_launch(const RmsArgs& a, int type, hipStream_t st, const char* name) {
         };
         const std::integral_constant<int, 64> t64{};
         const std::integral_constant<int, 256> t256{};
+        const std::integral_constant<int, 512> t512{};
+        const std::integral_constant<int, 4> c4{};
         const std::integral_constant<int, 1> c1{};
         const std::integral_constant<int, 2> c2{};
-        const std::integral_constant<int, 4> c4{};
-        const std::integral_constant<int, 8> c8{};
         note_path(a.D > RMS_MAX ? "rms wide" : vec ? "rms" : "rms single");
         if (a.D <= 512) go(t64, c1);
         else if (a.D <= 1024) go(t64, c2);
         else if (a.D <= 2048) go(t256, c1);
         else if (a.D <= 4096) go(t256, c2);
-        else if (a.D <= 8192) go(t256, c4);
-        else if (a.D <= RMS_MAX) go(t256, c8);
-        else hipLaunchKernelGGL((rms_wide_kernel<E>), grid_of(a.rows), dim3(1024), 0, st, a);
+        else if (a.D <= 8192) go(t512, c2);
+        else if (a.D <= RMS_MAX) go(t512, c4);
+        else hipLaunchKernelGGL((rms_wide_kernel<E>), grid_of(a.rows), dim3(512), 0, st, a);
     });
     return launch_status(name);
 }

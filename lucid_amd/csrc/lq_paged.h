@@ -161,7 +161,9 @@ template <int WAVES, int TILE = PG_K>
 struct Line {
     static constexpr int STEP = WAVES * TILE, NT = 64 * WAVES;
     static constexpr int PART = STEP < 256 ? 256 / STEP : 1, PART2 = STEP < 512 ? 512 / STEP : 1;  // 256, 512 positions
-    static constexpr int START = PART;
+    // a start is 256 positions' time; over 4-bit pages, which pass faster, 512 (1 / 2 / 3 / 5 steps of 256: 64 sequences of
+    // up to 8191 positions 49.1 / 46.8 / 48.3 / 52.3 us, long ones alike)
+    static constexpr int START = TILE == 64 ? 2 * PART : PART;
     static_assert((PART & (PART - 1)) == 0 && (PART2 & (PART2 - 1)) == 0, "masks");
     int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
     int64_t base;                    // first step of sequence b

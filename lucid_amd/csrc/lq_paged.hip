@@ -1,8 +1,8 @@
 // lq_paged.hip -- a key-value cache in pages: appending new tokens' keys and values, and the
 // attention of one new token per sequence over its pages.
 //
-// Layout.  k / v pages [pages][Hkv][page][hd] (fp16, bfloat16, or int8 codes with one float32
-// scale per row in [pages][Hkv][page]); table [seqs][table_stride] of page numbers; position p
+// Layout.  k / v pages [pages][Hkv][page][hd] (fp16, bfloat16, int8 codes with one float32
+// scale per row in [pages][Hkv][page], or 4-bit codes with bfloat16 scales and biases: lq_u4.h); table [seqs][table_stride] of page numbers; position p
 // of sequence s is slot p % page of page table[s][p / page].  A head's rows of one page lie next
 // to each other, so the attention of a head streams page * hd contiguous values.
 #include <hip/hip_runtime.h>

@@ -87,6 +87,12 @@ struct Place {
 // that, and 7.5 scales more from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
+// Bound by HBM where sequences are long: 1.47 million positions and key heads of 128 dims (218 MB) 47 us and 4.7 for
+// the join; within a workgroup's tiles that is 7 TB/s, what a read reaches, after some 10000 cycles from the plan over the
+// page numbers to the first tile, none of which can be earlier than the one before.  64 sequences of up to 8191 (172 MB): 47 us,
+// of which workgroups' second pieces cost a fifth.  Products on vector instructions, a key to a lane: 98 and 6.4 ms.
+// Scores by 4x4x4 products, which have no idle rows for four query heads to a key head: long ones 2% faster, but 58 us (49 then) for the 64 sequences
+// and 20 instead of 16 for 32 of up to 2047, as every lane then lays out a whole query.
 // ALL: for a float32 output.
 // ALIGNED: pages of whole tiles: a tile lies in one page, its addresses are a scalar and a constant of the lane.
 template <int G, int WAVES, bool ALL, bool ALIGNED, class Q>

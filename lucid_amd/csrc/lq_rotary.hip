@@ -46,7 +46,7 @@ __device__ __forceinline__ bool find_token(const RotaryArgs& r, int64_t t, Token
     return true;
 }
 
-// A row of x as it lies in the cache: scale and bias, or codes.
+// Head h of a token's queries, keys or values.
 template <class Src>
 __device__ __forceinline__ const typename Src::T* source_row(const RotaryArgs& r, int64_t t, int kind, int h) {
     const void* p = kind == ROW_Q ? r.q : kind == ROW_K ? r.a.k : r.a.v;
@@ -161,8 +161,11 @@ struct Raw8 {
 // a lane.  A lane keeps its place in the row for every head, so the angles of its dims are loaded once.  The values are on
 // their way before the token's place is looked up (a search, two numbers, a page number and the angles, each
 // after the other).  swap: the lane whose place holds the partners differs by this bit; 0: the partners are loaded.
-// Rows of a call from which a lane takes four: the loads of one hide nothing of the places' latency.
-constexpr int RT_T = 64;
+// Bound by HBM: 20452 tokens of 32 + 2 * 8 heads of 128 in bfloat16 106 us, 4.8 TB/s read and written, what a copy
+// reaches (one row a lane in workgroups of 256: 133, with the partners loaded 168).
+constexpr int RT_T = 64;  // threads; 128 or 256 of them, four rows a lane: 136 and 118 us
+// Rows of a call from which a lane takes four: the loads of one hide nothing of the places' latency.  One / four rows a
+// lane: 49152 rows alike, 98304 rows 13.7 / 10.6 us.
 constexpr int64_t RT_ROWS = 1 << 16;
 template <int AHEAD, class Src, class Out, class Cache>
 __global__ __launch_bounds__(RT_T) void rotary_kernel(RotaryArgs r, int lpr, int swap, uint32_t groups) {

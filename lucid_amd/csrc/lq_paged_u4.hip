@@ -20,12 +20,14 @@ constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_NST = 2;     // tiles on their way
 
 // Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
-// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes; where two pairs
-// share a shift, 256 + c for even p (a score of a 16-bit output has room for what that adds to its rounding).
+// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes; SHARE: where two
+// pairs share a shift, 256 + c for even p (a score of a 16-bit output has room for what that adds to its rounding).
+// CENTRE: one addition more for c - 7.5.
 // An and-or takes no literal, so masks and exponents are kept in registers whose values the compiler does not see.
-template <bool SHARE>
+template <bool SHARE, bool CENTRE>
 struct Widen8 {
-    static constexpr float EVEN = SHARE ? 256.0f : 16.0f, ODD = 16.0f;  // what is added to a code
+    // what is added to a code
+    static constexpr float EVEN = CENTRE ? -7.5f : SHARE ? 256.0f : 16.0f, ODD = CENTRE ? -7.5f : 16.0f;
     uint32_t m0, e0, m1, e1;
     __device__ __forceinline__ Widen8()
         : m0(SHARE ? 0x003c003cu : 0x03c003c0u), e0(SHARE ? 0x5c005c00u : 0x4c004c00u), m1(0x03c003c0u), e1(0x4c004c00u) {
@@ -33,11 +35,19 @@ struct Widen8 {
         if (SHARE) asm("" : "+v"(m1), "+v"(e1));
     }
     __device__ __forceinline__ u4v operator()(uint32_t w) const {
+        static_assert(!SHARE || !CENTRE, "one or the other");
         if constexpr (SHARE) {
             const uint32_t lo = w << 2, hi = w >> 6;
             return u4v{(lo & m0) | e0, (lo & m1) | e1, (hi & m0) | e0, (hi & m1) | e1};
         }
-        return u4v{((w << 6) & m0) | e0, ((w << 2) & m0) | e0, ((w >> 2) & m0) | e0, ((w >> 6) & m0) | e0};
+        u4v v = {((w << 6) & m0) | e0, ((w << 2) & m0) | e0, ((w >> 2) & m0) | e0, ((w >> 6) & m0) | e0};
+        if constexpr (CENTRE) {
+            typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+            const h2v down = {(_Float16)-23.5f, (_Float16)-23.5f};
+#pragma unroll
+            for (int p = 0; p < 4; ++p) v[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v, (uint32_t)v[p]) + down);
+        }
+        return v;
     }
 };
 
@@ -85,6 +95,8 @@ struct Place {
 // instruction more multiplies the row's scales and biases, bfloat16 as they are stored, by minus the queries' sums times
 // what was added and by their sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of
 // that, and 7.5 scales more from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
+// A float32 output is worth an addition to every pair of codes: c - 7.5 in both products, so that no sum grows by what is
+// taken off later (2-norm of the error of 300 to 60000 positions 2e-8 to 2e-7 of the output's, with offsets 3e-7 to 3e-6).
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
 // Bound by HBM where sequences are long: 1.47 million positions and key heads of 128 dims (218 MB) 47 us and 4.7 for
@@ -112,8 +124,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // scalar, and what follows from it
     Line<WAVES, U4_TILE> line;
     line.init(a, reinterpret_cast<int64_t*>(lds));
-    const Widen8<!ALL> key_codes;
-    const Widen8<false> value_codes;
+    using KeyCodes = Widen8<!ALL, ALL>;
+    const KeyCodes key_codes;
+    const Widen8<false, ALL> value_codes;
     constexpr int STEP = WAVES * U4_TILE;
     const int page = a.page, cols = STEP / page, slots = STEP - cols * page;
     const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
@@ -275,7 +288,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                 const float t1 = unpack2(B{}, pack2(B{}, r1, 0.0f))[0];
                 return g == 0 ? t0 : g == 1 ? t1 : g == 2 ? r1 - t1 : 0.0f;
             };
-            const uint32_t both = pack2(B{}, term(even + odd), term(-(Widen8<!ALL>::EVEN * even + Widen8<!ALL>::ODD * odd)));
+            const uint32_t both = pack2(B{}, term(even + odd), term(-(KeyCodes::EVEN * even + KeyCodes::ODD * odd)));
             const int at = G <= 4 ? G + s : 8 + s;
             qsum[0][(s >> 1) & 3] |= s & 1 ? both & 0xffff0000u : both >> 16;      // with the scales
             qsum[at >> 3][(at >> 1) & 3] |= at & 1 ? both << 16 : both & 0xffffu;  // with the biases
@@ -429,10 +442,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                     }
                 }
             const u4v offset = {0x4de04de0u, 0x4de04de0u, 0x4de04de0u, 0x4de04de0u};  // 23.5
+            if constexpr (!ALL) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                ones = mfma_16x16x32(P{}, offset, hi[j], ones);
-                if constexpr (ALL) ones = mfma_16x16x32(P{}, offset, lo[j], ones);
+                for (int j = 0; j < 2; ++j) ones = mfma_16x16x32(P{}, offset, hi[j], ones);
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)

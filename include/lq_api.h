@@ -827,7 +827,7 @@ int lq_argmax_next_f32(const float* d_x, int64_t rows, int64_t cols, int32_t* d_
  * to nearest even.  An int8 cache gets scale = max|x| / 127 and code = rne(x * (127 / max|x|)) per
  * row of hd; a row with an infinity or NaN gets a scale that is not finite and is attended as
  * NaN, one whose magnitudes are below 127 / FLT_MAX as zeros.  4 bits: bias = the bfloat16 at or below
- * the least x of a group, scale = the one at or above (max x - bias) / 15, code = rne((x - bias) * (1 / scale)) within
+ * the least x of a group, scale = the one at or above (max x - bias) * (1 / 15), code = rne((x - bias) * (1 / scale)) within
  * 0 .. 15; a group with an infinity or NaN, or whose width passes float32, has a scale and a bias of NaN; one whose
  * scale has no float32 reciprocal has the scale 0.  A token is left out when its
  * position is negative (a sequence of length 0), lies past the table, or its page number is

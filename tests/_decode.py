@@ -59,7 +59,7 @@ def quantize4(x, step):
     g = x.reshape(*x.shape[:-1], x.shape[-1] // step, step)
     with np.errstate(all="ignore"):
         bias = bf16_toward(g.min(-1), False)
-        scale = bf16_toward((g.max(-1) - bias) / np.float32(15), True)
+        scale = bf16_toward((g.max(-1) - bias) * (np.float32(1) / np.float32(15)), True)
         inv = np.float32(1) / scale
         none = ~(inv < np.inf)
         scale, inv = np.where(none, 0, scale).astype(np.float32), np.where(none, 0, inv).astype(np.float32)

@@ -166,7 +166,13 @@ struct Line {
     static constexpr int START = TILE == 64 ? 2 * PART : PART;
     static_assert((PART & (PART - 1)) == 0 && (PART2 & (PART2 - 1)) == 0, "masks");
     int64_t share, at, stop, start;  // steps of a workgroup; next step, end and start of this part
+    // Over 4-bit pages the later of two workgroups on a CU is the slower one: the older waves issue first (even parts ended
+    // after 34 and 43 us).  A workgroup of the first half takes 5/8 of the two's steps: long sequences 47.5 -> 44.3 us,
+    // 64 of up to 8191 46.8 -> 43.6 (1/2 in whole steps: 47.3 and 45.0, 11/16: 46.8 and 45.7; priorities that
+    // change with every tile: 45.1 and 44.3).
+    int64_t half, late;  // workgroups of the first half; steps of one of the second
     int64_t base;                    // first step of sequence b
+    static constexpr bool PAIRS = TILE == 64;  // two workgroups to a CU up to 128 dims
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
     int cost;                  // places of one head of sequence b on the line
     int unit, lead;            // steps that a part is a multiple of (0: any), places before a head's first step
@@ -266,9 +272,30 @@ struct Line {
         over = __builtin_amdgcn_readlane((int)over, from);
     }
     __device__ __forceinline__ void part_of(const PagedArgs& a, int64_t total) {
+        const int64_t n = blockIdx.x;
         share = unit ? unit : quotient(total + a.groups - 1, a.groups);
-        start = at = min((int64_t)blockIdx.x * share, total);
-        stop = min(at + share, total);
+        start = n * share;
+        int64_t mine = share;
+        if constexpr (PAIRS) {
+            half = a.groups / 2;
+            late = share;
+            if (!unit && a.hd <= 128) {
+                const int64_t pair = quotient(total + half - 1, half);
+                share = min(pair, (pair * 5 + 4) / 8);
+                late = pair - share;
+                start = min(n, half) * share + max(n - half, (int64_t)0) * late;
+                mine = n < half ? share : late;
+            }
+        }
+        start = at = min(start, total);
+        stop = min(at + mine, total);
+    }
+    // The workgroup with place x of the line.
+    __device__ __forceinline__ int owner(int64_t x) const {
+        if constexpr (PAIRS) {
+            if (x >= half * share) return (int)(half + quotient(x - half * share, late));
+        }
+        return (int)quotient(x, share);
     }
     __device__ __forceinline__ void advance(const PagedArgs& a) {
         while (at >= base + (int64_t)heads * cost) {
@@ -299,7 +326,7 @@ struct Line {
             p.slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
             if (a.groups && s0 == 0 && threadIdx.x == 0) {  // for the join
                 const int64_t end = base + (int64_t)hq * cost + lead + steps - 1;  // its last step
-                const int more = p.whole ? 0 : (int)quotient(end, share) - (int)blockIdx.x;
+                const int more = p.whole ? 0 : owner(end) - (int)blockIdx.x;
                 a.pieces[(int64_t)b * heads + hq] = make_int2((int)p.slot, more + 1);
             }
             return true;

@@ -99,10 +99,10 @@ struct Place {
 // taken off later (2-norm of the error of 300 to 60000 positions 2e-8 to 2e-7 of the output's, with offsets 3e-7 to 3e-6).
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
-// Bound by HBM where sequences are long: 1.47 million positions and key heads of 128 dims (218 MB) 47 us and 4.7 for
-// the join; within a workgroup's tiles that is 7 TB/s, what a read reaches, after some 10000 cycles from the plan over the
-// page numbers to the first tile, none of which can be earlier than the one before.  64 sequences of up to 8191 (172 MB): 47 us,
-// of which workgroups' second pieces cost a fifth.  Products on vector instructions, a key to a lane: 98 and 6.4 ms.
+// Bound by HBM where sequences are long: 1.47 million positions and key heads of 128 dims (218 MB) 44 us and 4.7 for
+// the join; a workgroup's first tile comes after 7 us (the plan, the page numbers, the copies: none of which can be earlier
+// than the one before), the others pass at 6 TB/s with the vector unit busy 47%.  64 sequences of up to 8191 (172 MB):
+// 44 us, of which workgroups' second pieces cost a fifth.  Products on vector instructions, a key to a lane: 98 and 6.4 ms.
 // Scores by 4x4x4 products, which have no idle rows for four query heads to a key head: long ones 2% faster, but 58 us (49 then) for the 64 sequences
 // and 20 instead of 16 for 32 of up to 2047, as every lane then lays out a whole query.
 // ALL: for a float32 output.

@@ -105,9 +105,9 @@ __device__ __forceinline__ int sequence_length(const PagedArgs& a, int b, bool& 
     return over ? (int)cap : len;
 }
 
-// The two kernels share this plan.  The work is a line of steps (WAVES tiles of 32 positions): all steps
+// The kernels share this plan.  The work is a line of steps (WAVES tiles of 32 positions, of 64 over 4-bit pages): all steps
 // of the first sequence's first key head (and tile of 16 query heads), then of its next one, and so
-// on.  Each workgroup takes an equal part of the line, whatever the sequences' lengths, and works
+// on.  Each workgroup takes an equal part of the line (PAIRS: one of two sizes), whatever the sequences' lengths, and works
 // through the pieces of sequences in it one after the other.  A piece costs some microseconds of dependent
 // loads before its first tile, which counts as START steps on the line (without it 64 sequences of 256 to
 // 8191 positions took 128 us, with it 110).  Where parts of 256 or 512 positions are enough for all, each
@@ -171,7 +171,7 @@ struct Line {
     // 64 of up to 8191 46.8 -> 43.6 (1/2 in whole steps: 47.3 and 45.0, 11/16: 46.8 and 45.7; priorities that
     // change with every tile: 45.1 and 44.3).
     int64_t half, late;  // workgroups of the first half; steps of one of the second
-    int64_t base;                    // first step of sequence b
+    int64_t base;        // first step of sequence b
     static constexpr bool PAIRS = TILE == 64;  // two workgroups to a CU up to 128 dims
     int b, len, steps, heads;  // heads: key heads times tiles of 16 query heads
     int cost;                  // places of one head of sequence b on the line

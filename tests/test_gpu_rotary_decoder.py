@@ -144,3 +144,26 @@ def test_generation_over_four_bits_repeats(gpu, served):
     second = pd.generate(prompts, 6)
     for x, y in zip(first, second):
         assert np.array_equal(x, y)
+
+
+def test_calls_that_draft_nothing_or_are_refused(gpu, served):
+    """No sequences, a token without drafts, and refusals that leave the sequences as they were."""
+    a, b = _make(served, "rotary", "float16"), _make(served, "rotary", "float16")
+    prompt = {0: np.arange(5, 25)}
+    for pd in (a, b):
+        pd.prefill(prompt)
+    assert a.speculate({}, [], []) == {}
+    logits = b.step({0: 8}).numpy()[0].astype(np.float64)
+    got = a.speculate({0: [8]}, np.zeros(1, np.float32), np.array([0.25], np.float32))
+    share = np.cumsum(np.exp(logits - logits.max()))
+    assert len(got[0]) == 1 and abs(share[got[0][0]] / share[-1] - 0.25) < 0.01
+    before = a.table.host_lengths().tolist()
+    zeros = np.zeros(2, np.float32)
+    for tokens, accept, sample in (({0: [1, 2]}, zeros[:1], zeros[:1]), ({0: [1, 2]}, zeros, zeros),
+                                   ({0: [1, a.vocab]}, zeros, zeros[:1]), ({0: []}, [], zeros[:1]),
+                                   ({1: [1, 2]}, zeros, zeros[:1]), ({7: [1, 2]}, zeros, zeros[:1]),
+                                   ({0: np.ones(a.positions, np.int64)}, np.zeros(a.positions), zeros[:1])):
+        with pytest.raises((ValueError, IndexError)):
+            a.speculate(tokens, accept, sample)
+        assert a.table.host_lengths().tolist() == before
+    assert _cos(a.step({0: 4}).numpy(), b.step({0: 4}).numpy()) > 0.999

@@ -542,7 +542,7 @@ class PageTable:
         if max(need) > self._table.shape[1]:
             raise ValueError(f"PageTable.grow: a sequence of {int(new.max())} positions needs {max(need)} pages, its "
                              f"row holds {self._table.shape[1]}")
-        more = sum(n - h for n, h in zip(need, self._held))
+        more = sum(max(n - h, 0) for n, h in zip(need, self._held))  # pages to spare (shrink) serve their own sequence
         if more > len(self._free):
             raise MemoryError(f"PageTable.grow: {more} pages needed, {len(self._free)} free")
         for s, n in enumerate(need):

@@ -860,8 +860,8 @@ int lq_paged_kv_append_rotary(const void* d_q, int64_t ldq, const void* d_k, con
  * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
  * lengths: the split over the positions is planned from it, and lengths past it are still
  * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and
- * finite; pages (and the scales of LQ_U4) 16-byte aligned.  Over LQ_U4 a weight meets its value's scale in 16-bit
- * terms relative to the sequence's largest scale: what lies 2^-31 below the largest weight times that scale is
+ * finite; pages (and the scales of LQ_U4) 16-byte aligned.  Over LQ_U4 a weight times its value's scale enters in
+ * 16-bit terms relative to the largest such product that the query meets: what lies 2^-35 below that product is
  * lost.  Workspace: lq_paged_attention_workspace_size bytes (0 where one
  * workgroup takes a whole sequence), no contents kept from call to call. */
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);

@@ -19,6 +19,11 @@ namespace {
 constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_NST = 2;     // tiles on their way
 
+// A weight times its value's scale enters a product in fp16, as 2^lift times it: the largest one that a query has met lies
+// between 2^U4_SET and 2^U4_LIMIT then, and what fp16 drops (half its least step) is 2^-35 of it.  The largest
+// product and not the largest scale decides: a row that attention ignores costs the others nothing, whatever its scale.
+constexpr int U4_SET = 10, U4_LIMIT = 15, U4_LIFT_MAX = 127;
+
 // Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
 // mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes; SHARE: where two
 // pairs share a shift, 256 + c for even p (a score of a 16-bit output has room for what that adds to its rounding).
@@ -87,8 +92,8 @@ struct Place {
 // operand T is position 16 (r / 4) + 4 T + r % 4, and the transposing read brings a lane the codes of its dim at just
 // these 16 positions.
 // Both products are fp16.  Queries of bfloat16 enter times a power of two (their largest value between 2^13 and 2^14:
-// fp16 then holds every bit of values down to 2^-27 of it), which goes into the scores' factor.  A weight enters with its
-// value's scale over the largest power of two among the scales so far, once rounded for a 16-bit output (what
+// fp16 then holds every bit of values down to 2^-27 of it), which goes into the scores' factor.  A weight enters times its
+// value's scale, relative to the largest such product so far (U4_SET), once rounded for a 16-bit output (what
 // one more rounding of the output would cost), as two terms (22 bits) for a float32 one; sums and maximum
 // stay float32.
 // A code c enters as 16 + c or 256 + c.  What that adds to a score is taken off where the biases come in: one
@@ -167,7 +172,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.0f, vbias = 0.0f;
-        int top = 0;  // the largest exponent among the values' scales, as stored
+        int lift = U4_LIFT_MAX;  // this lane's query's
+        auto scale_sums = [&](float f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ones[i] *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= f;
+        };
         // this lane's position in the tile that is issued next, and in the one whose page number is fetched next
         int key = first + lane;
         Place at, ahead;
@@ -337,18 +350,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
             for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
             const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
-            const int high = __builtin_amdgcn_readfirstlane(wave_max((int)(__float_as_uint(vs) >> 23 & 255)));
-            if (high > top) {
-                const float f = __builtin_amdgcn_ldexpf(1.0f, top - high);
-                top = high;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ones[i] *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][i] *= f;
-            }
-            *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = __builtin_amdgcn_ldexpf(vs, 127 - top);
+            *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = vs;
             *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) =
                 lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16))) : 0.0f;
             asm volatile("" ::: "memory");
@@ -407,17 +409,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             if (__any(mx > m + RESCALE_AT)) {
                 const float mn = fmaxf(m, weight_reference<P>(mx));
                 const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+                // the products' reference stays where it was: what they are multiplied by rises as the weights fall
+                const float rise = mn == -INFINITY ? 0.0f : fminf(mn - m, 1024.0f);
+                const int to = min(lift + (int)rise, U4_LIFT_MAX);
+                const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn) + (float)(to - lift));
+                lift = to;
                 m = mn;
                 l *= corr;
                 vbias *= corr;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ones[i] *= corr;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][i] *= corr;
+                scale_sums(f);
             }
             const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<P>;
+            float most = 0.0f;  // the largest weight times its value's scale
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
 #pragma unroll
@@ -426,8 +429,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                     l += e;
                     vbias = __builtin_fmaf(e, vb[T][i], vbias);
                     sc[T][i] = e * vf[T][i];
+                    most = fmaxf(most, fabsf(sc[T][i]));
                 }
             }
+            most = quarter_max(most);
+            if (__any(__builtin_amdgcn_ldexpf(most, lift) >= ldexpf(1.0f, U4_LIMIT))) {
+                const int to = min(lift, U4_SET + 127 - (int)(__float_as_uint(most) >> 23));
+                scale_sums(__builtin_amdgcn_ldexpf(1.0f, to - lift));
+                lift = to;
+            }
+            const float up = __builtin_amdgcn_ldexpf(1.0f, lift);
+#pragma unroll
+            for (int T = 0; T < 4; ++T)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[T][i] *= up;
             // O^T += C^T P^T: word j of a transposed read holds positions 8 j .. of this lane's 16, pairs four apart
             u4v hi[2], lo[2];
 #pragma unroll
@@ -466,7 +481,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums.o[d][i] = __builtin_amdgcn_ldexpf(o[d][i] - ones[0], top - 127) + extra;
+            for (int i = 0; i < 4; ++i) sums.o[d][i] = __builtin_amdgcn_ldexpf(o[d][i] - ones[0], -lift) + extra;
         paged_finish<false, WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
     paged_empty<WAVES, Q>(a);

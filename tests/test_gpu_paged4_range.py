@@ -1,0 +1,88 @@
+"""Attention over 4-bit pages whose rows differ far in size, against float64.
+
+The bound is that of test_gpu_paged4.py but for what fp16 drops of a weight times its value's scale: half its least
+step is 2^-35 of the largest such product that a query meets, whatever the scales of the rows that it ignores (that
+file allows 2^-31 of the largest weight times the largest scale, wherever they are)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from _decode import HALF, U, close, dev, rounded, types, values, values4
+from test_gpu_paged4 import TYPES, Cache4
+
+pytestmark = pytest.mark.gpu
+
+
+def _check(cache, q, got, group, scale, out):
+    w_eps, offset = (2.0 ** -22, 16) if out == "float32" else (2.0 ** -11, 256)
+    for b, n in enumerate(cache.lens):
+        for h in range(q.shape[1]):
+            (kc, ks, kb), (vc, vs, vb) = (tuple(a[:, h // group] for a in cache.rows[b][c]) for c in "kv")
+            x = q[b, h].astype(np.float64)
+            s = values4(kc, ks, kb) @ x * scale
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            want = w @ values4(vc, vs, vb)
+            vs, vb = (np.abs(a[:, 0]).astype(np.float64) for a in (vs, vb))
+            K = scale * 1.4427 * (((2 * offset + 15) * np.abs(ks).astype(np.float64) + np.abs(kb))
+                                  @ np.abs(x).reshape(-1, 32).sum(1)).max()
+            rel = 2 * ((cache.hd + 16) * U * K + 16 * U) + 2 * w_eps + (n + 64) * U
+            size = rel * (w @ (31 * vs + vb)) + n * 2.0 ** -35 * (w * vs).max() * 31
+            bound = size * (1 + HALF[out]) + HALF[out] * np.abs(want) + (2.0 ** -25 if out == "float16" else 1e-38)
+            close(got[b, h].astype(np.float64), want, bound, f"sequence {b}, head {h}")
+
+
+def _run(cache, rng, h, dtype, out, scale, positive=False):
+    import lucid_amd.nn.functional as F
+
+    q = rng.standard_normal((len(cache.lens), h, cache.hd))
+    q, qh = rounded(np.abs(q) + 0.3 if positive else q, dtype)
+    got = values(F.paged_attention(dev(qh), max_length=max(cache.lens), scale=scale, out_dtype=types()[out], **cache.tensors()))
+    return q, got
+
+
+def _store(cache, b, pos):
+    """The rows of sequence b at positions pos, as they are in ``rows``, into the pages."""
+    page_no, slot = cache.p.at(b, pos)
+    for c in "kv":
+        codes, scale, bias = cache.rows[b][c]
+        cache.codes[c][page_no, :, slot], cache.meta[c][page_no, :, slot] = codes[pos], np.stack([scale, bias], -2)[pos]
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n", [90, 3000])
+@pytest.mark.parametrize("k", [12, 24, 40, 100])
+def test_a_row_that_attention_ignores(gpu, dtype, out, page, n, k):
+    """Values of 2^k times the others' scale where the score lies some 60 below them: at 2^100 such a row still counts."""
+    rng = np.random.default_rng([n, k, page])
+    cache = Cache4(rng, [n, 70], 2, page, 64)
+    for b, length in enumerate(cache.lens):
+        pos = np.array([0, length // 2, length - 1])
+        (kc, ks, kb), (vc, vs, vb) = (cache.rows[b][c] for c in "kv")
+        kc[pos], ks[pos], kb[pos] = 0, 0, -8
+        vs[pos], vb[pos] = vs[pos] * 2.0 ** k, vb[pos] * 2.0 ** k
+        _store(cache, b, pos)
+    q, got = _run(cache, rng, 4, dtype, out, 0.125, positive=True)
+    _check(cache, q, got, 2, 0.125, out)
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("order", ["rising", "falling", "any"])
+@pytest.mark.parametrize("n,hd,spread", [(200, 32, 1.0), (700, 64, 8.0), (2600, 128, 1.0), (2600, 96, 8.0)])
+def test_scales_from_tiny_to_large(gpu, dtype, out, order, n, hd, spread):
+    """Rows of scales over 58 powers of two beside scores that rule some of them out: what the sums are relative to moves
+    through the whole sequence."""
+    rng = np.random.default_rng([n, hd, len(order)])
+    cache = Cache4(rng, [n, 33], 1, 16, hd)
+    for b, length in enumerate(cache.lens):
+        e = rng.uniform(-50, 8, length)
+        e = np.floor({"rising": np.sort(e), "falling": -np.sort(-e), "any": e}[order])[:, None, None]
+        _, vs, vb = cache.rows[b]["v"]
+        vs *= 2.0 ** e
+        vb *= 2.0 ** e
+        _store(cache, b, np.arange(length))
+    q, got = _run(cache, rng, 3, dtype, out, spread * hd ** -0.5)
+    _check(cache, q, got, 3, spread * hd ** -0.5, out)

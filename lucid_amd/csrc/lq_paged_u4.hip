@@ -19,6 +19,12 @@ namespace {
 constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_NST = 2;     // tiles on their way
 
+// Weights are 2^(score - base) in log2 units, base the running maximum plus this (a reference in whole numbers: one
+// follows the other by powers of two, which round nothing).  The sums of a million biases of 1e36, or of 4096 of
+// bfloat16's largest, then stay finite, as over the other caches.  The statistics that leave a piece are relative to
+// base itself, so that sums with different references stay comparable however large the scores.
+constexpr float U4_SHIFT = 20.0f;
+__device__ __forceinline__ float u4_reference(float mx) { return (fabsf(mx) < 0x1p22f ? ceilf(mx) : mx) + U4_SHIFT; }
 // A weight times its value's scale enters a product in fp16, as 2^lift times it: the largest one that a query has met lies
 // between 2^U4_SET and 2^U4_LIMIT then, and what fp16 drops (half its least step) is 2^-35 of it.  The largest
 // product and not the largest scale decides: a row that attention ignores costs the others nothing, whatever its scale.
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         vf4 o[DT], ones = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.0f, vbias = 0.0f;
+        float base = -INFINITY, l = 0.0f, vbias = 0.0f;
         int lift = U4_LIFT_MAX;  // this lane's query's
         auto scale_sums = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
@@ -399,33 +405,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                         asm volatile("" : "+v"(sc[T][i]));  // in the branch: not sixteen selects for every tile
                     }
             }
-            // weights relative to the running maximum, as the other caches' kernels form them
+            // weights relative to the running maximum, which may lag by 2^RESCALE_AT
             float mx = -INFINITY;
 #pragma unroll
             for (int T = 0; T < 4; ++T)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[T][i]);
             mx = quarter_max(mx) * sl2;
-            if (__any(mx > m + RESCALE_AT)) {
-                const float mn = fmaxf(m, weight_reference<P>(mx));
-                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            if (__any(mx > base + (RESCALE_AT - U4_SHIFT))) {
+                const float to = fmaxf(base, u4_reference(mx)), finite = to == -INFINITY ? 0.0f : to;
+                const float corr = __builtin_amdgcn_exp2f(base - finite);
                 // the products' reference stays where it was: what they are multiplied by rises as the weights fall
-                const float rise = mn == -INFINITY ? 0.0f : fminf(mn - m, 1024.0f);
-                const int to = min(lift + (int)rise, U4_LIFT_MAX);
-                const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn) + (float)(to - lift));
-                lift = to;
-                m = mn;
+                const int higher = min(lift + (int)fminf(finite - base, 1024.0f), U4_LIFT_MAX);
+                const float f = __builtin_amdgcn_exp2f(base - finite + (float)(higher - lift));
+                lift = higher;
+                base = to;
                 l *= corr;
                 vbias *= corr;
                 scale_sums(f);
             }
-            const float base = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT<P>;
+            const float from = base == -INFINITY ? 0.0f : base;
             float most = 0.0f;  // the largest weight times its value's scale
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -base));
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[T][i], sl2, -from));
                     l += e;
                     vbias = __builtin_fmaf(e, vb[T][i], vbias);
                     sc[T][i] = e * vf[T][i];
@@ -476,7 +481,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         // what all dims of a query share: the sum of its values' middles
         const float extra = quarter_sum(vbias);
         Sums<DT, P> sums;
-        sums.m = m;
+        sums.m = base;
         sums.l = l;
 #pragma unroll
         for (int d = 0; d < DT; ++d)

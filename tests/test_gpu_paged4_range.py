@@ -86,3 +86,20 @@ def test_scales_from_tiny_to_large(gpu, dtype, out, order, n, hd, spread):
         _store(cache, b, np.arange(length))
     q, got = _run(cache, rng, 3, dtype, out, spread * hd ** -0.5)
     _check(cache, q, got, 3, spread * hd ** -0.5, out)
+
+
+@pytest.mark.parametrize("dtype,out", [("float16", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n,power,offset", [(640, 120, 1.0), (20000, 120, -1.0), (640, 120, 0.0), (4096, 125, 0.0),
+                                            (20000, -90, 1.0), (640, -90, 0.0)])
+def test_values_near_the_ends_of_the_range(gpu, dtype, out, page, n, power, offset):
+    """Many values of 1e36, or some of the type's largest, have finite sums; of 1e-27 they keep their bits."""
+    rng = np.random.default_rng([n, power + 100])
+    cache = Cache4(rng, [n, 20], 1, page, 64, offset=offset)
+    for b, length in enumerate(cache.lens):
+        _, vs, vb = cache.rows[b]["v"]
+        vs *= 2.0 ** power
+        vb *= 2.0 ** power
+        _store(cache, b, np.arange(length))
+    q, got = _run(cache, rng, 2, dtype, out, 0.125)
+    _check(cache, q, got, 2, 0.125, out)

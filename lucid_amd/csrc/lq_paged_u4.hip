@@ -31,27 +31,19 @@ __device__ __forceinline__ float u4_reference(float mx) { return (fabsf(mx) < 0x
 constexpr int U4_SET = 10, U4_LIMIT = 15, U4_LIFT_MAX = 127;
 
 // Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
-// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes; SHARE: where two
-// pairs share a shift, 256 + c for even p (a score of a 16-bit output has room for what that adds to its rounding).
-// CENTRE: one addition more for c - 7.5.
-// An and-or takes no literal, so masks and exponents are kept in registers whose values the compiler does not see.
-template <bool SHARE, bool CENTRE>
+// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes.  CENTRE: one
+// addition more for c - 7.5.
+// An and-or takes no literal, so mask and exponent are kept in registers whose values the compiler does not see.
+template <bool CENTRE>
 struct Widen8 {
-    // what is added to a code
-    static constexpr float EVEN = CENTRE ? -7.5f : SHARE ? 256.0f : 16.0f, ODD = CENTRE ? -7.5f : 16.0f;
-    uint32_t m0, e0, m1, e1;
-    __device__ __forceinline__ Widen8()
-        : m0(SHARE ? 0x003c003cu : 0x03c003c0u), e0(SHARE ? 0x5c005c00u : 0x4c004c00u), m1(0x03c003c0u), e1(0x4c004c00u) {
-        asm("" : "+v"(m0), "+v"(e0));
-        if (SHARE) asm("" : "+v"(m1), "+v"(e1));
+    static constexpr float ADDED = CENTRE ? -7.5f : 16.0f;  // to a code
+    uint32_t mask, exponent;
+    __device__ __forceinline__ Widen8() : mask(0x03c003c0u), exponent(0x4c004c00u) {
+        asm("" : "+v"(mask), "+v"(exponent));
     }
     __device__ __forceinline__ u4v operator()(uint32_t w) const {
-        static_assert(!SHARE || !CENTRE, "one or the other");
-        if constexpr (SHARE) {
-            const uint32_t lo = w << 2, hi = w >> 6;
-            return u4v{(lo & m0) | e0, (lo & m1) | e1, (hi & m0) | e0, (hi & m1) | e1};
-        }
-        u4v v = {((w << 6) & m0) | e0, ((w << 2) & m0) | e0, ((w >> 2) & m0) | e0, ((w >> 6) & m0) | e0};
+        u4v v = {((w << 6) & mask) | exponent, ((w << 2) & mask) | exponent, ((w >> 2) & mask) | exponent,
+                 ((w >> 6) & mask) | exponent};
         if constexpr (CENTRE) {
             typedef _Float16 h2v __attribute__((ext_vector_type(2)));
             const h2v down = {(_Float16)-23.5f, (_Float16)-23.5f};
@@ -99,15 +91,17 @@ struct Place {
 // these 16 positions.
 // Both products are fp16.  Queries of bfloat16 enter times a power of two (their largest value between 2^13 and 2^14:
 // fp16 then holds every bit of values down to 2^-27 of it), which goes into the scores' factor.  A weight enters times its
-// value's scale, relative to the largest such product so far (U4_SET), once rounded for a 16-bit output (what
-// one more rounding of the output would cost), as two terms (22 bits) for a float32 one; sums and maximum
-// stay float32.
-// A code c enters as 16 + c or 256 + c.  What that adds to a score is taken off where the biases come in: one
-// instruction more multiplies the row's scales and biases, bfloat16 as they are stored, by minus the queries' sums times
-// what was added and by their sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of
-// that, and 7.5 scales more from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
+// value's scale, relative to the largest such product so far (U4_SET), as two terms (within 2^-23 of it); sums and
+// maximum stay float32.
+// A code c enters as 16 + c.  What that adds to a score is taken off where the biases come in: one instruction more
+// multiplies the row's scales and biases, bfloat16 as they are stored, by minus the queries' sums times 16 and by their
+// sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of that, and 7.5 scales more
+// from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
 // A float32 output is worth an addition to every pair of codes: c - 7.5 in both products, so that no sum grows by what is
-// taken off later (2-norm of the error of 300 to 60000 positions 2e-8 to 2e-7 of the output's, with offsets 3e-7 to 3e-6).
+// taken off later (2-norm of the error of 300 to 60000 positions 2e-8 to 2e-7 of the output's, with 16 + c 3e-7 to 3e-6,
+// which 16 bits do not show; 64 sequences of up to 8191 positions 53 us where 16-bit outputs take 49).
+// With one term to a weight of a 16-bit output, and 256 + c for half of a key's codes, those took 46 us: the error of
+// fp16 outputs over long sequences was 1.4 times what their rounding alone gives.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
 // Bound by HBM where sequences are long: 1.47 million positions and key heads of 128 dims (218 MB) 44 us and 4.7 for
@@ -116,9 +110,9 @@ struct Place {
 // 44 us, of which workgroups' second pieces cost a fifth.  Products on vector instructions, a key to a lane: 98 and 6.4 ms.
 // Scores by 4x4x4 products, which have no idle rows for four query heads to a key head: long ones 2% faster, but 58 us (49 then) for the 64 sequences
 // and 20 instead of 16 for 32 of up to 2047, as every lane then lays out a whole query.
-// ALL: for a float32 output.
+// CENTRE: for a float32 output.
 // ALIGNED: pages of whole tiles: a tile lies in one page, its addresses are a scalar and a constant of the lane.
-template <int G, int WAVES, bool ALL, bool ALIGNED, class Q>
+template <int G, int WAVES, bool CENTRE, bool ALIGNED, class Q>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged_u4_kernel(PagedArgs a) {
     using P = ElemF16;
     using B = ElemBF16;
@@ -135,9 +129,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // scalar, and what follows from it
     Line<WAVES, U4_TILE> line;
     line.init(a, reinterpret_cast<int64_t*>(lds));
-    using KeyCodes = Widen8<!ALL, ALL>;
-    const KeyCodes key_codes;
-    const Widen8<false, ALL> value_codes;
+    const Widen8<CENTRE> codes;
     constexpr int STEP = WAVES * U4_TILE;
     const int page = a.page, cols = STEP / page, slots = STEP - cols * page;
     const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
@@ -289,25 +281,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         for (int i = 0; i < OPS; ++i) qsum[i] = u4v{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < G; ++s) {
-            float even = 0.0f, odd = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 const f2v u = unpack2(P{}, q[s][p]);
-                even += u[0];
-                odd += u[1];
+                sum += u[0] + u[1];
             }
 #pragma unroll
             for (int p = 0; p < 4; ++p)  // halves of words p / 2 and p / 2 + 2
                 qf[s][p] = __builtin_amdgcn_perm(q[s][2 + (p >> 1)], q[s][p >> 1], p & 1 ? 0x07060302u : 0x05040100u);
-            even = quarter_sum(even);
-            odd = quarter_sum(odd);
+            sum = quarter_sum(sum);
             // lane group g holds the g-th of three terms of the sum, and of what the codes' offsets add, negative
             auto term = [&](float x) {
                 const float t0 = unpack2(B{}, pack2(B{}, x, 0.0f))[0], r1 = x - t0;
                 const float t1 = unpack2(B{}, pack2(B{}, r1, 0.0f))[0];
                 return g == 0 ? t0 : g == 1 ? t1 : g == 2 ? r1 - t1 : 0.0f;
             };
-            const uint32_t both = pack2(B{}, term(even + odd), term(-(KeyCodes::EVEN * even + KeyCodes::ODD * odd)));
+            const uint32_t both = pack2(B{}, term(sum), term(-codes.ADDED * sum));
             const int at = G <= 4 ? G + s : 8 + s;
             qsum[0][(s >> 1) & 3] |= s & 1 ? both & 0xffff0000u : both >> 16;      // with the scales
             qsum[at >> 3][(at >> 1) & 3] |= at & 1 ? both << 16 : both & 0xffffu;  // with the biases
@@ -373,7 +363,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                     if constexpr (OPS == 2) sc[T] = mfma_16x16x32(B{}, meta[T][1], qsum[1], sc[T]);
 #pragma unroll
                     for (int s = 0; s < G; ++s)
-                        x[T & 1][s] = mfma_16x16x32(P{}, key_codes(code[T][s]), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
+                        x[T & 1][s] = mfma_16x16x32(P{}, codes(code[T][s]), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
                 }
                 if (T > 0) {
 #pragma unroll
@@ -450,29 +440,32 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                 for (int i = 0; i < 4; ++i) sc[T][i] *= up;
             // O^T += C^T P^T: word j of a transposed read holds positions 8 j .. of this lane's 16, pairs four apart
             u4v hi[2], lo[2];
+            float minus = -1.0f;
+            asm("" : "+v"(minus));  // a product with it reads a half of hi as it lies: no conversion
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     const float x = sc[2 * j][p], y = sc[2 * j + 1][p];
                     hi[j][p] = pack2(P{}, x, y);
-                    if constexpr (ALL) {
-                        const f2v u = unpack2(P{}, hi[j][p]);
-                        lo[j][p] = pack2(P{}, x - u[0], y - u[1]);
-                    }
+                    const f2v u = unpack2(P{}, hi[j][p]);
+                    lo[j][p] = pack2(P{}, __builtin_fmaf(u[0], minus, x), __builtin_fmaf(u[1], minus, y));
                 }
             const u4v offset = {0x4de04de0u, 0x4de04de0u, 0x4de04de0u, 0x4de04de0u};  // 23.5
-            if constexpr (!ALL) {
+            if constexpr (!CENTRE) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) ones = mfma_16x16x32(P{}, offset, hi[j], ones);
+                for (int j = 0; j < 2; ++j) {
+                    ones = mfma_16x16x32(P{}, offset, hi[j], ones);
+                    ones = mfma_16x16x32(P{}, offset, lo[j], ones);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const u4v v = value_codes((uint32_t)vcode[d][j]);
+                    const u4v v = codes((uint32_t)vcode[d][j]);
                     o[d] = mfma_16x16x32(P{}, v, hi[j], o[d]);
-                    if constexpr (ALL) o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
+                    o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
                 }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its LDS may be filled again
             if (t + NST < tiles) issue(t + NST);
@@ -500,11 +493,11 @@ void paged_u4_launch(const PagedArgs& a, int q_type, bool few, dim3 grid, hipStr
         auto launch = [&](auto groups, auto waves) {
             constexpr int G = decltype(groups)::value, W = decltype(waves)::value;
             auto all = [&](auto every) {
-                constexpr bool ALL = decltype(every)::value;
+                constexpr bool CENTRE = decltype(every)::value;
                 if (a.page % U4_TILE == 0)
-                    hipLaunchKernelGGL((paged_u4_kernel<G, W, ALL, true, Q>), grid, dim3(64 * W), 0, st, a);
+                    hipLaunchKernelGGL((paged_u4_kernel<G, W, CENTRE, true, Q>), grid, dim3(64 * W), 0, st, a);
                 else
-                    hipLaunchKernelGGL((paged_u4_kernel<G, W, ALL, false, Q>), grid, dim3(64 * W), 0, st, a);
+                    hipLaunchKernelGGL((paged_u4_kernel<G, W, CENTRE, false, Q>), grid, dim3(64 * W), 0, st, a);
             };
             if (a.out_f32) all(std::true_type{});
             else all(std::false_type{});

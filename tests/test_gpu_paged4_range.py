@@ -15,8 +15,9 @@ from test_gpu_paged4 import TYPES, Cache4
 pytestmark = pytest.mark.gpu
 
 
-def _check(cache, q, got, group, scale, out):
-    w_eps, offset = (2.0 ** -22, 16) if out == "float32" else (2.0 ** -11, 256)
+def _check(cache, q, got, group, scale, out, w_eps=None, offset=None):
+    if w_eps is None:
+        w_eps, offset = (2.0 ** -22, 16) if out == "float32" else (2.0 ** -11, 256)
     for b, n in enumerate(cache.lens):
         for h in range(q.shape[1]):
             (kc, ks, kb), (vc, vs, vb) = (tuple(a[:, h // group] for a in cache.rows[b][c]) for c in "kv")
@@ -103,3 +104,31 @@ def test_values_near_the_ends_of_the_range(gpu, dtype, out, page, n, power, offs
         _store(cache, b, np.arange(length))
     q, got = _run(cache, rng, 2, dtype, out, 0.125)
     _check(cache, q, got, 2, 0.125, out)
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("lens,h,hkv,hd,page", [([3, 9, 700, 900], 32, 8, 128, 64), ([4000, 70], 8, 8, 64, 16),
+                                                ([1300, 5000], 12, 3, 96, 32), ([80, 2000], 4, 2, 256, 64)])
+def test_sixteen_bit_outputs_are_rounded_once(gpu, dtype, out, lens, h, hkv, hd, page):
+    """Weights of 22 bits and codes with 16 added for every output type.  Over all outputs of a call the 2-norm of the
+    error is what rounding the exact ones gives, 5% more (some thousand roundings, whose mean square varies by 1 or 2%), and
+    8.4e-6 of the outputs': the float32 outputs' 4e-6 (test_gpu_paged4.py) with terms of 31 scales where those have 15."""
+    rng = np.random.default_rng([hd, page])
+    cache = Cache4(rng, lens, hkv, page, hd)
+    group = h // hkv
+    q, got = _run(cache, rng, h, dtype, out, hd ** -0.5)
+    _check(cache, q, got, group, hd ** -0.5, out, 2.0 ** -22, 16)
+    want = np.array([[cache.attend(b, j, q[b, j], group, hd ** -0.5, 0, 0, 0)[0] for j in range(h)] for b in range(len(lens))])
+    norm = np.linalg.norm
+    alone = norm(rounded(want, out)[0] - want)
+    assert norm(got - want) <= 1.05 * alone + 8.4e-6 * norm(want)
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("n,hd,spread", [(300, 64, 40.0), (3000, 128, 40.0), (2000, 192, 8.0)])
+def test_scores_far_apart(gpu, dtype, out, n, hd, spread):
+    """Attention that a few keys rule, whose scores are large beside what decides between them."""
+    rng = np.random.default_rng([n, hd])
+    cache = Cache4(rng, [n, 100], 1, 64, hd, offset=0.5)
+    q, got = _run(cache, rng, 4, dtype, out, spread * hd ** -0.5)
+    _check(cache, q, got, 4, spread * hd ** -0.5, out, 2.0 ** -22, 16)

@@ -19,12 +19,12 @@ namespace {
 constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_NST = 2;     // tiles on their way
 
-// Weights are 2^(score - base) in log2 units, base the running maximum plus this (a reference in whole numbers: one
-// follows the other by powers of two, which round nothing).  The sums of a million biases of 1e36, or of 4096 of
-// bfloat16's largest, then stay finite, as over the other caches.  The statistics that leave a piece are relative to
-// base itself, so that sums with different references stay comparable however large the scores.
-constexpr float U4_SHIFT = 20.0f;
-__device__ __forceinline__ float u4_reference(float mx) { return (fabsf(mx) < 0x1p22f ? ceilf(mx) : mx) + U4_SHIFT; }
+// Weights are relative to the running maximum, to the next whole number above it in log2 units: one reference then
+// follows another by powers of two, which round nothing, and the exponents of the weights that count stay near 0.  Values'
+// scales and biases, and with them all that leaves a piece, enter times this: the sums of a million values of 1e36, or of 4096
+// of bfloat16's largest, are finite then, as over the other caches.
+constexpr float U4_DOWN = 0x1p-20f;
+__device__ __forceinline__ float u4_reference(float mx) { return fabsf(mx) < 0x1p22f ? ceilf(mx) : mx; }
 // A weight times its value's scale enters a product in fp16, as 2^lift times it: the largest one that a query has met lies
 // between 2^U4_SET and 2^U4_LIMIT then, and what fp16 drops (half its least step) is 2^-35 of it.  The largest
 // product and not the largest scale decides: a row that attention ignores costs the others nothing, whatever its scale.
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         vf4 o[DT], ones = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
-        float base = -INFINITY, l = 0.0f, vbias = 0.0f;
+        float m = -INFINITY, l = 0.0f, vbias = 0.0f;
         int lift = U4_LIFT_MAX;  // this lane's query's
         auto scale_sums = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
@@ -345,10 +345,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are 0
 #pragma unroll
             for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
-            const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) : 0.0f;
+            const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) * U4_DOWN : 0.0f;
             *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = vs;
             *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) =
-                lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16))) : 0.0f;
+                lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16)) * U4_DOWN) : 0.0f;
             asm volatile("" ::: "memory");
             vf4 sc[4], x[2][G], f[2][G];
             auto factors = [&](int T) __attribute__((always_inline)) {
@@ -402,19 +402,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[T][i]);
             mx = quarter_max(mx) * sl2;
-            if (__any(mx > base + (RESCALE_AT - U4_SHIFT))) {
-                const float to = fmaxf(base, u4_reference(mx)), finite = to == -INFINITY ? 0.0f : to;
-                const float corr = __builtin_amdgcn_exp2f(base - finite);
+            if (__any(mx > m + RESCALE_AT)) {
+                const float to = fmaxf(m, u4_reference(mx)), finite = to == -INFINITY ? 0.0f : to;
+                const float corr = __builtin_amdgcn_exp2f(m - finite);
                 // the products' reference stays where it was: what they are multiplied by rises as the weights fall
-                const int higher = min(lift + (int)fminf(finite - base, 1024.0f), U4_LIFT_MAX);
-                const float f = __builtin_amdgcn_exp2f(base - finite + (float)(higher - lift));
+                const int higher = min(lift + (int)fminf(finite - m, 1024.0f), U4_LIFT_MAX);
+                const float f = __builtin_amdgcn_exp2f(m - finite + (float)(higher - lift));
                 lift = higher;
-                base = to;
+                m = to;
                 l *= corr;
                 vbias *= corr;
                 scale_sums(f);
             }
-            const float from = base == -INFINITY ? 0.0f : base;
+            const float from = m == -INFINITY ? 0.0f : m;
             float most = 0.0f;  // the largest weight times its value's scale
 #pragma unroll
             for (int T = 0; T < 4; ++T) {
@@ -474,8 +474,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         // what all dims of a query share: the sum of its values' middles
         const float extra = quarter_sum(vbias);
         Sums<DT, P> sums;
-        sums.m = base;
-        sums.l = l;
+        sums.m = m;
+        sums.l = l * U4_DOWN;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll

@@ -132,3 +132,16 @@ def test_scores_far_apart(gpu, dtype, out, n, hd, spread):
     cache = Cache4(rng, [n, 100], 1, 64, hd, offset=0.5)
     q, got = _run(cache, rng, 4, dtype, out, spread * hd ** -0.5)
     _check(cache, q, got, 4, spread * hd ** -0.5, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,hd", [(300, 64), (300, 128), (3000, 64), (3000, 128)])
+def test_float32_outputs_keep_the_bits_of_the_weights(gpu, dtype, n, hd):
+    """The weights that count have exponents near 0, whose rounding is 2^-25 of a weight and not 2^-20: what is left are
+    some ten roundings to a score of a few units (2^-22 each), alike in the 2-norm: 2^-22 root(10), and as much for the
+    sums: 1.1e-6 at most where all meet."""
+    rng = np.random.default_rng(n + hd)
+    cache = Cache4(rng, [n], 2, 64, hd)
+    q, got = _run(cache, rng, 8, dtype, "float32", hd ** -0.5)
+    want = np.array([cache.attend(0, j, q[0, j], 4, hd ** -0.5, 0, 0, 0)[0] for j in range(8)])
+    assert np.linalg.norm(got[0] - want) <= 1.1e-6 * np.linalg.norm(want)

@@ -860,9 +860,9 @@ int lq_paged_kv_append_rotary(const void* d_q, int64_t ldq, const void* d_k, con
  * whose positions include a page outside [0, pages) or past its table NaN.  max_length is the host's bound of the
  * lengths: the split over the positions is planned from it, and lengths past it are still
  * attended whole, only slower.  hd a multiple of 8, at most 256; scale positive and
- * finite; pages (and the scales of LQ_U4) 16-byte aligned.  Over LQ_U4 a weight times its value's scale enters in
- * 16-bit terms relative to the largest such product that the query meets: what lies 2^-35 below that product is
- * lost.  Workspace: lq_paged_attention_workspace_size bytes (0 where one
+ * finite; pages (and the scales of LQ_U4) 16-byte aligned.  Over LQ_U4 a weight times its value's scale enters as
+ * two 16-bit terms, within 2^-23 of it; what lies 2^-35 below the largest such product that the query meets is lost.
+ * Workspace: lq_paged_attention_workspace_size bytes (0 where one
  * workgroup takes a whole sequence), no contents kept from call to call. */
 size_t lq_paged_attention_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t hd, int64_t max_length);
 int lq_paged_attention(const void* d_q, int q_type, int64_t ldq, int64_t B, int64_t H, int64_t Hkv, int64_t hd,

@@ -30,18 +30,43 @@ __device__ __forceinline__ float u4_reference(float mx) { return fabsf(mx) < 0x1
 // product and not the largest scale decides: a row that attention ignores costs the others nothing, whatever its scale.
 constexpr int U4_SET = 10, U4_LIMIT = 15, U4_LIFT_MAX = 127;
 
-// Eight fp16 values for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in the
-// mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes.  CENTRE: one
-// addition more for c - 7.5.
+// The low half of byte I of a word, a signed number, over 16 in float32 (its bits).
+template <int I>
+__device__ __forceinline__ uint32_t nibble_to_f32(uint32_t w) {
+    uint32_t f;
+#define LQ_NIBBLE(i)                                                                                     \
+    asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_" #i : "=v"(f) : "v"(w))
+    if constexpr (I == 0) LQ_NIBBLE(0);
+    if constexpr (I == 1) LQ_NIBBLE(1);
+    if constexpr (I == 2) LQ_NIBBLE(2);
+    if constexpr (I == 3) LQ_NIBBLE(3);
+#undef LQ_NIBBLE
+    return f;
+}
+
+// Eight values of type E for the codes c of a word, in four registers; pair p holds codes p and p + 4.  A code lies in
+// the mantissa under the exponent that gives it its weight: 16 + c, one shift and one and-or for two codes.  CENTRE: in
+// fp16 one addition more for c - 7.5; in bfloat16, which has none of pairs, (c - 8) / 16 by conversions of a signed nibble.
 // An and-or takes no literal, so mask and exponent are kept in registers whose values the compiler does not see.
-template <bool CENTRE>
+template <class E, bool CENTRE>
 struct Widen8 {
-    static constexpr float ADDED = CENTRE ? -7.5f : 16.0f;  // to a code
+    static constexpr float ADDED = !CENTRE ? 16.0f : E::code == LQ_F16 ? -7.5f : -8.0f;  // to a code
+    static constexpr float TIMES = CENTRE && E::code == LQ_BF16 ? 0.0625f : 1.0f;        // and their sum
     uint32_t mask, exponent;
-    __device__ __forceinline__ Widen8() : mask(0x03c003c0u), exponent(0x4c004c00u) {
-        asm("" : "+v"(mask), "+v"(exponent));
+    __device__ __forceinline__ Widen8()
+        : mask(E::code == LQ_F16 ? 0x03c003c0u : 0x00780078u), exponent(E::code == LQ_F16 ? 0x4c004c00u : 0x41804180u) {
+        asm("" : "+s"(mask), "+v"(exponent));
     }
     __device__ __forceinline__ u4v operator()(uint32_t w) const {
+        if constexpr (E::code == LQ_BF16 && CENTRE) {
+            const uint32_t even = w ^ 0x88888888u, odd = even >> 4;  // two's complement of c - 8
+            auto pair = [](uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); };
+            return u4v{pair(nibble_to_f32<0>(even), nibble_to_f32<2>(even)), pair(nibble_to_f32<0>(odd), nibble_to_f32<2>(odd)),
+                       pair(nibble_to_f32<1>(even), nibble_to_f32<3>(even)), pair(nibble_to_f32<1>(odd), nibble_to_f32<3>(odd))};
+        }
+        if constexpr (E::code == LQ_BF16)
+            return u4v{((w << 3) & mask) | exponent, ((w >> 1) & mask) | exponent, ((w >> 5) & mask) | exponent,
+                       ((w >> 9) & mask) | exponent};
         u4v v = {((w << 6) & mask) | exponent, ((w << 2) & mask) | exponent, ((w >> 2) & mask) | exponent,
                  ((w >> 6) & mask) | exponent};
         if constexpr (CENTRE) {
@@ -89,17 +114,18 @@ struct Place {
 // (l, g) holds the scores and weights of query l at positions 16 g + 4 T + i: row r of the first product's
 // operand T is position 16 (r / 4) + 4 T + r % 4, and the transposing read brings a lane the codes of its dim at just
 // these 16 positions.
-// Both products are fp16.  Queries of bfloat16 enter times a power of two (their largest value between 2^13 and 2^14:
-// fp16 then holds every bit of values down to 2^-27 of it), which goes into the scores' factor.  A weight enters times its
+// Keys' codes meet queries in the queries' type.  Queries of bfloat16 enter times a power of two, which goes into the
+// scores' factor and halves the exponent of their largest: products with keys of the inverse size stay in float32's
+// range, and no dim above 2^-126 of the largest loses a bit.  Values' codes meet weights in fp16.  A weight enters times its
 // value's scale, relative to the largest such product so far (U4_SET), as two terms (within 2^-23 of it); sums and
 // maximum stay float32.
 // A code c enters as 16 + c.  What that adds to a score is taken off where the biases come in: one instruction more
 // multiplies the row's scales and biases, bfloat16 as they are stored, by minus the queries' sums times 16 and by their
 // sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of that, and 7.5 scales more
 // from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
-// A float32 output is worth an addition to every pair of codes: c - 7.5 in both products, so that no sum grows by what is
-// taken off later (2-norm of the error of 300 to 60000 positions 2e-8 to 2e-7 of the output's, with 16 + c 3e-7 to 3e-6,
-// which 16 bits do not show; 64 sequences of up to 8191 positions 53 us where 16-bit outputs take 49).
+// A float32 output is worth codes around 0 in both products (Widen8), so that no sum grows by what is taken off later: 2-norm
+// of the error of 300 to 30000 positions 1.5e-7 to 6e-7 of the output's (bfloat16 keys' codes as 16 + c: 5e-7 to 2e-6),
+// which 16 bits do not show.  64 sequences of up to 8191 positions take 52 us in float32, 47 in fp16.
 // With one term to a weight of a 16-bit output, and 256 + c for half of a key's codes, those took 46 us: the error of
 // fp16 outputs over long sequences was 1.4 times what their rounding alone gives.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
@@ -129,7 +155,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // scalar, and what follows from it
     Line<WAVES, U4_TILE> line;
     line.init(a, reinterpret_cast<int64_t*>(lds));
-    const Widen8<CENTRE> codes;
+    const Widen8<P, CENTRE> value_codes;
+    const auto key_codes = [&] {
+        if constexpr (Q::code == LQ_BF16) return Widen8<Q, CENTRE>{};
+        else return value_codes;
+    }();
     constexpr int STEP = WAVES * U4_TILE;
     const int page = a.page, cols = STEP / page, slots = STEP - cols * page;
     const uint32_t slot = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * SLOT;
@@ -266,14 +296,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             for (int s = 0; s < G; ++s)
 #pragma unroll
                 for (int p = 0; p < 4; ++p) top = max(top, max(q[s][p] & 0x7fffu, (q[s][p] >> 16) & 0x7fffu));
-            const int e = max((int)(__float_as_uint(quarter_max(__uint_as_float(top << 16))) >> 23) - 127, -100);
-            sl2 = ldexpf(sl2, e - 13);
+            // half of the largest value's exponent, where the scores' factor stays above float32's end
+            const int e = max(((int)(__float_as_uint(quarter_max(__uint_as_float(top << 16))) >> 23) - 127) >> 1,
+                              -126 - ((int)(__float_as_uint(sl2) >> 23) - 127));
+            sl2 = __builtin_amdgcn_ldexpf(sl2, e);
+            const float by = __builtin_amdgcn_ldexpf(1.0f / key_codes.TIMES, -e);
 #pragma unroll
             for (int s = 0; s < G; ++s)
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const f2v u = unpack2(B{}, q[s][p]);
-                    q[s][p] = pack2(P{}, ldexpf(u[0], 13 - e), ldexpf(u[1], 13 - e));
+                    const f2v u = unpack2(Q{}, q[s][p]);
+                    q[s][p] = pack2(Q{}, u[0] * by, u[1] * by);
                 }
         }
         u4v qf[G], qsum[OPS];
@@ -284,20 +317,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             float sum = 0.0f;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                const f2v u = unpack2(P{}, q[s][p]);
+                const f2v u = unpack2(Q{}, q[s][p]);
                 sum += u[0] + u[1];
             }
 #pragma unroll
             for (int p = 0; p < 4; ++p)  // halves of words p / 2 and p / 2 + 2
                 qf[s][p] = __builtin_amdgcn_perm(q[s][2 + (p >> 1)], q[s][p >> 1], p & 1 ? 0x07060302u : 0x05040100u);
-            sum = quarter_sum(sum);
+            sum = quarter_sum(sum) * key_codes.TIMES;
             // lane group g holds the g-th of three terms of the sum, and of what the codes' offsets add, negative
             auto term = [&](float x) {
                 const float t0 = unpack2(B{}, pack2(B{}, x, 0.0f))[0], r1 = x - t0;
                 const float t1 = unpack2(B{}, pack2(B{}, r1, 0.0f))[0];
                 return g == 0 ? t0 : g == 1 ? t1 : g == 2 ? r1 - t1 : 0.0f;
             };
-            const uint32_t both = pack2(B{}, term(sum), term(-codes.ADDED * sum));
+            const uint32_t both = pack2(B{}, term(sum), term(-key_codes.ADDED * sum));
             const int at = G <= 4 ? G + s : 8 + s;
             qsum[0][(s >> 1) & 3] |= s & 1 ? both & 0xffff0000u : both >> 16;      // with the scales
             qsum[at >> 3][(at >> 1) & 3] |= at & 1 ? both << 16 : both & 0xffffu;  // with the biases
@@ -363,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                     if constexpr (OPS == 2) sc[T] = mfma_16x16x32(B{}, meta[T][1], qsum[1], sc[T]);
 #pragma unroll
                     for (int s = 0; s < G; ++s)
-                        x[T & 1][s] = mfma_16x16x32(P{}, codes(code[T][s]), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
+                        x[T & 1][s] = mfma_16x16x32(Q{}, key_codes(code[T][s]), qf[s], vf4{0.f, 0.f, 0.f, 0.f});
                 }
                 if (T > 0) {
 #pragma unroll
@@ -463,7 +496,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const u4v v = codes((uint32_t)vcode[d][j]);
+                    const u4v v = value_codes((uint32_t)vcode[d][j]);
                     o[d] = mfma_16x16x32(P{}, v, hi[j], o[d]);
                     o[d] = mfma_16x16x32(P{}, v, lo[j], o[d]);
                 }

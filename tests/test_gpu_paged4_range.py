@@ -145,3 +145,62 @@ def test_float32_outputs_keep_the_bits_of_the_weights(gpu, dtype, n, hd):
     q, got = _run(cache, rng, 8, dtype, "float32", hd ** -0.5)
     want = np.array([cache.attend(0, j, q[0, j], 4, hd ** -0.5, 0, 0, 0)[0] for j in range(8)])
     assert np.linalg.norm(got[0] - want) <= 1.1e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("n,hd,page", [(200, 64, 16), (2500, 128, 64), (90, 256, 128)])
+def test_queries_of_very_different_dims(gpu, dtype, out, n, hd, page):
+    """Groups of dims whose queries are far smaller than the others' and whose keys are far larger: each counts as much
+    as the others (fp16 queries as far as that type goes)."""
+    rng = np.random.default_rng([n, hd])
+    cache = Cache4(rng, [n, 70], 1, page, hd, offset=0.3)
+    groups = hd // 32
+    powers = np.array([0.0, 44.0, -20.0, 60.0, 7.0, -70.0, 30.0, 1.0])[:groups] if dtype == "bfloat16" else \
+        np.array([0.0, 10.0, -3.0, 12.0, 2.0, 5.0, 9.0, 1.0])[:groups]
+    for b, length in enumerate(cache.lens):
+        _, ks, kb = cache.rows[b]["k"]
+        ks *= 2.0 ** powers
+        kb *= 2.0 ** powers
+        _store(cache, b, np.arange(length))
+    import lucid_amd.nn.functional as F
+
+    q, qh = rounded(rng.standard_normal((2, 3, hd)) * np.repeat(2.0 ** -powers, 32), dtype)
+    got = values(F.paged_attention(dev(qh), max_length=n, out_dtype=types()[out], **cache.tensors()))
+    _check(cache, q, got, 3, hd ** -0.5, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("out", ["bfloat16", "float32"])
+@pytest.mark.parametrize("size", [1e-37, 1e-30, 1e30, 1e38])
+@pytest.mark.parametrize("n", [70, 1500])
+def test_queries_of_any_size(gpu, out, size, n):
+    """bfloat16 queries at the ends of the range, a row of zeros among them, keys of the inverse size."""
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(n)
+    cache = Cache4(rng, [n, 70], 1, 16, 64)
+    power = -np.round(np.log2(size))
+    for b, length in enumerate(cache.lens):
+        _, ks, kb = cache.rows[b]["k"]
+        ks *= 2.0 ** power
+        kb *= 2.0 ** power
+        _store(cache, b, np.arange(length))
+    x = rng.uniform(-1, 1, (2, 3, 64)) * 2.0 ** -power
+    x[1, 1] = 0
+    q, qh = rounded(x, "bfloat16")
+    got = values(F.paged_attention(dev(qh), max_length=n, out_dtype=types()[out], **cache.tensors()))
+    _check(cache, q, got, 3, 0.125, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("scale", [1e-45, 1e-38, 1e-12])
+def test_tiny_scales(gpu, dtype, out, scale):
+    """A scale so small that all positions weigh the same, with queries of zeros and of ordinary size."""
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng(3)
+    cache = Cache4(rng, [90, 1100], 1, 16, 64)
+    x = rng.standard_normal((2, 3, 64))
+    x[:, 1] = 0
+    q, qh = rounded(x, dtype)
+    got = values(F.paged_attention(dev(qh), max_length=1100, scale=scale, out_dtype=types()[out], **cache.tensors()))
+    _check(cache, q, got, 3, scale, out, 2.0 ** -22, 16)

@@ -15,10 +15,10 @@ from test_gpu_paged4 import TYPES, Cache4
 pytestmark = pytest.mark.gpu
 
 
-def _check(cache, q, got, group, scale, out, w_eps=None, offset=None):
+def _check(cache, q, got, group, scale, out, w_eps=None, offset=None, skip=0):
     if w_eps is None:
         w_eps, offset = (2.0 ** -22, 16) if out == "float32" else (2.0 ** -11, 256)
-    for b, n in enumerate(cache.lens):
+    for b, n in list(enumerate(cache.lens))[skip:]:
         for h in range(q.shape[1]):
             (kc, ks, kb), (vc, vs, vb) = (tuple(a[:, h // group] for a in cache.rows[b][c]) for c in "kv")
             x = q[b, h].astype(np.float64)

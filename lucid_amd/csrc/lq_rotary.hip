@@ -360,7 +360,8 @@ int paged_append_rotary(const char* name, const void* q, int64_t ldq, const void
     const int lpr = hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
     const int64_t apart = rot / 16;  // lanes between partners: an exchange where that is a power of two
     const int swap = !interleaved && rot > 0 && (apart & (apart - 1)) == 0 ? (int)apart : 0;
-    note_path(vec ? "rotary" : "rotary single");
+    const bool few = tokens * heads < RT_ROWS;
+    note_path(!vec ? "rotary single" : few ? "rotary" : "rotary four rows");
     with_float(src_type, [&](auto s) {
         using S = decltype(s);
         with_half(q_type, [&](auto o) {
@@ -370,7 +371,6 @@ int paged_append_rotary(const char* name, const void* q, int64_t ldq, const void
                     hipLaunchKernelGGL(ak, grid_of(tokens * heads), dim3(64), 0, st, r);
                     return;
                 }
-                const bool few = tokens * heads < RT_ROWS;
                 const int64_t each = RT_T / lpr * (few ? 1 : 4), groups = (heads + each - 1) / each;
                 const dim3 grid = grid_of(tokens * groups);
                 if (few) hipLaunchKernelGGL(one, grid, dim3(RT_T), 0, st, r, lpr, swap, (uint32_t)groups);

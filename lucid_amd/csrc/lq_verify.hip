@@ -136,33 +136,30 @@ struct Weights {
           d(rejected && a.d ? static_cast<const typename E::T*>(a.d) + row * a.ldd : nullptr), lse((double)a.lse[row]),
           dlse(rejected && a.d ? (double)a.dlse[row] : 0.0), vocab(a.vocab), rejected(rejected),
           draft(rejected ? a.drafts[row] : -1) {}
-    template <int N>
-    __device__ __forceinline__ void operator()(int j, double2 (&w)[N]) const {
-        float u[N], v[N];
+    __device__ __forceinline__ void operator()(int j, double2 (&w)[8]) const {
+        float u[8], v[8];
 #pragma unroll
-        for (int i = 0; i < N; ++i) u[i] = v[i] = -INFINITY;
-        if (N == 8 && j + N <= vocab) {
-            if constexpr (N == 8) {
-                load8_any<E>(x + j, u);
-                if (d) load8_any<E>(d + j, v);
-            }
+        for (int i = 0; i < 8; ++i) u[i] = v[i] = -INFINITY;
+        if (j + 8 <= vocab) {
+            load8_any<E>(x + j, u);
+            if (d) load8_any<E>(d + j, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+            for (int i = 0; i < 8; ++i)
                 if (j + i < vocab) {
                     u[i] = E::load(x[j + i]);
                     if (d) v[i] = E::load(d[j + i]);
                 }
         }
-        double p[N];
+        double p[8];
 #pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = exp((double)u[i] - lse);  // -inf past the vocabulary: 0
+        for (int i = 0; i < 8; ++i) p[i] = exp((double)u[i] - lse);  // -inf past the vocabulary: 0
         if (d) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = make_double2(fmax(p[i] - exp((double)v[i] - dlse), 0.0), p[i]);
+            for (int i = 0; i < 8; ++i) w[i] = make_double2(fmax(p[i] - exp((double)v[i] - dlse), 0.0), p[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = make_double2(rejected && j + i != draft ? p[i] : 0.0, p[i]);
+            for (int i = 0; i < 8; ++i) w[i] = make_double2(rejected && j + i != draft ? p[i] : 0.0, p[i]);
         }
     }
 };

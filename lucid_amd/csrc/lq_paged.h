@@ -169,7 +169,9 @@ struct Line {
     // Over 4-bit pages the later of two workgroups on a CU is the slower one: the older waves issue first (even parts ended
     // after 34 and 43 us).  A workgroup of the first half takes 5/8 of the two's steps: long sequences 47.5 -> 44.3 us,
     // 64 of up to 8191 46.8 -> 43.6 (1/2 in whole steps: 47.3 and 45.0, 11/16: 46.8 and 45.7; priorities that
-    // change with every tile: 45.1 and 44.3).
+    // change with every tile: 45.1 and 44.3).  Calls of both kinds, even parts / 5/8: 32 dims 30.5 / 29.0 and 31.2 / 28.8
+    // us, 64 dims 37 / 34.4 and 37.2 / 34.3, 96 dims 46.2 / 43.8 and 43.6 / 41.2, 128 dims 54.2 / 52.9 and 51.3 / 48.8.  That
+    // takes workgroups n and n + groups / 2 to share a CU; where other work holds the CUs the first half end later instead.
     int64_t half, late;  // workgroups of the first half; steps of one of the second
     int64_t base;        // first step of sequence b
     static constexpr bool PAIRS = TILE == 64;  // two workgroups to a CU up to 128 dims

@@ -19,9 +19,9 @@ __device__ __forceinline__ float bf16_at_or_below(float x) {
 
 // A group whose least and largest values are lo and hi; hi = +inf marks one that holds what is not finite.
 // The bias is at or below lo and 15 scales reach hi (to 2^-26 of the width: the product with float32's 1 / 15, which lies
-// above it), so no value is cut; both are rounded to bfloat16 outward, which costs at most 2^-7 of a step and 2^-8 of the
-// bias in resolution.  The product and not the quotient, as float32 programs on this card divide by a constant: where
-// both sides of a rounding are as near, pages filled by either hold the same codes.
+// 2^-24.2 of it above it, is rounded by 2^-24 at most), so no value is cut; both are rounded to bfloat16 outward, which
+// costs at most 2^-7 of a step and 2^-8 of the bias in resolution.  The product is the rule of the pages (a quotient would
+// give the next bfloat16 for widths at the border of two).
 struct Group4 {
     float scale, bias, inv;
     __device__ __forceinline__ Group4(float lo, float hi) {

@@ -19,16 +19,16 @@ namespace {
 constexpr int U4_TILE = 64;   // positions of a wave's tile
 constexpr int U4_NST = 2;     // tiles on their way
 
-// Weights are relative to the running maximum, to the next whole number above it in log2 units: one reference then
-// follows another by powers of two, which round nothing, and the exponents of the weights that count stay near 0.  Values'
-// scales and biases, and with them all that leaves a piece, enter times this: the sums of a million values of 1e36, or of 4096
-// of bfloat16's largest, are finite then, as over the other caches.
-constexpr float U4_DOWN = 0x1p-20f;
-__device__ __forceinline__ float u4_reference(float mx) { return fabsf(mx) < 0x1p22f ? ceilf(mx) : mx; }
-// A weight times its value's scale enters a product in fp16, as 2^lift times it: the largest one that a query has met lies
-// between 2^U4_SET and 2^U4_LIMIT then, and what fp16 drops (half its least step) is 2^-35 of it.  The largest
-// product and not the largest scale decides: a row that attention ignores costs the others nothing, whatever its scale.
-constexpr int U4_SET = 10, U4_LIMIT = 15, U4_LIFT_MAX = 127;
+// What the sums of a wave are relative to, all in whole powers of two, which round nothing:
+// * weights to the running maximum of a query's scores, to the next whole number above it in log2 units (the exponents of
+//   the weights that count stay near 0);
+// * scales and biases to the largest of the wave's values, 2^large.  What leaves the wave is in their own units again, or in
+//   2^U4_DOWN of them for a reference as much higher where they are as large as 2^U4_LARGE: the sums of a million values of
+//   1e36, or of 4096 of bfloat16's largest, are finite then, as over the other caches, and the smallest keep their bits;
+// * a weight times its value's scale, which enters a product in fp16, to the largest one that the query has met: as 2^lift
+//   times it, between 2^U4_SET and 2^U4_LIMIT for the largest; what fp16 drops (half its least step) is 2^-35 of that.  The
+//   largest product and not the largest scale decides: a row that attention ignores costs the others nothing.
+constexpr int U4_LARGE = 80, U4_DOWN = 20, U4_SET = 10, U4_LIMIT = 15;
 
 // The low half of byte I of a word, a signed number, over 16 in float32 (its bits).
 template <int I>
@@ -202,15 +202,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = vf4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.0f, vbias = 0.0f;
-        int lift = U4_LIFT_MAX;  // this lane's query's
-        auto scale_sums = [&](float f) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ones[i] *= f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[d][i] *= f;
-        };
+        int lift = 1024, large = -127;  // of this lane's query: above what any product needs; of the wave
         // this lane's position in the tile that is issued next, and in the one whose page number is fetched next
         int key = first + lane;
         Place at, ahead;
@@ -380,10 +372,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             // codes are finite: a weight of 0 drops what lies past the end once its scale and bias are 0
 #pragma unroll
             for (int s = 0; s < G; ++s) *reinterpret_cast<lds_f32*>(tile + KM + 256 * s + 4 * lane) = ks[s];
-            const float vs = lane < left ? bf16_bits_to_f32((uint16_t)vw) * U4_DOWN : 0.0f;
+            const int mine = lane < left ? (int)(max(vw & 0x7fffu, vw >> 16 & 0x7fffu) >> 7) - 127 : -127;
+            if (__any(mine > large)) {
+                const int to = __builtin_amdgcn_readfirstlane(wave_max(mine));
+                vbias = __builtin_amdgcn_ldexpf(vbias, large - to);
+                lift += to - large;
+                large = to;
+            }
+            const float vs = lane < left ? __builtin_amdgcn_ldexpf(bf16_bits_to_f32((uint16_t)vw), -large) : 0.0f;
             *reinterpret_cast<lds_f32*>(tile + VM + 4 * lane) = vs;
             *reinterpret_cast<lds_f32*>(slot + VBIAS + 4 * lane) =
-                lane < left ? __builtin_fmaf(7.5f, vs, bf16_bits_to_f32((uint16_t)(vw >> 16)) * U4_DOWN) : 0.0f;
+                lane < left ? __builtin_fmaf(7.5f, vs, __builtin_amdgcn_ldexpf(bf16_bits_to_f32((uint16_t)(vw >> 16)), -large)) : 0.0f;
             asm volatile("" ::: "memory");
             vf4 sc[4], x[2][G], f[2][G];
             auto factors = [&](int T) __attribute__((always_inline)) {
@@ -438,16 +437,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[T][i]);
             mx = quarter_max(mx) * sl2;
             if (__any(mx > m + RESCALE_AT)) {
-                const float to = fmaxf(m, u4_reference(mx)), finite = to == -INFINITY ? 0.0f : to;
+                const float to = fmaxf(m, ceilf(mx)), finite = to == -INFINITY ? 0.0f : to;
                 const float corr = __builtin_amdgcn_exp2f(m - finite);
-                // the products' reference stays where it was: what they are multiplied by rises as the weights fall
-                const int higher = min(lift + (int)fminf(finite - m, 1024.0f), U4_LIFT_MAX);
-                const float f = __builtin_amdgcn_exp2f(m - finite + (float)(higher - lift));
-                lift = higher;
+                lift += (int)fminf(finite - m, 4096.0f);  // the products' reference stays where it was
                 m = to;
                 l *= corr;
                 vbias *= corr;
-                scale_sums(f);
             }
             const float from = m == -INFINITY ? 0.0f : m;
             float most = 0.0f;  // the largest weight times its value's scale
@@ -465,14 +460,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
             most = quarter_max(most);
             if (__any(__builtin_amdgcn_ldexpf(most, lift) >= ldexpf(1.0f, U4_LIMIT))) {
                 const int to = min(lift, U4_SET + 127 - (int)(__float_as_uint(most) >> 23));
-                scale_sums(__builtin_amdgcn_ldexpf(1.0f, to - lift));
+                const float f = __builtin_amdgcn_ldexpf(1.0f, to - lift);
                 lift = to;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ones[i] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][i] *= f;
             }
-            const float up = __builtin_amdgcn_ldexpf(1.0f, lift);
 #pragma unroll
             for (int T = 0; T < 4; ++T)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[T][i] *= up;
+                for (int i = 0; i < 4; ++i) sc[T][i] = __builtin_amdgcn_ldexpf(sc[T][i], lift);
             // O^T += C^T P^T: word j of a transposed read holds positions 8 j .. of this lane's 16, pairs four apart
             u4v hi[2], lo[2];
             float minus = -1.0f;
@@ -509,12 +509,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && G > 4 ? 1 : 2) void paged
         // what all dims of a query share: the sum of its values' middles
         const float extra = quarter_sum(vbias);
         Sums<DT, P> sums;
-        sums.m = m;
-        sums.l = l * U4_DOWN;
+        const int down = large >= U4_LARGE && fabsf(m) < 0x1p22f ? U4_DOWN : 0;
+        sums.m = m + (float)down;
+        sums.l = __builtin_amdgcn_ldexpf(l, -down);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums.o[d][i] = __builtin_amdgcn_ldexpf(o[d][i] - ones[0], -lift) + extra;
+            for (int i = 0; i < 4; ++i)
+                sums.o[d][i] = __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(o[d][i] - ones[0], -lift) + extra, large - down);
         paged_finish<false, WAVES, SLOT, DT, Q>(a, w, lds, ml, sums, bad);
     }
     paged_empty<WAVES, Q>(a);

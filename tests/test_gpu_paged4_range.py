@@ -204,3 +204,41 @@ def test_tiny_scales(gpu, dtype, out, scale):
     q, qh = rounded(x, dtype)
     got = values(F.paged_attention(dev(qh), max_length=1100, scale=scale, out_dtype=types()[out], **cache.tensors()))
     _check(cache, q, got, 3, scale, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,hd,page", [(640, 64, 16), (3000, 128, 64)])
+@pytest.mark.parametrize("power", [-114, -60, 0, 60, 100])
+def test_values_of_any_size_keep_their_bits(gpu, dtype, n, hd, page, power):
+    """The 2-norm of a float32 output's error is the same part of the output, however small or large the values: the 4e-6
+    of test_gpu_paged4.py."""
+    rng = np.random.default_rng([n, hd])
+    cache = Cache4(rng, [n], 2, page, hd)
+    _, vs, vb = cache.rows[0]["v"]
+    vs *= 2.0 ** power
+    vb *= 2.0 ** power
+    _store(cache, 0, np.arange(n))
+    q, got = _run(cache, rng, 4, dtype, "float32", hd ** -0.5)
+    want = np.array([cache.attend(0, j, q[0, j], 2, hd ** -0.5, 0, 0, 0)[0] for j in range(4)])
+    assert np.linalg.norm(got[0] - want) <= 4e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype,out", [("float16", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("n", [200, 3000, 9000])
+@pytest.mark.parametrize("first", [0, 150, 2900])
+def test_large_values_from_some_position_on(gpu, dtype, out, n, first):
+    """Values of 2^100 after ones of 2^60, their scores as much lower, so that both count."""
+    if first >= n:
+        first = n - 20
+    rng = np.random.default_rng([n, first])
+    cache = Cache4(rng, [n, 40], 1, 64, 64)
+    (kc, ks, kb), (vc, vs, vb) = (cache.rows[0][c] for c in "kv")
+    vs *= 2.0 ** 60
+    vb *= 2.0 ** 60
+    pos = np.arange(first, n, 7)
+    kc[pos], ks[pos], kb[pos] = 0, 0, -3.5  # some 28 below the others
+    vs[pos] *= 2.0 ** 40
+    vb[pos] *= 2.0 ** 40
+    _store(cache, 0, np.arange(n))
+    q, got = _run(cache, rng, 2, dtype, out, 0.125, positive=True)
+    _check(cache, q, got, 2, 0.125, out, 2.0 ** -22, 16)

@@ -124,8 +124,9 @@ struct Place {
 // sums, in three bfloat16 terms each (24 bits).  An output gets 16 + c less 23.5, by a row of that, and 7.5 scales more
 // from the biases: the rounding of a weight then meets codes around 0, not around 7.5.
 // A float32 output is worth codes around 0 in both products (Widen8), so that no sum grows by what is taken off later: 2-norm
-// of the error of 300 to 30000 positions 1.5e-7 to 6e-7 of the output's (bfloat16 keys' codes as 16 + c: 5e-7 to 2e-6),
-// which 16 bits do not show.  64 sequences of up to 8191 positions take 52 us in float32, 47 in fp16.
+// of the error of 300 to 131071 positions 1.2e-7 to 6e-7 of the output's (bfloat16 keys' codes as 16 + c: 5e-7 to 2e-6).
+// With 16 + c in both it is 3e-5 at 131071 positions, whose values cancel: 1.01 times what rounding alone gives an fp16
+// output.  64 sequences of up to 8191 positions take 52 us in float32, 47 in fp16.
 // With one term to a weight of a 16-bit output, and 256 + c for half of a key's codes, those took 46 us: the error of
 // fp16 outputs over long sequences was 1.4 times what their rounding alone gives.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for

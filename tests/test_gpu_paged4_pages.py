@@ -61,3 +61,38 @@ def test_sizes_far_from_one(gpu, dtype, out, size, page):
     scale = 0.125 / size
     got = values(F.paged_attention(dev(qh), max_length=1400, scale=scale, out_dtype=types()[out], **cache.tensors()))
     _check(cache, q, got, 2, scale, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("page", [3, 100, 320, 5000])
+@pytest.mark.parametrize("lens", [[90, 256, 640], [4000, 1, 999]])
+@pytest.mark.parametrize("hd,dtype", [(64, "float16"), (128, "bfloat16"), (160, "float16")])
+def test_pages_of_any_length(gpu, page, lens, hd, dtype):
+    """Pages that end inside a tile, that hold several tiles, that hold whole sequences."""
+    import lucid_amd.nn.functional as F
+
+    rng = np.random.default_rng([page, hd])
+    cache = Cache4(rng, lens, 1, page, hd)
+    q, qh = rounded(rng.standard_normal((3, 2, hd)), dtype)
+    for out in (dtype, "float32"):
+        got = values(F.paged_attention(dev(qh), max_length=max(lens), out_dtype=types()[out], **cache.tensors()))
+        _check(cache, q, got, 2, hd ** -0.5, out, 2.0 ** -22, 16)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_queries_at_any_address(gpu, dtype):
+    """Rows of queries that 16-byte reads do not fit."""
+    import lucid_amd as L
+    from lucid_amd import _C
+
+    rng = np.random.default_rng(1)
+    cache = Cache4(rng, [90, 1500], 2, 16, 64)
+    ld = 4 * 64 + 3
+    x, host = rounded(rng.standard_normal((2, ld)), dtype)
+    t, rows, out = cache.tensors(), dev(host), L.empty((2, 4, 64), L.float32, "gpu")
+    size = _C.lib().lq_paged_attention_workspace_size(2, 4, 2, 64, 1500)
+    ws = L.empty((size,), np.uint8, "gpu")
+    _C.call("lq_paged_attention", rows.data_ptr(), _C.F16 if dtype == "float16" else _C.BF16, ld, 2, 4, 2, 64,
+            t["k_pages"].data_ptr(), t["v_pages"].data_ptr(), _C.U4, t["k_scale"].data_ptr(), t["v_scale"].data_ptr(),
+            cache.p.pages, 16, t["table"].data_ptr(), t["table"].shape[1], t["lengths"].data_ptr(), 1500, 0.125,
+            out.data_ptr(), _C.F32, ws.data_ptr(), size, None)
+    _check(cache, x[:, :256].reshape(2, 4, 64), out.numpy(), 2, 0.125, "float32", 2.0 ** -22, 16)

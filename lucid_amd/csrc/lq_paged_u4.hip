@@ -131,10 +131,10 @@ struct Place {
 // fp16 outputs over long sequences was 1.4 times what their rounding alone gives.
 // A tile comes to the wave's LDS by copies of codes, scales, biases and the page numbers of a later tile; the wave waits for
 // the older of two tiles alone.
-// 1.47 million positions and key heads of 128 dims (218 MB, 31 us of reading): 48 us and 4.9 for the join.  No unit is
+// 1.47 million positions and key heads of 128 dims (218 MB, 31 us of reading): 51 us and 5.1 for the join.  No unit is
 // full: a workgroup's first tile comes after 8.3 us in the median, 14.2 at most (the plan, the page numbers, the copies:
-// none of which can be earlier than the one before), the vector unit is busy 53% of the time, the matrix cores 16%, and
-// the waves, two to a SIMD, wait 23% of theirs.  64 sequences of up to 8191 (172 MB): 47 us and 6.1, of which
+// none of which can be earlier than the one before), the vector unit is busy 55% of the time, the matrix cores 17%, and
+// the waves, two to a SIMD, wait 23% of theirs.  64 sequences of up to 8191 (172 MB): 47 us and 5.8, of which
 // workgroups' second pieces cost a fifth.  Products on vector instructions, a key to a lane: 98 and 6.4 ms.
 // Scores by 4x4x4 products, which have no idle rows for four query heads to a key head, in an earlier form: long
 // ones 2% faster, but 58 instead of 49 us for the 64 sequences and 20 instead of 16 for 32 of up to 2047, as every lane
